@@ -39,7 +39,7 @@ enum {
   MAGI_E_CUDA = -8      /* a CUDA runtime / driver call failed                                 */
 };
 
-enum { MAGI_DTYPE_BF16 = 0, MAGI_DTYPE_FP8_E4M3 = 1, MAGI_DTYPE_F32 = 2 };
+enum { MAGI_DTYPE_BF16 = 0, MAGI_DTYPE_FP8_E4M3 = 1, MAGI_DTYPE_F32 = 2, MAGI_DTYPE_F16 = 3 };
 enum { MAGI_NORM_LAYERNORM_1P = 0, MAGI_NORM_RMSNORM_1P = 1, MAGI_NORM_NONE = 2 /* magi_linear_qk_norm_rope_fwd only */ };
 
 typedef struct magi_ctx magi_ctx;
@@ -379,6 +379,107 @@ MAGI_API int magi_ulysses_create(magi_ctx* ctx, const void* id128, int rank, int
 MAGI_API int magi_ulysses_destroy(magi_ulysses* u);
 MAGI_API int magi_ulysses_a2a_in(magi_ulysses* u, const void* send, void* recv, int64_t row_bytes, void* stream);
 MAGI_API int magi_ulysses_a2a_out(magi_ulysses* u, const void* full, void* recv, int64_t row_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------------------------
+ * Token-paged 8-bit cache.  Unlike magi_kv_cache (one page = one chunk of video tokens, book-kept on the host) its pages
+ * hold a few tokens of a SEQUENCE and all of its book-keeping lives on the device, so that a step which appends one
+ * token to every sequence of a batch - or forks, copies, frees and compacts sequences - can be captured in a CUDA graph.
+ * No reference counterpart (the reference caches whole chunks only, inference/model/dit/dit_module.py:800-931).
+ *
+ * The memory belongs to the caller; this struct is a view of it (host struct, read during the call only):
+ *   k8, v8           e4m3 [n_layers, n_pages, n_kv_heads, page_tokens, 128], 16-byte aligned, finite wherever not written
+ *   k_scale, v_scale fp32 [n_layers, n_pages, n_kv_heads]: value = code * scale, scale a power of two in [2^-60, 2^60]
+ *   page_table       int32 [max_seqs, max_pages_per_seq], -1 = no page
+ *   seq_lens         int32 [max_seqs]
+ *   page_refs        int32 [n_pages]: sequences that hold the page, 0 = free
+ *   workspace        magi_token_cache_workspace_bytes() bytes of the cache's own scratch, 16-byte aligned
+ * page_tokens is 16, 32, 64 or 128.  One page id names the page of that number in every layer.  Index arguments (seqs,
+ * starts, ...) are int32 device arrays of n <= 1024 entries.  Calls on one cache must be stream-ordered, except that
+ * appends and attention of different layers may overlap.
+ * A book-keeping call (reserve, branch, free, compact) happens whole or not at all: an index out of range, a sequence
+ * named twice, a sequence that would exceed its table row (MAGI_E_RANGE) or too few free pages (MAGI_E_NOMEM) leave the
+ * cache as it was and set the context's device status word (magi_ctx_status).  New pages are the lowest-numbered free
+ * ones, in the order of the entries.
+ */
+typedef struct {
+  uint32_t struct_size;
+  int32_t n_layers, n_pages, page_tokens, n_kv_heads, max_seqs, max_pages_per_seq;
+  void* k8;
+  void* v8;
+  float* k_scale;
+  float* v_scale;
+  int32_t* page_table;
+  int32_t* seq_lens;
+  int32_t* page_refs;
+  void* workspace;
+} magi_token_cache;
+MAGI_API int64_t magi_token_cache_workspace_bytes(int32_t n_pages);
+/* Appends room for n_new[i] tokens to sequence seqs[i]: takes the pages, advances seq_lens and writes the position of the
+ * first new token to starts[i] (-1 for every entry of a refused call). */
+MAGI_API int magi_token_cache_reserve(magi_ctx* ctx, const magi_token_cache* c, const int32_t* seqs, const int32_t* n_new,
+                                      int n, int32_t* starts, void* stream);
+/* Quantises new tokens into their pages in one layer.  k, v: bf16 [total_new, n_kv_heads, 128] (strides in elements);
+ * entry i owns rows [cu_new[i], cu_new[i+1]), at most max_new of them (cu_new NULL: one row each), which go to positions
+ * starts[i], starts[i] + 1, ... of sequence seqs[i]; a negative start skips the entry.  The scale of a (page, head) is the
+ * smallest power of two that keeps its finite values within +-448; tokens that the page already holds are re-quantised
+ * when it grows.  NaN stays NaN, infinities saturate.  An entry that does not lie inside its sequence, and a page that
+ * other sequences share, is left alone and sets the status word to MAGI_E_RANGE. */
+MAGI_API int magi_token_cache_append(magi_ctx* ctx, const magi_token_cache* c, int layer, const int32_t* seqs,
+                                     const int32_t* starts, const int32_t* cu_new, int n, int max_new, int total_new,
+                                     const void* k, int64_t k_stride_t, int64_t k_stride_h, const void* v,
+                                     int64_t v_stride_t, int64_t v_stride_h, void* stream);
+/* Makes the empty sequences dst[i] equal to src[i].  share != 0 (fork): full pages are shared, a page that is not full is
+ * copied; share == 0 (copy): every page is copied.  A src may repeat; it must not be a dst of the same call. */
+MAGI_API int magi_token_cache_branch(magi_ctx* ctx, const magi_token_cache* c, const int32_t* src, const int32_t* dst, int n,
+                                     int share, void* stream);
+/* Empties sequences; pages that nobody holds any more become free. */
+MAGI_API int magi_token_cache_free(magi_ctx* ctx, const magi_token_cache* c, const int32_t* seqs, int n, void* stream);
+/* Moves the pages in use to the lowest numbers: the i-th page in use beyond their count goes to the i-th free one below. */
+MAGI_API int magi_token_cache_compact(magi_ctx* ctx, const magi_token_cache* c, void* stream);
+
+/* Attention over the token-paged cache, for one new token per sequence up to whole prompts.  Query row r of sequence
+ * entry i (rows [cu_q[i], cu_q[i+1]) of q, at most max_q; cu_q NULL: one row each) stands at position
+ * p = seq_lens[seqs[i]] - n_q + r and sees the cached positions < seq_lens that are <= p (causal) and > p - window
+ * (window > 0): out = softmax(scale q k^T) v in fp32, head h reading kv head h / (n_q_heads / n_kv_heads).  A row that sees
+ * nothing is zero with lse = -inf; rows of q that no entry owns are not written. */
+typedef struct {
+  uint32_t struct_size;
+  int32_t layer;
+  const void* q;                 /* bf16 [total_q, n_q_heads, 128]; 16-byte aligned, strides in elements, multiples of 8 */
+  int64_t q_stride_t, q_stride_h;
+  void* out;                     /* bf16 [total_q, n_q_heads, 128]                                       */
+  int64_t o_stride_t, o_stride_h;
+  float* lse;                    /* fp32 [total_q, n_q_heads] natural-log-sum-exp, or NULL               */
+  const int32_t* seqs;           /* device int32 [n]; an entry may repeat                                */
+  const int32_t* cu_q;           /* device int32 [n + 1], or NULL                                        */
+  int32_t n, total_q, max_q, n_q_heads;
+  float softmax_scale;           /* <= 0: 1/sqrt(128)                                                    */
+  int32_t causal, window;
+  void* workspace;               /* magi_paged_attn_workspace_bytes() bytes, 16-byte aligned, this call's own */
+} magi_paged_attn_params;
+MAGI_API int64_t magi_paged_attn_workspace_bytes(magi_ctx* ctx, int32_t max_q, int32_t n_q_heads, int32_t n_kv_heads);
+MAGI_API int magi_paged_attn_fwd(magi_ctx* ctx, const magi_token_cache* c, const magi_paged_attn_params* p, void* stream);
+
+/* Rotary embedding by position: channel pairs (i, i + rot_dim/2) ("half") or (2i, 2i + 1) ("interleaved") of the first
+ * rot_dim channels are turned by positions[t] * inv_freq[i] and multiplied by mscale; the other channels are copied.
+ * inverse != 0 turns backwards: the transposed operator, i.e. the gradient of the forward one.  The angle is formed in
+ * 64 bits and reduced to one turn before it is rounded, so far positions keep their phase.  out may be x (same strides).
+ * The table-driven rotary of the DiT (half layout, fused with the norm) is magi_qk_norm_rope_fwd. */
+typedef struct {
+  uint32_t struct_size;
+  int32_t dtype;                 /* MAGI_DTYPE_BF16, MAGI_DTYPE_F16 or MAGI_DTYPE_F32                    */
+  const void* x;                 /* [T, H, head_dim], last dim contiguous; strides in elements           */
+  int64_t x_stride_t, x_stride_h;
+  void* out;
+  int64_t out_stride_t, out_stride_h;
+  const void* positions;         /* device int32 or int64 [T]                                            */
+  int32_t positions_are_int64;
+  int32_t T, H, head_dim, rot_dim;
+  int32_t interleaved, inverse;
+  float mscale;
+  const double* inv_freq;        /* device fp64 [rot_dim / 2]: radians per position                      */
+} magi_rotary_params;
+MAGI_API int magi_rotary_fwd(magi_ctx* ctx, const magi_rotary_params* p, void* stream);
 
 #ifdef __cplusplus
 }

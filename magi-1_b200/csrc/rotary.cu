@@ -1,0 +1,173 @@
+// Rotary embedding by position, both channel layouts, on the first rot_dim channels of a head, forward and transposed:
+//     (a, b) -> mscale * (a cos - b sin, b cos + a sin),  angle = positions[t] * inv_freq[i]
+// Memory-bound: each element is read once and written once in 16-byte pieces.  A block takes a group of tokens, forms the
+// group's cosines and sines once in shared memory (64-bit product, reduced to a fraction of a turn before it becomes fp32:
+// at position 10^6 a 32-bit product alone would be 0.03 radians off) and applies them to every head.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace magi {
+
+constexpr int kRotThreads = 256;
+constexpr int kRotAngles = 2048;  // angles a block holds: 16 KB
+
+struct RotaryKernelParams {
+  const void* x;
+  void* out;
+  int64_t x_st, x_sh, o_st, o_sh;
+  const void* positions;
+  int pos64;
+  int T, H, dim, half;
+  int group;            // tokens of a block
+  int heads_per_block;
+  int inverse;
+  float mscale;
+  const double* inv_freq;
+};
+
+template <class E>
+__device__ __forceinline__ float to_f(E v);
+template <>
+__device__ __forceinline__ float to_f(float v) { return v; }
+template <>
+__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+template <>
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <class E>
+__device__ __forceinline__ E from_f(float v);
+template <>
+__device__ __forceinline__ float from_f(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_f(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __float2bfloat16_rn(v); }
+
+template <class E, int V>
+struct alignas(sizeof(E) * V) Piece {
+  E v[V];
+};
+
+// A unit is V channels of "half"'s first part with their V partners, or V consecutive channels of the interleaved layout,
+// or V channels behind rot_dim that are copied.  V = 1 is the form for odd sizes and unaligned views (interleaved: one pair).
+template <class E, int V, bool kInterleaved>
+__global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotaryKernelParams p) {
+  __shared__ float2 cs[kRotAngles];
+  const int t0 = blockIdx.x * p.group;
+  const int nt = min(p.group, p.T - t0);
+  for (int i = threadIdx.x; i < nt * p.half; i += kRotThreads) {
+    const int t = i / p.half, c = i - t * p.half;
+    const double pos = p.pos64 ? (double)__ldg(reinterpret_cast<const long long*>(p.positions) + t0 + t)
+                               : (double)__ldg(reinterpret_cast<const int*>(p.positions) + t0 + t);
+    const double turns = pos * (__ldg(p.inv_freq + c) * 0.15915494309189535);  // 1 / (2 pi)
+    float s, co;
+    sincospif(2.0f * (float)(turns - rint(turns)), &s, &co);
+    cs[i] = make_float2(co * p.mscale, (p.inverse ? -s : s) * p.mscale);
+  }
+  __syncthreads();
+  constexpr int kStep = kInterleaved && V == 1 ? 2 : V;  // channels that a rotated unit covers in its first part
+  const int rot_units = kInterleaved ? 2 * p.half / kStep : p.half / kStep;
+  const int units = rot_units + (p.dim - 2 * p.half) / V;
+  const int h0 = blockIdx.y * p.heads_per_block, nh = min(p.heads_per_block, p.H - h0);
+  const int total = nt * nh * units;
+  for (int u = threadIdx.x; u < total; u += kRotThreads) {
+    const int th = u / units, k = u - th * units;
+    const int t = th / nh, h = h0 + th - t * nh;
+    const E* x = static_cast<const E*>(p.x) + (int64_t)(t0 + t) * p.x_st + (int64_t)h * p.x_sh;
+    E* o = static_cast<E*>(p.out) + (int64_t)(t0 + t) * p.o_st + (int64_t)h * p.o_sh;
+    const float2* a = cs + t * p.half;
+    if (k >= rot_units) {
+      const int c = 2 * p.half + (k - rot_units) * V;
+      *reinterpret_cast<Piece<E, V>*>(o + c) = *reinterpret_cast<const Piece<E, V>*>(x + c);
+    } else if constexpr (!kInterleaved) {
+      const int c = k * V;
+      Piece<E, V> lo = *reinterpret_cast<const Piece<E, V>*>(x + c), hi = *reinterpret_cast<const Piece<E, V>*>(x + p.half + c);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float2 r = a[c + i];
+        const float l = to_f(lo.v[i]), g = to_f(hi.v[i]);
+        lo.v[i] = from_f<E>(l * r.x - g * r.y);
+        hi.v[i] = from_f<E>(g * r.x + l * r.y);
+      }
+      *reinterpret_cast<Piece<E, V>*>(o + c) = lo;
+      *reinterpret_cast<Piece<E, V>*>(o + p.half + c) = hi;
+    } else if constexpr (V == 1) {
+      const float2 r = a[k];
+      const float l = to_f(x[2 * k]), g = to_f(x[2 * k + 1]);
+      o[2 * k] = from_f<E>(l * r.x - g * r.y);
+      o[2 * k + 1] = from_f<E>(g * r.x + l * r.y);
+    } else {
+      const int c = k * V;
+      Piece<E, V> w = *reinterpret_cast<const Piece<E, V>*>(x + c);
+#pragma unroll
+      for (int i = 0; i < V; i += 2) {
+        const float2 r = a[(c + i) / 2];
+        const float l = to_f(w.v[i]), g = to_f(w.v[i + 1]);
+        w.v[i] = from_f<E>(l * r.x - g * r.y);
+        w.v[i + 1] = from_f<E>(g * r.x + l * r.y);
+      }
+      *reinterpret_cast<Piece<E, V>*>(o + c) = w;
+    }
+  }
+}
+
+template <class E>
+static void launch_rotary(const RotaryKernelParams& k, bool vec, bool inter, dim3 grid, cudaStream_t st) {
+  constexpr int V = 16 / sizeof(E);
+  if (vec) {
+    if (inter) rotary_kernel<E, V, true><<<grid, kRotThreads, 0, st>>>(k);
+    else rotary_kernel<E, V, false><<<grid, kRotThreads, 0, st>>>(k);
+  } else {
+    if (inter) rotary_kernel<E, 1, true><<<grid, kRotThreads, 0, st>>>(k);
+    else rotary_kernel<E, 1, false><<<grid, kRotThreads, 0, st>>>(k);
+  }
+}
+
+}  // namespace magi
+
+extern "C" int magi_rotary_fwd(magi_ctx* ctx, const magi_rotary_params* p, void* stream) {
+  using namespace magi;
+  if (!ctx) return MAGI_E_BADARG;
+  if (!p || p->struct_size != sizeof(magi_rotary_params)) return set_err(ctx, MAGI_E_BADARG, "rotary: bad struct_size");
+  if (p->dtype != MAGI_DTYPE_BF16 && p->dtype != MAGI_DTYPE_F16 && p->dtype != MAGI_DTYPE_F32)
+    return set_err(ctx, MAGI_E_BADARG, "rotary: dtype is bf16, fp16 or fp32");
+  if (p->T < 0 || p->H <= 0 || p->head_dim <= 0 || p->rot_dim < 0 || p->rot_dim > p->head_dim || p->rot_dim % 2)
+    return set_err(ctx, MAGI_E_BADARG, "rotary: bad shape (rot_dim must be even and at most head_dim)");
+  if (p->rot_dim / 2 > kRotAngles) return set_err(ctx, MAGI_E_BADARG, "rotary: rot_dim above %d", 2 * kRotAngles);
+  if (p->T == 0) return MAGI_OK;
+  if (!p->x || !p->out || !p->positions || (p->rot_dim > 0 && !p->inv_freq)) return set_err(ctx, MAGI_E_BADARG, "rotary: null tensor");
+  const int esz = p->dtype == MAGI_DTYPE_F32 ? 4 : 2;
+  const int V = 16 / esz;
+  if ((reinterpret_cast<uintptr_t>(p->x) | reinterpret_cast<uintptr_t>(p->out)) % esz)
+    return set_err(ctx, MAGI_E_ALIGN, "rotary: x and out must be aligned to their type");
+  // 16-byte pieces wherever every row, both parts of a head and the tail start on one; single channels otherwise
+  const bool vec = !((reinterpret_cast<uintptr_t>(p->x) | reinterpret_cast<uintptr_t>(p->out)) & 15) && p->x_stride_t % V == 0 &&
+                   p->x_stride_h % V == 0 && p->out_stride_t % V == 0 && p->out_stride_h % V == 0 && p->head_dim % V == 0 &&
+                   p->rot_dim % (p->interleaved ? V : 2 * V) == 0;
+  RotaryKernelParams k = {p->x, p->out, p->x_stride_t, p->x_stride_h, p->out_stride_t, p->out_stride_h, p->positions,
+                          p->positions_are_int64, p->T, p->H, p->head_dim, p->rot_dim / 2, 1, p->H, p->inverse, p->mscale, p->inv_freq};
+  // tokens of a block: enough work for its threads, no more angles than it holds
+  const int64_t per_token = (int64_t)p->H * p->head_dim / (vec ? V : 1);
+  int64_t group = (4 * kRotThreads + per_token - 1) / per_token;
+  if (k.half > 0 && group > kRotAngles / k.half) group = kRotAngles / k.half;
+  if (group > p->T) group = p->T;
+  k.group = (int)group;
+  const int64_t bx = ((int64_t)p->T + group - 1) / group;
+  // few tokens: the heads are split over blocks, each of which forms the angles again
+  int by = 1;
+  while (bx * by < ctx->sm_count && by * 2 <= p->H && group * per_token / (by * 2) >= kRotThreads) by *= 2;
+  k.heads_per_block = (p->H + by - 1) / by;
+  const dim3 grid((unsigned)bx, (unsigned)((p->H + k.heads_per_block - 1) / k.heads_per_block));
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  int prev = 0;
+  cudaGetDevice(&prev);
+  if (prev != ctx->device) cudaSetDevice(ctx->device);
+  if (p->dtype == MAGI_DTYPE_F32) launch_rotary<float>(k, vec, p->interleaved, grid, st);
+  else if (p->dtype == MAGI_DTYPE_F16) launch_rotary<__half>(k, vec, p->interleaved, grid, st);
+  else launch_rotary<__nv_bfloat16>(k, vec, p->interleaved, grid, st);
+  const cudaError_t e = cudaGetLastError();
+  if (prev != ctx->device) cudaSetDevice(prev);
+  if (e != cudaSuccess) return set_err(ctx, MAGI_E_CUDA, "rotary launch failed: %s", cudaGetErrorString(e));
+  return MAGI_OK;
+}

@@ -10,7 +10,7 @@ LIB_PATH = os.path.join(_HERE, "libmagi_attn.so")
 
 MAGI_OK = 0
 E_BADARG, E_ALIGN, E_ARCH, E_RANGE, E_NOMEM, E_NCCL, E_TIMEOUT, E_CUDA = -1, -2, -3, -4, -5, -6, -7, -8
-DTYPE_BF16, DTYPE_FP8_E4M3, DTYPE_F32 = 0, 1, 2
+DTYPE_BF16, DTYPE_FP8_E4M3, DTYPE_F32, DTYPE_F16 = 0, 1, 2, 3
 NORM_LAYERNORM_1P, NORM_RMSNORM_1P, NORM_NONE = 0, 1, 2
 
 EXPORTS = [
@@ -21,6 +21,9 @@ EXPORTS = [
     "magi_peer_alloc", "magi_peer_open", "magi_peer_close", "magi_peer_free", "magi_selftest_bounded_wait",
     "magi_bias_modulate_add", "magi_div_clamp_to_e4m3", "magi_linear_qk_norm_rope_fwd", "magi_linear_qkv_norm_rope_fwd",
     "magi_ulysses_unique_id", "magi_ulysses_create", "magi_ulysses_destroy", "magi_ulysses_a2a_in", "magi_ulysses_a2a_out",
+    "magi_token_cache_workspace_bytes", "magi_token_cache_reserve", "magi_token_cache_append", "magi_token_cache_branch",
+    "magi_token_cache_free", "magi_token_cache_compact", "magi_paged_attn_workspace_bytes", "magi_paged_attn_fwd",
+    "magi_rotary_fwd",
 ]
 
 
@@ -92,6 +95,38 @@ class ModulateParams(C.Structure):
     ]
 
 
+class TokenCache(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32),
+        ("n_layers", C.c_int32), ("n_pages", C.c_int32), ("page_tokens", C.c_int32), ("n_kv_heads", C.c_int32),
+        ("max_seqs", C.c_int32), ("max_pages_per_seq", C.c_int32),
+        ("k8", C.c_void_p), ("v8", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+        ("page_table", C.c_void_p), ("seq_lens", C.c_void_p), ("page_refs", C.c_void_p), ("workspace", C.c_void_p),
+    ]
+
+
+class PagedAttnParams(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("layer", C.c_int32),
+        ("q", C.c_void_p), ("q_stride_t", C.c_int64), ("q_stride_h", C.c_int64),
+        ("out", C.c_void_p), ("o_stride_t", C.c_int64), ("o_stride_h", C.c_int64),
+        ("lse", C.c_void_p), ("seqs", C.c_void_p), ("cu_q", C.c_void_p),
+        ("n", C.c_int32), ("total_q", C.c_int32), ("max_q", C.c_int32), ("n_q_heads", C.c_int32),
+        ("softmax_scale", C.c_float), ("causal", C.c_int32), ("window", C.c_int32), ("workspace", C.c_void_p),
+    ]
+
+
+class RotaryParams(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("dtype", C.c_int32),
+        ("x", C.c_void_p), ("x_stride_t", C.c_int64), ("x_stride_h", C.c_int64),
+        ("out", C.c_void_p), ("out_stride_t", C.c_int64), ("out_stride_h", C.c_int64),
+        ("positions", C.c_void_p), ("positions_are_int64", C.c_int32),
+        ("T", C.c_int32), ("H", C.c_int32), ("head_dim", C.c_int32), ("rot_dim", C.c_int32),
+        ("interleaved", C.c_int32), ("inverse", C.c_int32), ("mscale", C.c_float), ("inv_freq", C.c_void_p),
+    ]
+
+
 def _load():
     if not os.path.exists(LIB_PATH):
         raise ImportError(
@@ -127,6 +162,15 @@ def _load():
         "magi_chunk_attn_fwd_noalloc": (C.c_int, [C.POINTER(AttnParams), vp, vp, C.c_char_p, i32]),
         "magi_bias_modulate_add": (C.c_int, [vp, C.POINTER(ModulateParams), vp]),
         "magi_div_clamp_to_e4m3": (C.c_int, [vp, vp, i64, i32, i32, vp, i32, vp, i64, vp]),
+        "magi_token_cache_workspace_bytes": (C.c_int64, [i32]),
+        "magi_token_cache_reserve": (C.c_int, [vp, C.POINTER(TokenCache), vp, vp, i32, vp, vp]),
+        "magi_token_cache_append": (C.c_int, [vp, C.POINTER(TokenCache), i32, vp, vp, vp, i32, i32, i32, vp, i64, i64, vp, i64, i64, vp]),
+        "magi_token_cache_branch": (C.c_int, [vp, C.POINTER(TokenCache), vp, vp, i32, i32, vp]),
+        "magi_token_cache_free": (C.c_int, [vp, C.POINTER(TokenCache), vp, i32, vp]),
+        "magi_token_cache_compact": (C.c_int, [vp, C.POINTER(TokenCache), vp]),
+        "magi_paged_attn_workspace_bytes": (C.c_int64, [vp, i32, i32, i32]),
+        "magi_paged_attn_fwd": (C.c_int, [vp, C.POINTER(TokenCache), C.POINTER(PagedAttnParams), vp]),
+        "magi_rotary_fwd": (C.c_int, [vp, C.POINTER(RotaryParams), vp]),
         "magi_peer_alloc": (C.c_int, [vp, C.c_uint64, C.POINTER(vp), C.c_char_p]),
         "magi_peer_open": (C.c_int, [vp, C.c_char_p, C.POINTER(vp)]),
         "magi_peer_close": (C.c_int, [vp, vp]),

@@ -1,0 +1,546 @@
+"""Token-paged 8-bit cache on the GPU: append, book-keeping and attention against plain 64-bit counterparts."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import paged_ref as R
+
+pytestmark = pytest.mark.gpu
+
+E_RANGE, E_NOMEM = -4, -5
+
+
+def i32(v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+def make_cache(lens, page, hkv, layers=1, extra=2, spare_rows=0, seed=0, per_row=None, poison=True):
+    """A cache with lens[i] tokens of random codes in row i, pages scattered; what lies behind a sequence's end, in free
+    pages and in their scales, is NaN codes and huge scales unless poison is off."""
+    import magi_b200 as mb
+    rng = np.random.RandomState(seed)
+    counts = [-(-n // page) for n in lens]
+    n_pages = sum(counts) + extra
+    c = mb.TokenPagedKVCache(layers, n_pages, page, hkv, len(lens) + spare_rows, per_row or max(counts + [1]))
+    order, at = rng.permutation(n_pages), 0
+    table, refs = np.full((c.max_seqs, c.max_pages_per_seq), -1, np.int32), np.zeros(n_pages, np.int32)
+    shape = (layers, n_pages, hkv, page, 128)
+    codes = [R.to_code(np.clip(rng.randn(*shape) * 90, -448, 448)) for _ in range(2)]
+    scales = [2.0 ** rng.randint(-9, -4, shape[:3]) for _ in range(2)]
+    used = np.zeros(n_pages, bool)
+    for i, n in enumerate(counts):
+        ids = order[at:at + n]
+        at += n
+        table[i, :n], refs[ids], used[ids] = ids, 1, True
+        if n and lens[i] % page and poison:
+            for x in codes:
+                x[:, ids[-1], :, lens[i] % page:] = 0x7f
+    if poison:
+        for x, s in zip(codes, scales):
+            x[:, ~used], s[:, ~used] = 0xff, 2.0 ** 60
+    for t, x in ((c.k8, codes[0]), (c.v8, codes[1])):
+        t.view(torch.uint8).copy_(torch.from_numpy(x))
+    for t, x in ((c.k_scale, scales[0]), (c.v_scale, scales[1]), (c.page_table, table), (c.page_refs, refs)):
+        t.copy_(torch.from_numpy(x))
+    c.seq_lens[:len(lens)] = i32(list(lens))
+    return c
+
+
+def strided_bf16(t, h, seed, pad=0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(t, h + pad, 128 + 8 * pad, generator=g).to(torch.bfloat16).cuda()
+    return x[:, :h, :128]
+
+
+def status():
+    import magi_b200 as mb
+    return mb.Context.get().status()
+
+
+def check_attn(c, q, seqs, cu, **kw):
+    import magi_b200 as mb
+    total, hq, _ = q.shape
+    n_q = [b - a for a, b in zip(cu, cu[1:])]
+    out = torch.full((total, hq, 128), 7.0, dtype=torch.bfloat16, device="cuda")
+    single = all(n == 1 for n in n_q) and total == len(seqs)
+    got, lse = mb.paged_attn(q, c, kw.pop("layer", 0), i32(seqs), None if single else i32(cu), max_q=max(n_q + [1]), out=out, **kw)
+    torch.cuda.synchronize()
+    assert got is out and status() == 0
+    kw.pop("softmax_scale", None) if kw.get("softmax_scale") is None else None
+    ref, ref_l, tol, tol_l = R.attention(R.Books(c), 0, q.double().cpu().numpy(), seqs, cu, c.n_kv_heads,
+                                         scale=kw.get("softmax_scale"), causal=kw.get("causal", True), window=kw.get("window", 0))
+    o, l = got.double().cpu().numpy(), lse.double().cpu().numpy()
+    owned = np.zeros(total, bool)
+    owned[cu[0]:cu[-1]] = True
+    assert (o[~owned] == 7.0).all(), "rows that no entry owns were written"
+    err = np.abs(o - ref)[owned]
+    assert np.array_equal(np.isnan(o[owned]), np.isnan(ref[owned]))
+    fine = np.isfinite(ref[owned])
+    assert (err[fine] <= tol[owned][fine]).all(), f"worst {np.nanmax(err / np.maximum(tol[owned], 1e-30))} of the tolerance"
+    both = np.isneginf(ref_l[owned]) == np.isneginf(l[owned])
+    assert both.all()
+    fl = np.isfinite(ref_l[owned])
+    assert (np.abs(l - ref_l)[owned][fl] <= tol_l[owned][fl]).all()
+    return o
+
+
+# ---------------------------------------------------------------------------------------- attention
+@pytest.mark.parametrize("page", [16, 32, 64, 128])
+@pytest.mark.parametrize("hq,hkv", [(6, 1), (8, 8), (48, 8), (16, 1), (20, 1), (6, 2)])
+def test_one_token_per_sequence(page, hq, hkv):
+    lens = [1, 0, 15, 16, 17, 127, 128, 129, 255, 257, 640, 1000]
+    c = make_cache(lens, page, hkv, seed=page + hq)
+    check_attn(c, strided_bf16(len(lens), hq, 3), list(range(len(lens))), list(range(len(lens) + 1)))
+
+
+@pytest.mark.parametrize("page,hq,hkv,window,causal", [(16, 6, 1, 0, True), (64, 48, 8, 0, True), (32, 6, 2, 5, True), (128, 8, 2, 100, True),
+                                                       (64, 6, 1, 0, False), (16, 12, 2, 129, False), (32, 24, 8, 1, True)])
+def test_several_tokens_per_sequence(page, hq, hkv, window, causal):
+    # more rows than keys, rows at every offset of a 128-key tile, an entry without rows
+    lens, n_q = [0, 3, 130, 256, 300, 77, 391], [4, 5, 2, 9, 17, 0, 64]
+    c = make_cache(lens, page, hkv, seed=page)
+    cu = np.concatenate([[0], np.cumsum(n_q)]).tolist()
+    q = strided_bf16(cu[-1] + 3, hq, 5, pad=1)  # three rows that no entry owns
+    check_attn(c, q, list(range(len(lens))), cu, window=window, causal=causal)
+
+
+@pytest.mark.parametrize("page,hq,hkv", [(64, 48, 8), (16, 6, 1), (128, 4, 4)])
+def test_prompts(page, hq, hkv):
+    lens, n_q = [513, 200, 333], [513, 129, 40]
+    c = make_cache(lens, page, hkv, seed=1)
+    check_attn(c, strided_bf16(sum(n_q), hq, 9), [0, 1, 2], np.concatenate([[0], np.cumsum(n_q)]).tolist())
+
+
+def test_long_context_is_split_and_joined():
+    c = make_cache([40003, 129], 64, 1, seed=2)
+    check_attn(c, strided_bf16(2, 6, 1), [0, 1], [0, 1, 2])
+    check_attn(c, strided_bf16(5, 6, 2), [0, 1], [0, 3, 5], softmax_scale=0.3)
+
+
+def test_the_same_sequence_twice_and_an_order_of_their_own():
+    c = make_cache([70, 400, 129], 32, 2, seed=4)
+    o = check_attn(c, strided_bf16(4, 4, 8)[[0, 1, 0, 2]], [2, 1, 2, 0], [0, 1, 2, 3, 4])
+    assert np.array_equal(o[0], o[2])
+
+
+def test_sharp_softmax_and_pages_of_very_different_scale():
+    """Scores of +-100s and V scales 2^40 apart: the weights of the small pages must not vanish where they win."""
+    c = make_cache([300], 16, 1, seed=6)
+    used = c.page_table[0, :19].long()
+    c.v_scale[0, used, 0] = torch.tensor([2.0 ** (40 * ((i % 3) - 1)) for i in range(19)], device="cuda")
+    c.k_scale[0, used, 0] = 2.0 ** -3
+    check_attn(c, strided_bf16(1, 6, 11), [0], [0, 1])
+    # one page wins by far, and it is one of the small ones
+    import magi_b200 as mb
+    c.k8.view(torch.uint8)[0, used, 0] = 0x38  # every key is all ones
+    c.k_scale[0, used, 0] = 2.0 ** -10
+    c.k_scale[0, used[3], 0] = 1.0
+    c.v_scale[0, used, 0] = 2.0 ** 20
+    c.v_scale[0, used[3], 0] = 2.0 ** -20
+    q = torch.full((1, 6, 128), 2.0, dtype=torch.bfloat16, device="cuda")
+    check_attn(c, q, [0], [0, 1])
+
+
+def test_nan_and_infinity_where_nothing_looks():
+    """NaN in later tokens than a row may see stays out of it and reaches the rows that do see it."""
+    c = make_cache([260], 32, 1, seed=7)
+    ids = c.page_table[0].long()
+    page, off = int(ids[250 // 32]), 250 % 32
+    c.v8.view(torch.uint8)[0, page, 0, off, 5] = 0x7f   # V of position 250, channel 5
+    page2, off2 = int(ids[255 // 32]), 255 % 32
+    c.k8.view(torch.uint8)[0, page2, 0, off2] = 0xff     # K of position 255
+    o = check_attn(c, strided_bf16(16, 6, 12), [0], [0, 16])   # positions 244 .. 259
+    assert np.isfinite(o[:6]).all() and np.isnan(o[6:11, :, 5]).all() and np.isfinite(o[6:11, :, 6:]).all() and np.isnan(o[11:]).all()
+
+
+def test_nan_and_infinite_queries_stay_in_their_rows():
+    c = make_cache([200], 64, 1, seed=8)
+    q = strided_bf16(3, 6, 13).clone()
+    import magi_b200 as mb
+    clean, _ = mb.paged_attn(q, c, 0, i32([0]), i32([0, 3]), max_q=3)
+    q[0, 2, 17] = math.nan
+    q[1, 4, 3] = math.inf
+    out, lse = mb.paged_attn(q, c, 0, i32([0]), i32([0, 3]), max_q=3)
+    bad = torch.zeros(3, 6, dtype=torch.bool, device="cuda")
+    bad[0, 2] = bad[1, 4] = True
+    assert out[bad].isnan().all() and lse[bad].isnan().all()
+    assert torch.equal(out[~bad], clean[~bad])
+
+
+def test_queries_of_any_size():
+    c = make_cache([150], 64, 1, seed=9)
+    q = strided_bf16(6, 6, 14) * torch.tensor([1e-30, 0.0, 1e-3, 30.0, 1.0, 1e-38], device="cuda")[:, None, None].to(torch.bfloat16)
+    check_attn(c, q, [0], [0, 6])
+
+
+def test_layers_and_out_and_strides():
+    import magi_b200 as mb
+    c = make_cache([100, 33], 32, 2, layers=3, seed=10)
+    q = strided_bf16(2, 4, 15, pad=2)
+    books = R.Books(c)
+    for layer in range(3):
+        wide = torch.zeros(4, 7, 144, dtype=torch.bfloat16, device="cuda")
+        out, lse = mb.paged_attn(q, c, layer, i32([0, 1]), out=wide[:, 1:5, 8:136])
+        ref, _, tol, _ = R.attention(books, layer, q.double().cpu().numpy(), [0, 1], [0, 1, 2], 2)
+        assert (np.abs(out[:2].double().cpu().numpy() - ref) <= tol).all()
+        wide[:2, 1:5, 8:136] = 0
+        assert (wide == 0).all()
+        none = mb.paged_attn(q, c, layer, i32([0, 1]), return_lse=False)
+        assert none[1] is None and torch.equal(none[0], mb.paged_attn(q, c, layer, i32([0, 1]))[0])
+
+
+def test_results_do_not_change_from_call_to_call():
+    import magi_b200 as mb
+    c = make_cache([5000, 77, 1300], 64, 2, seed=20)
+    q = strided_bf16(3, 12, 21)
+    first = mb.paged_attn(q, c, 0, i32([0, 1, 2]))
+    for _ in range(5):
+        again = mb.paged_attn(q, c, 0, i32([0, 1, 2]))
+        assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
+def test_two_streams_at_once():
+    import magi_b200 as mb
+    c = make_cache([9000, 500], 64, 2, layers=2, seed=22)
+    q = strided_bf16(2, 12, 23)
+    want = [mb.paged_attn(q, c, layer, i32([0, 1])) for layer in range(2)]
+    side = [torch.cuda.Stream() for _ in range(2)]
+    seqs = i32([0, 1])
+    torch.cuda.synchronize()
+    got = [[mb.paged_attn(q, c, layer, seqs, stream=side[layer]) for layer in range(2)] for _ in range(20)]
+    torch.cuda.synchronize()
+    for pair in got:
+        for w, g in zip(want, pair):
+            assert torch.equal(w[0], g[0]) and torch.equal(w[1], g[1])
+
+
+def test_a_table_that_points_nowhere_is_reported():
+    import magi_b200 as mb
+    c = make_cache([300], 64, 1, seed=24)
+    c.page_table[0, 2] = 10 ** 6
+    mb.paged_attn(strided_bf16(1, 6, 1), c, 0, i32([0]))
+    assert status() == E_RANGE
+    mb.paged_attn(strided_bf16(1, 6, 1), c, 0, i32([5]))
+    assert status() == E_RANGE and status() == 0
+
+
+# ---------------------------------------------------------------------------------------- append
+@pytest.mark.parametrize("page", [16, 32, 64, 128])
+@pytest.mark.parametrize("hkv", [1, 3, 8])
+def test_append_matches_the_definition(page, hkv):
+    rng = np.random.RandomState(page + hkv)
+    lens, new = [0, 1, 15, 16, 130, 255, 7, 64], [1, 16, 1, 3, 300, 1, 0, 129]
+    total = [a + b for a, b in zip(lens, new)]
+    c = make_cache(total, page, hkv, layers=2, seed=1)
+    cu = np.concatenate([[0], np.cumsum(new)]).tolist()
+    size = np.exp(2 * rng.randn(cu[-1], 1, 1))
+    k, v = [torch.from_numpy(rng.randn(cu[-1], hkv, 128) * size).to(torch.bfloat16).cuda() for _ in range(2)]
+    wide = torch.zeros(cu[-1], hkv + 1, 264, dtype=torch.bfloat16, device="cuda")
+    wide[:, :hkv, :128], wide[:, :hkv, 136:] = k, v
+    books = R.Books(c)
+    for i in range(len(lens)):
+        books.append(1, i, lens[i], k[cu[i]:cu[i + 1]].double().cpu().numpy(), v[cu[i]:cu[i + 1]].double().cpu().numpy())
+    c.append(1, i32(list(range(len(lens)))), i32(lens), wide[:, :hkv, :128], wide[:, :hkv, 136:], i32(cu), max_new=max(new))
+    torch.cuda.synchronize()
+    assert status() == 0 and books.same(c) is None, books.same(c)
+
+
+def test_token_by_token():
+    """Scales that grow many times over; the last page is written token after token."""
+    rng = np.random.RandomState(3)
+    c = make_cache([0, 5], 32, 2, seed=2, extra=8, per_row=4)
+    books = R.Books(c)
+    for step in range(70):
+        size = 2.0 ** rng.randint(-30, 30)
+        k, v = [torch.from_numpy(rng.randn(2, 2, 128) * size).to(torch.bfloat16).cuda() for _ in range(2)]
+        starts = c.reserve(i32([1, 0]), i32([1, 1]))
+        assert starts.tolist() == books.reserve([1, 0], [1, 1])
+        c.append(0, i32([1, 0]), starts, k, v)
+        for i, s in enumerate((1, 0)):
+            books.append(0, s, books.lens[s] - 1, k[i:i + 1].double().cpu().numpy(), v[i:i + 1].double().cpu().numpy())
+    assert status() == 0 and books.same(c) is None, books.same(c)
+
+
+def test_append_of_unusual_values():
+    c = make_cache([0], 16, 1, seed=2, extra=4, per_row=2)
+    c.reserve(i32([0]), i32([20]))
+    books = R.Books(c)
+    x = torch.zeros(20, 1, 128)
+    x[0, 0, :6] = torch.tensor([math.nan, math.inf, -math.inf, 3.0, -448.0, 1e-30])
+    x[1:15, 0] = torch.randn(14, 128) * 100
+    x[16, 0, :4] = torch.tensor([1e38, -3e38, 1e-38, 0.0])    # beyond 448 * 2^60: the scale's end, saturated
+    x = x.to(torch.bfloat16).cuda()
+    tiny = (torch.randn(20, 1, 128) * 1e-30).to(torch.bfloat16).cuda()  # below the smallest scale: zeros
+    c.append(0, i32([0]), i32([0]), x, tiny, i32([0, 20]), max_new=20)
+    books.append(0, 0, 0, x.double().cpu().numpy(), tiny.double().cpu().numpy())
+    assert status() == 0 and books.same(c) is None, books.same(c)
+    assert float(c.k_scale[0, int(c.page_table[0, 1]), 0]) == 2.0 ** 60 and float(c.v_scale[0, int(c.page_table[0, 0]), 0]) == 2.0 ** -60
+
+
+def test_rewriting_tokens_in_the_middle_keeps_their_neighbours():
+    c = make_cache([50], 32, 1, seed=5, poison=False)
+    books = R.Books(c)
+    k, v = [(torch.randn(10, 1, 128) * 1000).to(torch.bfloat16).cuda() for _ in range(2)]
+    c.append(0, i32([0]), i32([27]), k, v, i32([0, 10]), max_new=10)
+    books.append(0, 0, 27, k.double().cpu().numpy(), v.double().cpu().numpy())
+    assert status() == 0 and books.same(c) is None, books.same(c)
+
+
+def test_append_refuses_on_the_device_and_writes_nothing():
+    c = make_cache([40, 20], 16, 1, seed=6, spare_rows=1)
+    k = torch.ones(8, 1, 128, dtype=torch.bfloat16, device="cuda")
+    before = R.Books(c)
+    for seqs, starts, cu, most in (([0], [36], [0, 8], 8),      # beyond the sequence
+                                   ([7], [0], [0, 8], 8),       # no such sequence
+                                   ([-1], [0], [0, 8], 8),
+                                   ([0], [0], [0, 9], 9),       # more rows than there are
+                                   ([0], [0], [0, 8], 4),       # more than max_new
+                                   ([0], [0], [5, 2], 4),       # backwards
+                                   ([2], [0], [0, 8], 8)):      # an empty sequence
+        c.append(0, i32(seqs), i32(starts), k, k, i32(cu), max_new=most)
+        assert status() == E_RANGE, (seqs, starts, cu)
+        assert before.same(c) is None
+    c.append(0, i32([0]), i32([-1]), k, k, i32([0, 8]), max_new=8)   # skipped, not refused
+    assert status() == 0 and before.same(c) is None
+    c.fork(i32([0]), i32([2]))
+    shared = R.Books(c)
+    c.append(0, i32([2]), i32([0]), k, k, i32([0, 8]), max_new=8)    # a page that two sequences hold
+    assert status() == E_RANGE and shared.same(c) is None
+
+
+# ---------------------------------------------------------------------------------------- books
+@pytest.mark.parametrize("page,hkv,layers,seed", [(16, 1, 1, 0), (32, 3, 2, 1), (64, 8, 2, 2), (128, 2, 1, 3), (16, 2, 3, 4)])
+def test_random_histories(page, hkv, layers, seed):
+    """Reserve, append, fork, copy, free and compact in random order, refused calls among them, against plain Python."""
+    rng = np.random.RandomState(seed)
+    c = make_cache([0] * 12, page, hkv, layers=layers, extra=60, seed=seed, per_row=9, poison=False)
+    books = R.Books(c)
+    refused = 0
+    for step in range(120):
+        op = rng.choice(["reserve", "reserve", "fork", "copy", "free", "compact"])
+        n = rng.randint(1, 5)
+        some = rng.permutation(12)[:n].tolist() if rng.rand() < 0.9 else rng.randint(-1, 13, n).tolist()
+        if op == "reserve":
+            add = [int(a) for a in rng.randint(0, 2 * page, n)]
+            want = books.reserve(some, add)
+            starts = c.reserve(i32(some), i32(add))
+            assert starts.tolist() == (want if want is not None else [-1] * n)
+            ok = want is not None
+            if ok and sum(add):
+                k, v = [torch.from_numpy(rng.randn(sum(add), hkv, 128) * 2.0 ** rng.randint(-4, 5)).to(torch.bfloat16).cuda() for _ in range(2)]
+                cu = np.concatenate([[0], np.cumsum(add)]).tolist()
+                layer = int(rng.randint(layers))
+                c.append(layer, i32(some), starts, k, v, i32(cu), max_new=max(add))
+                for i, s in enumerate(some):
+                    books.append(layer, s, want[i], k[cu[i]:cu[i + 1]].double().cpu().numpy(), v[cu[i]:cu[i + 1]].double().cpu().numpy())
+        elif op in ("fork", "copy"):
+            src = [int(s) for s in rng.randint(0, 12, n)]
+            if rng.rand() < 0.7:
+                some = [s for s in range(12) if books.lens[s] == 0][:n] or some
+                src = src[:len(some)]
+            ok = books.branch(src, some, op == "fork")
+            getattr(c, op)(i32(src), i32(some))
+        elif op == "free":
+            ok = books.free(some)
+            c.free(i32(some))
+        else:
+            books.compact()
+            c.compact()
+            ok = True
+        st = status()
+        assert (st == 0) == ok and st in (0, E_RANGE, E_NOMEM), (step, op, st, ok)
+        refused += not ok
+        if step % 10 == 9 or not ok:
+            diff = books.same(c)
+            assert diff is None, (step, op, diff)
+    assert refused > 3
+
+
+def test_reserve_of_many_pages_at_once():
+    import magi_b200 as mb
+    c = mb.TokenPagedKVCache(1, 40000, 16, 1, 600, 2500)
+    c.page_refs[::7] = 1
+    books = R.Books(c)
+    n_new = [int(v) for v in np.random.RandomState(0).randint(0, 900, 500)]
+    seqs = np.random.RandomState(1).permutation(600)[:500].tolist()
+    starts = c.reserve(i32(seqs), i32(n_new))
+    assert starts.tolist() == books.reserve(seqs, n_new) and books.same(c) is None and status() == 0
+    c.free(i32(seqs))
+    books.free(seqs)
+    assert books.same(c) is None
+    c.reserve(i32([0]), i32([40000]))
+    books.reserve([0], [40000])
+    assert books.same(c) is None and status() == 0
+    c.compact()
+    books.table, books.refs = [[] for _ in range(600)], None
+    assert status() == 0 and int((c.page_refs[:int((c.page_refs > 0).sum())] == 0).sum()) == 0
+
+
+def test_refusals_leave_everything_as_it_was():
+    c = make_cache([20, 40, 0, 0], 16, 1, extra=2, seed=3, per_row=8)
+    books = R.Books(c)
+    for call, want in ((lambda: c.reserve(i32([0, 0]), i32([1, 1])), E_RANGE),
+                       (lambda: c.reserve(i32([0, 9]), i32([1, 1])), E_RANGE),
+                       (lambda: c.reserve(i32([0, -1]), i32([1, 1])), E_RANGE),
+                       (lambda: c.reserve(i32([0, 1]), i32([1, -1])), E_RANGE),
+                       (lambda: c.reserve(i32([0]), i32([109])), E_RANGE),          # beyond the table row
+                       (lambda: c.reserve(i32([0]), i32([2 ** 31 - 1])), E_RANGE),
+                       (lambda: c.reserve(i32([0, 1]), i32([1, 57])), E_NOMEM),
+                       (lambda: c.fork(i32([0]), i32([1])), E_RANGE),               # not empty
+                       (lambda: c.fork(i32([0, 1]), i32([2, 2])), E_RANGE),
+                       (lambda: c.fork(i32([0, 2]), i32([2, 3])), E_RANGE),         # a source that this call fills
+                       (lambda: c.fork(i32([2]), i32([2])), E_RANGE),
+                       (lambda: c.fork(i32([4]), i32([2])), E_RANGE),
+                       (lambda: c.copy(i32([1]), i32([2])), E_NOMEM),
+                       (lambda: c.free(i32([0, 0])), E_RANGE),
+                       (lambda: c.free(i32([0, 4])), E_RANGE)):
+        r = call()
+        assert status() == want
+        assert r is None or (r == -1).all()
+        assert books.same(c) is None
+    c.free(i32([2, 3]))    # empty already: nothing to do
+    assert status() == 0 and books.same(c) is None
+    c.fork(i32([2]), i32([3]))   # an empty sequence has empty branches
+    assert status() == 0 and books.same(c) is None
+    empty = i32([])
+    c.reserve(empty, empty), c.fork(empty, empty), c.copy(empty, empty), c.free(empty)
+    assert status() == 0 and books.same(c) is None
+
+
+# ---------------------------------------------------------------------------------------- together
+def _step(mb, c, layer_in, seqs, ones, freq, pos):
+    """One decode step of a toy model of two layers: rotate, reserve, append, attend."""
+    starts = c.reserve(seqs, ones)
+    outs = []
+    for layer, (q, k, v) in enumerate(layer_in):
+        c.append(layer, seqs, starts, mb.rotary(k, starts, freq), v)
+        outs.append(mb.paged_attn(mb.rotary(q, starts, freq), c, layer, seqs))
+    return starts, outs
+
+
+def test_a_serving_loop():
+    """Prompts read in, branches forked, tokens appended, a branch dropped, the pool compacted: attention of the result
+    equals attention over the exact history (up to the 8-bit codes, which the reference reads from the cache)."""
+    import magi_b200 as mb
+    hq, hkv, layers = 12, 2, 2
+    c = mb.TokenPagedKVCache(layers, 64, 16, hkv, 8, 20)
+    freq, _ = mb.rotary_frequencies(96)
+    books = R.Books(c)
+    g = torch.Generator(device="cuda").manual_seed(0)
+    n = [37, 90]
+    starts = c.reserve(i32([0, 1]), i32(n))
+    books.reserve([0, 1], n)
+    cu = [0, 37, 127]
+    pos = torch.cat([torch.arange(37), torch.arange(90)]).int().cuda()
+    for layer in range(layers):
+        q, k, v = [torch.randn(127, h, 128, generator=g, device="cuda").to(torch.bfloat16) for h in (hq, hkv, hkv)]
+        k = mb.rotary(k, pos, freq)
+        c.append(layer, i32([0, 1]), starts, k, v, i32(cu), max_new=90)
+        for i in range(2):
+            books.append(layer, i, 0, *[t[cu[i]:cu[i + 1]].double().cpu().numpy() for t in (k, v)])
+        out, _ = mb.paged_attn(mb.rotary(q, pos, freq), c, layer, i32([0, 1]), i32(cu), max_q=90)
+        ref, _, tol, _ = R.attention(books, layer, mb.rotary(q, pos, freq).double().cpu().numpy(), [0, 1], cu, hkv)
+        assert (np.abs(out.double().cpu().numpy() - ref) <= tol).all()
+    c.fork(i32([0, 0, 1]), i32([2, 5, 4]))
+    books.branch([0, 0, 1], [2, 5, 4], True)
+    assert books.same(c) is None
+    live = [0, 1, 2, 4, 5]
+    for step in range(20):
+        if step == 9:
+            c.free(i32([1, 0]))
+            books.free([1, 0])
+            c.compact()
+            books.compact()
+            live = [2, 4, 5]
+            assert books.same(c) is None
+        seqs, ones = i32(live), i32([1] * len(live))
+        ins = [[torch.randn(len(live), h, 128, generator=g, device="cuda").to(torch.bfloat16) for h in (hq, hkv, hkv)] for _ in range(layers)]
+        starts, outs = _step(mb, c, ins, seqs, ones, freq, None)
+        want = books.reserve(live, [1] * len(live))
+        assert starts.tolist() == want
+        for layer, (q, k, v) in enumerate(ins):
+            kr = mb.rotary(k, starts, freq)
+            for i, s in enumerate(live):
+                books.append(layer, s, want[i], kr[i:i + 1].double().cpu().numpy(), v[i:i + 1].double().cpu().numpy())
+        assert books.same(c) is None, step
+        for layer, (q, k, v) in enumerate(ins):
+            ref, _, tol, _ = R.attention(books, layer, mb.rotary(q, starts, freq).double().cpu().numpy(), live, list(range(len(live) + 1)), hkv)
+            assert (np.abs(outs[layer][0].double().cpu().numpy() - ref) <= tol).all()
+    assert status() == 0
+
+
+def test_a_captured_step_replays():
+    """The whole step in one graph, replayed over page boundaries, equals the eager steps; another graph of the same cache
+    lives beside it."""
+    import magi_b200 as mb
+    hq, hkv, layers = 6, 1, 2
+    lens = [14, 300, 0]
+
+    def fresh():
+        return make_cache(lens, 16, hkv, layers=layers, extra=12, seed=4, per_row=24)
+
+    freq, _ = mb.rotary_frequencies(128)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    steps = [[[torch.randn(3, h, 128, generator=g, device="cuda").to(torch.bfloat16) for h in (hq, hkv, hkv)] for _ in range(layers)] for _ in range(8)]
+    seqs, ones = i32([0, 1, 2]), i32([1, 1, 1])
+    eager, want = fresh(), []
+    for ins in steps:
+        want.append([o[0].clone() for o in _step(mb, eager, ins, seqs, ones, freq, None)[1]])
+    c = fresh()
+    saved = [t.clone() for t in (c.page_table, c.seq_lens, c.page_refs)]
+    static = [[t.clone() for t in layer] for layer in steps[0]]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        _step(mb, c, static, seqs, ones, freq, None)
+    torch.cuda.current_stream().wait_stream(side)
+    graph, other = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        _, outs = _step(mb, c, static, seqs, ones, freq, None)
+    with torch.cuda.graph(other):
+        look = mb.paged_attn(static[0][0], c, 0, seqs)
+    c2 = fresh()
+    for t, s in zip((c.k8, c.v8, c.k_scale, c.v_scale), (c2.k8, c2.v8, c2.k_scale, c2.v_scale)):
+        t.view(torch.uint8).copy_(s.view(torch.uint8))
+    for t, s in zip((c.page_table, c.seq_lens, c.page_refs), saved):
+        t.copy_(s)
+    for ins, w in zip(steps, want):
+        for a, b in zip(static, ins):
+            for x, y in zip(a, b):
+                x.copy_(y)
+        graph.replay()
+        other.replay()
+        torch.cuda.synchronize()
+        for o, e in zip(outs, w):
+            assert torch.equal(o[0], e)
+        assert torch.equal(look[0], mb.paged_attn(static[0][0], c, 0, seqs)[0])
+    assert status() == 0
+    assert R.Books(eager).same(c) is None
+
+
+# ---------------------------------------------------------------------------------------- arguments
+def test_arguments_are_checked():
+    import magi_b200 as mb
+    c = make_cache([10], 16, 2, seed=1)
+    q, k = strided_bf16(1, 4, 1), strided_bf16(1, 2, 2)
+    one, seqs = i32([1]), i32([0])
+    for bad in (lambda: mb.TokenPagedKVCache(1, 4, 48, 1, 1, 1), lambda: mb.TokenPagedKVCache(0, 4, 16, 1, 1, 1),
+                lambda: c.reserve(torch.tensor([0]), one), lambda: c.reserve(seqs.long(), one), lambda: c.reserve(seqs, i32([1, 2])),
+                lambda: c.reserve(i32([[0]]), one), lambda: c.reserve(i32([0, 0, 0])[::2], i32([1, 1])), lambda: c.reserve(i32([0] * 1025), i32([0] * 1025)),
+                lambda: c.append(0, seqs, one, k.float(), k), lambda: c.append(0, seqs, one, k[:, :1], k[:, :1]),
+                lambda: c.append(0, seqs, one, k, k[:0]), lambda: c.append(0, seqs, one, k[:0], k[:0]),
+                lambda: c.append(0, seqs, one, k, k, i32([0])), lambda: c.append(0, seqs, one, k, k, max_new=2),
+                lambda: mb.paged_attn(q.cpu(), c, 0, seqs), lambda: mb.paged_attn(q.half(), c, 0, seqs),
+                lambda: mb.paged_attn(q[:, :3], c, 0, seqs), lambda: mb.paged_attn(q, c, 0, i32([0, 0])),
+                lambda: mb.paged_attn(q, c, 0, seqs, window=-1), lambda: mb.paged_attn(q, c, 0, seqs, i32([0, 1, 1])),
+                lambda: mb.paged_attn(q, c, 0, seqs, out=q[:0]), lambda: mb.paged_attn(q, c, 0, seqs, max_q=2)):
+        with pytest.raises(ValueError):
+            bad()
+    for bad in (lambda: mb.paged_attn(q, c, 1, seqs), lambda: mb.paged_attn(q, c, -1, seqs), lambda: c.append(1, seqs, one, k, k),
+                lambda: mb.paged_attn(torch.zeros(1, 4, 132, dtype=torch.bfloat16, device="cuda")[..., 2:130], c, 0, seqs)):
+        with pytest.raises(mb.MagiError):
+            bad()
+    assert mb.paged_attn(q[:0], c, 0, i32([]))[0].shape == (0, 4, 128)
+    assert status() == 0
