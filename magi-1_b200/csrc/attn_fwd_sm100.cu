@@ -343,6 +343,20 @@ int make_tile_map(magi_ctx* ctx, CUtensorMap* m, const void* base, int64_t strid
   return MAGI_OK;
 }
 
+// [rows, 128] bytes -> 2-D map, box = box_rows whole rows, 128-byte swizzle.
+int make_rows_map(magi_ctx* ctx, CUtensorMap* m, const void* base, int rows, int box_rows, const char* what) {
+  EncodeTiledFn fn = get_encode_fn();
+  if (!fn) return set_err(ctx, MAGI_E_CUDA, "cuTensorMapEncodeTiled entry point not found");
+  cuuint64_t dims[2] = {(cuuint64_t)kHeadDim, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)kHeadDim};
+  cuuint32_t box[2] = {(cuuint32_t)kHeadDim, (cuuint32_t)box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_err(ctx, MAGI_E_CUDA, "%s: cuTensorMapEncodeTiled failed (%d)", what, (int)r);
+  return MAGI_OK;
+}
+
 int attn_fp8_init_device(magi_ctx* ctx);
 // Opt in to > 48 KB of dynamic shared memory; called once per context with its device current.
 int attn_init_device(magi_ctx* ctx) {

@@ -89,8 +89,8 @@ class TokenPagedKVCache:
         # zero-filled once: attention multiplies what lies behind a sequence's end by zero, so it has to be finite
         self.k8 = torch.zeros(shape, dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn)
         self.v8 = torch.zeros(shape, dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn)
-        self.k_scale = torch.zeros(shape[:3], dtype=torch.float32, device=dev)
-        self.v_scale = torch.zeros_like(self.k_scale)
+        self.k_scale = torch.full(shape[:3], 2.0 ** -60, dtype=torch.float32, device=dev)
+        self.v_scale = self.k_scale.clone()
         self.page_table = torch.full((self.max_seqs, self.max_pages_per_seq), -1, dtype=torch.int32, device=dev)
         self.seq_lens = torch.zeros(self.max_seqs, dtype=torch.int32, device=dev)
         self.page_refs = torch.zeros(self.n_pages, dtype=torch.int32, device=dev)
@@ -226,7 +226,7 @@ def paged_attn(q: torch.Tensor, cache: TokenPagedKVCache, layer: int, seqs: torc
     p.causal, p.window = int(bool(causal)), int(window)
     p.workspace = ws.data_ptr()
     check(lib.magi_paged_attn_fwd(cache.ctx.handle, C.byref(cache._view), C.byref(p), raw), cache.ctx.handle)
-    KERNEL_LAUNCHES[0] += 1
+    KERNEL_LAUNCHES[0] += 2  # attention and join
     return out, lse
 
 
