@@ -40,7 +40,11 @@ int make_rows_map(magi_ctx* ctx, CUtensorMap* m, const void* base, int rows, int
 constexpr int kPaTile = 128;                   // keys of a tile
 constexpr int kPaTileBytes = kPaTile * kHeadDim;
 constexpr int kPaNear = 64;                    // entries whose lengths a block keeps in shared memory
-constexpr float kPaShift = 8.0f;               // P = 2^(w - max + 8) <= 256: e4m3 then reaches 2^-18 of the largest weight
+// P = 2^(w - reference + 5).  The reference of a row is the exact maximum when it is set and stays while no weight exceeds
+// e4m3's 448 = 2^8.8, that is until the maximum has grown 14-fold: nearly every tile then needs one vote of the group in
+// place of its maxima, and the tensor core goes on summing in TMEM.  The residual term is e5m2, whose smallest step is 2^-16:
+// a weight is dropped only below 2^-22 of the reference, so a long tail of small weights behind one large one keeps its mass.
+constexpr float kPaShift = 5.0f, kPaLimit = 8.8f;
 
 struct PagedAttnKernelParams {
   PagedView c;
@@ -141,32 +145,39 @@ struct PaStart {
 template <int RG, int G>
 struct PaShared {
   static constexpr int kRows = RG * G;
-  static constexpr int kStages = G == 1 ? 4 : 8;
+  static constexpr int kStages = kRows == 16 ? 5 : kRows == 32 ? 4 : 6;
   static constexpr int kWarps = 4 * G;                         // softmax warps
-  static constexpr int kThreads = 64 + 32 * kWarps;
+  static constexpr int kFirst = 2;                             // the first of them
+  static constexpr int kThreads = 32 * (kFirst + kWarps);
   static constexpr int kRing = 0;
-  static constexpr int kP = kRing + kStages * kPaTileBytes;    // two buffers [128 keys][128 bytes]: terms at byte 0 and 64
-  static constexpr int kQ = kP + 2 * kPaTileBytes;             // [2 terms][kRows][128 bytes]
+  // Two buffers of P, a byte per (key, row) and term.  Up to 32 rows: all four share the 128-byte rows [key] of one tile
+  // (term 0 of buffer 0 and 1, then term 1 of both, 32 bytes each); else each is a tile of its own.
+  static constexpr int kPBuf = kRows <= 32 ? 32 : 2 * kPaTileBytes;
+  static constexpr int kPTerm = kRows <= 32 ? 64 : kPaTileBytes;
+  static constexpr int kP = kRing + kStages * kPaTileBytes;
+  static constexpr int kQ = kP + (kRows <= 32 ? 1 : 4) * kPaTileBytes;  // [2 terms][kRows][128 bytes]
   static constexpr int kScales = kQ + 2 * kRows * 128;         // [kStages][2][8] page scales of the last kStages tiles
-  static constexpr int kMax = kScales + kStages * 64;          // [2][G][4][RG] warp maxima
-  static constexpr int kRowM = kMax + 2 * G * 4 * RG * 4;      // [kWarps][RG]
-  static constexpr int kRowA = kRowM + kWarps * RG * 4;        // [2][kWarps][RG] factors of the last two tiles
-  static constexpr int kRowS = kRowA + 2 * kWarps * RG * 4;    // [2][kRows] scale of a query row
+  static constexpr int kMax = kScales + kStages * 64;          // [G][4][RG] warp maxima, and sums at a unit's end
+  static constexpr int kNegM = kMax + G * 4 * RG * 4;          // [kRows]
+  static constexpr int kFactor = kNegM + kRows * 4;            // [kRows]
+  static constexpr int kRowS = kFactor + kRows * 4;            // [2][kRows] scale of a query row
   static constexpr int kRowPos = kRowS + 2 * kRows * 4;        // [2][kRows] its position
-  static constexpr int kSum = kRowPos + 2 * kRows * 4;         // [G][4][RG] sums over a warp's keys
-  static constexpr int kNan = kSum + G * 4 * RG * 4;           // [2][128][4] channels whose V is NaN (boundary tiles)
+  static constexpr int kInv = kRowPos + 2 * kRows * 4;         // [kWarps][RG]
+  static constexpr int kAt = kInv + kWarps * RG * 4;           // [kWarps][RG] where a row of the result starts
+  static constexpr int kNan = kAt + kWarps * RG * 8;             // [2][128][4] channels whose V is NaN (boundary tiles)
   static constexpr int kNanAny = kNan + 2 * kPaTile * 16;      // [2][4] whether a warp's keys have any
   static constexpr int kNear = kNanAny + 32;                   // [kPaNear] entries
   static constexpr int kStart = kNear + kPaNear * 16;
   static constexpr int kBar = kStart + 64;
-  static constexpr int kNumBars = 3 * kStages + 6 + 1 + G + 1 + 1;
+  static constexpr int kNumBars = 3 * kStages + 8;
   static constexpr int kMisc = kBar + kNumBars * 8;
   static constexpr int kTotal = kMisc + 16;
   static constexpr int kDynamic = kTotal + 1024;
-  static constexpr uint32_t kTmemCols = 4 * kRows;             // S and O, two buffers each
+  static constexpr uint32_t kTmemCols = kRows <= 32 ? 4 * kRows : 512;             // S twice, O (the allocation is a power of two)
 };
 static_assert(PaShared<16, 1>::kDynamic * 2 + 2048 <= 233472, "two blocks of the small form per SM");
-static_assert(PaShared<32, 2>::kDynamic <= 232448, "shared memory per block");
+static_assert(PaShared<32, 1>::kDynamic * 2 + 2048 <= 233472, "two blocks of the middle form per SM");
+static_assert(PaShared<32, 3>::kDynamic <= 232448, "shared memory per block");
 
 __device__ __forceinline__ void tma_load_2d(void* smem_dst, const CUtensorMap* m, uint64_t* bar, int c0, int c1) {
   asm volatile(
@@ -195,11 +206,84 @@ __device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t* r) {
   if constexpr (N == 16) tmem_ld16(taddr, r);
   else tmem_ld32(taddr, r);
 }
+__device__ __forceinline__ uint32_t pack4_e4m3(float a, float b, float c, float d) {
+  return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3) |
+         (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3) << 16;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 // Largest value over the warp, NaN left out.
 __device__ __forceinline__ float warp_max(float v) {
   float r;
-  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));  // volatile: not to be moved under a branch
   return r;
+}
+
+// A whole warp waits, its lanes staying together: lane 0 asks, by predicate and not by branch, and the warp votes.  (32 lanes
+// asking for one barrier are served one after the other, about 200 cycles a question; a branch on the lane leaves lane 0
+// behind on its own, and the warp-wide instructions that follow need all lanes at once.)
+__device__ __forceinline__ bool warp_wait(bool ok, uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  if (!ok) return false;
+  const uint32_t addr = smem_u32(bar), lane = threadIdx.x & 31;
+  long long t0 = 0;
+  while (true) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred l, p;\n\t"
+        "setp.eq.u32 l, %3, 0;\n\t"
+        "setp.ne.u32 p, %3, %3;\n\t"
+        "@l mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %4;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(addr), "r"(parity), "r"(lane), "r"((uint32_t)MAGI_WAIT_HINT_NS)
+        : "memory");
+    if (__any_sync(0xffffffffu, done)) break;
+    const long long now = clock64();
+    if (t0 == 0) t0 = now;
+    const bool late = now - t0 > 1000000000LL;
+    if (__any_sync(0xffffffffu, late)) *abort_flag = 1;
+    __syncwarp();
+    if (__any_sync(0xffffffffu, *abort_flag != 0)) return false;
+  }
+  __syncwarp();  // what lane 0 has seen is there for the others
+  return true;
+}
+// One arrival for the warp, after what all its lanes did before.
+__device__ __forceinline__ void warp_arrive(uint64_t* bar) {
+  __syncwarp();
+  asm volatile(
+      "{\n\t.reg .pred l;\n\t"
+      "setp.eq.u32 l, %1, 0;\n\t"
+      "@l mbarrier.arrive.shared::cta.b64 _, [%0];\n\t}"
+      ::"r"(smem_u32(bar)), "r"(threadIdx.x & 31)
+      : "memory");
+}
+
+// Barriers of a softmax group (128 threads) and of all softmax warps.  A warp counts once only if its lanes arrive together.
+__device__ __forceinline__ bool group_any(int id, bool v) {
+  uint32_t r;
+  __syncwarp();
+  asm volatile(
+      "{\n\t.reg .pred a, b;\n\t"
+      "setp.ne.u32 a, %1, 0;\n\t"
+      "bar.red.or.pred b, %2, 128, a;\n\t"
+      "selp.u32 %0, 1, 0, b;\n\t}"
+      : "=r"(r)
+      : "r"((uint32_t)v), "r"(id)
+      : "memory");
+  return r != 0;
+}
+__device__ __forceinline__ void group_sync(int id) {
+  __syncwarp();
+  asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void all_sync(int id) {
+  __syncwarp();
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(N) : "memory");
 }
 
 template <int RG, int G>
@@ -218,9 +302,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
   uint64_t* p_full = s_full + 2;
   uint64_t* o_full = p_full + 2;
   uint64_t* q_full = o_full + 2;
-  uint64_t* group_bar = q_full + 1;
-  uint64_t* fix_bar = group_bar + G;
-  uint64_t* drain_bar = fix_bar + 1;
+  uint64_t* drain_bar = q_full + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kMisc + 4);
   PaStart* start = reinterpret_cast<PaStart*>(smem + L::kStart);
@@ -241,8 +323,6 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       mbar_init(&o_full[x], 1);
     }
     mbar_init(q_full, L::kWarps);
-    for (int g = 0; g < G; ++g) mbar_init(&group_bar[g], 4);
-    mbar_init(fix_bar, L::kWarps);
     mbar_init(drain_bar, 1);
     *abort_flag = 0;
     fence_mbar_init();
@@ -406,8 +486,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv, ++fill) {
           const int stage = fill % kStages, use = fill / kStages;
-          if (use > 0) ok = mbar_wait(&kv_empty[stage], (use & 1) ^ 1, abort_flag);
-          ok = __all_sync(0xffffffffu, ok);
+          if (use > 0) ok = warp_wait(ok, &kv_empty[stage], (use & 1) ^ 1, abort_flag);
           if (!ok) break;
           if (lane == 0) mbar_expect_tx(&kv_full[stage], n_load << (p.page_shift + 7));
           __syncwarp();
@@ -431,7 +510,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
     // ------------------------------------------------------------------ UMMA issuer
     if (lane == 0) {
       constexpr uint32_t idesc_s = umma_idesc(kPaTile, R, 0, 0, 0, 0);
-      constexpr uint32_t idesc_o = umma_idesc(kHeadDim, R, 0, 0, 1, 1);
+      constexpr uint32_t idesc_o = umma_idesc(kHeadDim, R, 0, 0, 1, 1), idesc_r = umma_idesc(kHeadDim, R, 0, 1, 1, 1);  // B e4m3, e5m2
       constexpr uint32_t desc_hi = (1024u >> 4) | (1u << 14) | (2u << 29);  // 1024 bytes between groups of 8 rows, 128-byte swizzle
       const uint32_t ring = (smem_u32(smem + L::kRing) >> 4) | (1u << 16);
       const uint32_t q_lo = (smem_u32(smem + L::kQ) >> 4) | (1u << 16);
@@ -440,18 +519,20 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       int i = 0;       // tiles so far
       int units = 0;
       bool pending = false;  // the second product of tile i - 1 is still to be issued
+      bool opens = true;     // that tile is its segment's first: O starts from zero
       auto second = [&](int k) {
         const int fill = 2 * k + 1, stage = fill % kStages;
         ok = mbar_wait(&kv_full[stage], (uint32_t)(fill / kStages) & 1, abort_flag);
         ok = ok && mbar_wait(&p_full[k & 1], (uint32_t)(k >> 1) & 1, abort_flag);
         if (!ok) return;
         tc_fence_after_sync();
-        const uint32_t d = tmem_base + 2 * R + (k & 1) * R;
-        const uint32_t a = ring + stage * (kPaTileBytes >> 4), bb = p_lo + (k & 1) * (kPaTileBytes >> 4);
-        umma_ss_f8_lh<0>(d, a, bb, desc_hi, idesc_o);
+        const uint32_t d = tmem_base + 2 * R;
+        const uint32_t a = ring + stage * (kPaTileBytes >> 4), bb = p_lo + (k & 1) * (L::kPBuf >> 4);
+        if (opens) umma_ss_f8_lh<0>(d, a, bb, desc_hi, idesc_o);
+        else umma_ss_f8_lh<1>(d, a, bb, desc_hi, idesc_o);
 #pragma unroll
-        for (int s = 1; s < 8; ++s)  // 32 keys per instruction; then the residual term, 64 bytes further
-          umma_ss_f8_lh<1>(d, a + (s & 3) * 256, bb + (s & 3) * 256 + (s >> 2) * 4, desc_hi, idesc_o);
+        for (int s = 1; s < 8; ++s)  // 32 keys per instruction; then the residual term
+          umma_ss_f8_lh<1>(d, a + (s & 3) * 256, bb + (s & 3) * 256 + (s >> 2) * (L::kPTerm >> 4), desc_hi, s < 4 ? idesc_o : idesc_r);
         umma_commit(&o_full[k & 1]);
         umma_commit(&kv_empty[stage]);
       };
@@ -477,6 +558,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
           umma_commit(&kv_empty[stage]);
           if (pending) second(i - 1);
           pending = true;
+          opens = x == 0;
         }
         ++units;
         t += n_seg;
@@ -490,135 +572,115 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       }
     }
     __syncwarp();
-  } else {
+  } else if (warp >= L::kFirst) {
     // ------------------------------------------------------------------ softmax and output
-    const int sw = warp - 2, g = sw >> 2;     // softmax warp, its group
+    // No early exits in here: a warp whose wait gave up goes on without waiting, so that the named barriers always meet.
+    const int sw = warp - L::kFirst, g = sw >> 2;  // softmax warp, its group
     const int quarter = warp & 3;             // TMEM lanes of this warp
     const int key = quarter * 32 + lane;      // key of the tile; channel of the output
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
+    const uint32_t t_o = tmem_base + lane_base + 2 * R + g * RG;
     const float* scales = reinterpret_cast<const float*>(smem + L::kScales);
-    float* max_sh = reinterpret_cast<float*>(smem + L::kMax);
-    float* row_m = reinterpret_cast<float*>(smem + L::kRowM) + sw * RG;
-    float* row_a = reinterpret_cast<float*>(smem + L::kRowA) + sw * RG;
-    float* row_s_all = reinterpret_cast<float*>(smem + L::kRowS);
-    int* row_pos_all = reinterpret_cast<int*>(smem + L::kRowPos);
-    float* sum_sh = reinterpret_cast<float*>(smem + L::kSum) + g * 4 * RG;
+    float* max_sh = reinterpret_cast<float*>(smem + L::kMax) + g * 4 * RG;
+    float* neg_m = reinterpret_cast<float*>(smem + L::kNegM) + g * RG;     // kPaShift - reference maximum of a row
+    float* factor = reinterpret_cast<float*>(smem + L::kFactor) + g * RG;
+    float* inv_sh = reinterpret_cast<float*>(smem + L::kInv) + sw * RG;
+    int64_t* at_sh = reinterpret_cast<int64_t*>(smem + L::kAt) + sw * RG;
     uint32_t* nan_sh = reinterpret_cast<uint32_t*>(smem + L::kNan);
     uint32_t* nan_any = reinterpret_cast<uint32_t*>(smem + L::kNanAny);
     bool ok = true;
     int i = 0, units = 0;
-    int fixes = 0;                            // boundary tiles so far (phase of fix_bar)
-    int turns = 0;                            // group barriers so far
-    auto group_sync = [&]() {
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&group_bar[g]);
-      ok = ok && mbar_wait(&group_bar[g], turns & 1, abort_flag);
-      ok = __all_sync(0xffffffffu, ok);
-      ++turns;
-    };
-    while (t < st.t1 && ok) {
+    int fixes = 0;                            // boundary tiles so far
+    while (t < st.t1) {
       unit_tiles<R>(p, ent, j, &unit);
       const int n_seg = (int)min((int64_t)(unit.tiles - off), st.t1 - t);
-      float* row_s = row_s_all + (units & 1) * R;
-      int* row_pos = row_pos_all + (units & 1) * R;
+      float* row_s = reinterpret_cast<float*>(smem + L::kRowS) + (units & 1) * R;
+      int* row_pos = reinterpret_cast<int*>(smem + L::kRowPos) + (units & 1) * R;
       // ---- query rows of the unit as two e4m3 terms, each row scaled by a power of two so that its largest entry is in (224, 448]
-#pragma unroll 1
-      for (int r = sw; r < R; r += L::kWarps) {
-        const int flat = unit.first + r;
-        const int tok = flat / p.group;
-        float f[4] = {0.f, 0.f, 0.f, 0.f};
-        if (r < unit.rows) {
-          const uint2 raw = *reinterpret_cast<const uint2*>(p.q + (int64_t)(ent.row0 + tok) * p.q_st + (int64_t)(h * p.group + flat - tok * p.group) * p.q_sh + lane * 4);
-          f[0] = __uint_as_float(raw.x << 16);
-          f[1] = __uint_as_float(raw.x & 0xffff0000u);
-          f[2] = __uint_as_float(raw.y << 16);
-          f[3] = __uint_as_float(raw.y & 0xffff0000u);
+      {
+        constexpr int kMine = R / L::kWarps;
+        uint2 raw[kMine];
+        int toks[kMine];
+#pragma unroll
+        for (int x = 0; x < kMine; ++x) {
+          const int r = sw + x * L::kWarps, flat = unit.first + r, tok = flat / p.group;
+          toks[x] = tok;
+          raw[x] = make_uint2(0, 0);
+          if (r < unit.rows)
+            raw[x] = *reinterpret_cast<const uint2*>(p.q + (int64_t)(ent.row0 + tok) * p.q_st + (int64_t)(h * p.group + flat - tok * p.group) * p.q_sh + lane * 4);
         }
-        const float top = fmaxf(fmaxf(fabsf(f[0]), fabsf(f[1])), fmaxf(fabsf(f[2]), fabsf(f[3])));
-        const bool odd = !(fabsf(f[0]) < INFINITY && fabsf(f[1]) < INFINITY && fabsf(f[2]) < INFINITY && fabsf(f[3]) < INFINITY);
-        const float all = warp_max(top);
-        const uint32_t bits = __float_as_uint(all);
-        // below 2^-92 the entries keep fewer bits: their scores are then below 2^-16 whatever the keys are
-        const int e = max((int)(bits >> 23) - 127 - ((bits & 0x7fffffu) <= 0x600000u ? 8 : 7), -100);
-        const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
-        uint32_t hi = 0, lo = 0;
-        if (__any_sync(0xffffffffu, odd)) {
-          hi = 0x7f7f7f7fu;  // a row with NaN or infinity has no softmax: NaN throughout
-        } else {
-          float res[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) f[k] *= inv;
-          hi = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(f[0], f[1]), __NV_SATFINITE, __NV_E4M3) |
-               (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(f[2], f[3]), __NV_SATFINITE, __NV_E4M3) << 16;
+        for (int x = 0; x < kMine; ++x) {
+          const int r = sw + x * L::kWarps;
+          float f[4] = {__uint_as_float(raw[x].x << 16), __uint_as_float(raw[x].x & 0xffff0000u), __uint_as_float(raw[x].y << 16), __uint_as_float(raw[x].y & 0xffff0000u)};
+          const float top = fmaxf(fmaxf(fabsf(f[0]), fabsf(f[1])), fmaxf(fabsf(f[2]), fabsf(f[3])));
+          const bool odd = !(fabsf(f[0]) < INFINITY && fabsf(f[1]) < INFINITY && fabsf(f[2]) < INFINITY && fabsf(f[3]) < INFINITY);
+          const uint32_t bits = __float_as_uint(warp_max(top));
+          // below 2^-92 the entries keep fewer bits: their scores are then below 2^-16 whatever the keys are
+          const int e = max((int)(bits >> 23) - 127 - ((bits & 0x7fffffu) <= 0x600000u ? 8 : 7), -100);
+          const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
+          uint32_t hi = 0x7f7f7f7fu, lo = 0;  // a row with NaN or infinity has no softmax: NaN throughout
+          if (!__any_sync(0xffffffffu, odd)) {
+            float res[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const __half_raw hr = __nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)(hi >> (8 * k)), __NV_E4M3);
-            res[k] = f[k] - __half2float(*reinterpret_cast<const __half*>(&hr));
+            for (int k = 0; k < 4; ++k) f[k] *= inv;
+            hi = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(f[0], f[1]), __NV_SATFINITE, __NV_E4M3) |
+                 (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(f[2], f[3]), __NV_SATFINITE, __NV_E4M3) << 16;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const __half_raw hr = __nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)(hi >> (8 * k)), __NV_E4M3);
+              res[k] = f[k] - __half2float(*reinterpret_cast<const __half*>(&hr));
+            }
+            lo = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(res[0], res[1]), __NV_SATFINITE, __NV_E4M3) |
+                 (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(res[2], res[3]), __NV_SATFINITE, __NV_E4M3) << 16;
           }
-          lo = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(res[0], res[1]), __NV_SATFINITE, __NV_E4M3) |
-               (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(res[2], res[3]), __NV_SATFINITE, __NV_E4M3) << 16;
+          const int at = r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4;
+          *reinterpret_cast<uint32_t*>(smem + L::kQ + at) = hi;
+          *reinterpret_cast<uint32_t*>(smem + L::kQ + R * 128 + at) = lo;
+          if (lane == 0) {
+            row_s[r] = __uint_as_float((uint32_t)(127 + e) << 23) * p.scale_log2;
+            row_pos[r] = ent.len - ent.n_q + toks[x];
+          }
         }
-        const int at = r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4;
-        *reinterpret_cast<uint32_t*>(smem + L::kQ + at) = hi;
-        *reinterpret_cast<uint32_t*>(smem + L::kQ + R * 128 + at) = lo;
-        if (lane == 0) {
-          row_s[r] = __uint_as_float((uint32_t)(127 + e) << 23) * p.scale_log2;
-          row_pos[r] = ent.len - ent.n_q + tok;
-        }
+        if ((sw & 3) == 0 && lane < RG) neg_m[lane] = INFINITY;
       }
       fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(q_full);
-      ok = mbar_wait(q_full, units & 1, abort_flag);  // the other warps' row scales and positions
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      float m = -INFINITY;  // lane r < RG: running maximum of row r
-      float l[RG], acc[RG];
+      warp_arrive(q_full);
+      ok = warp_wait(ok, q_full, units & 1, abort_flag);  // the other warps' row scales and positions
+      const bool idle = g * RG >= unit.rows;  // a group without rows only keeps step
+      float m = -INFINITY;    // lane r < RG: reference maximum of row r, at most kPaLimit - kPaShift below the running one
+      uint32_t nan_rows = 0;  // rows whose result in this thread's channel is NaN (boundary tiles)
+      uint64_t l2[RG / 2];    // sums over this thread's keys, rows in pairs
 #pragma unroll
-      for (int r = 0; r < RG; ++r) l[r] = acc[r] = 0.f;
-      auto add_output = [&](int k) {  // O^T of tile k: acc = acc * factor(k) + O
-        if (ok) ok = mbar_wait(&o_full[k & 1], (uint32_t)(k >> 1) & 1, abort_flag);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) return;
-        tc_fence_after_sync();
-        uint32_t o[RG];
-        tmem_ld<RG>(tmem_base + lane_base + 2 * R + (k & 1) * R + g * RG, o);
-        tmem_wait_ld();
-        const float4* a4 = reinterpret_cast<const float4*>(row_a + (k & 1) * L::kWarps * RG);
-#pragma unroll
-        for (int r = 0; r < RG; r += 4) {
-          const float4 a = a4[r / 4];
-          acc[r] = fmaf(acc[r], a.x, __uint_as_float(o[r]));
-          acc[r + 1] = fmaf(acc[r + 1], a.y, __uint_as_float(o[r + 1]));
-          acc[r + 2] = fmaf(acc[r + 2], a.z, __uint_as_float(o[r + 2]));
-          acc[r + 3] = fmaf(acc[r + 3], a.w, __uint_as_float(o[r + 3]));
-        }
-      };
+      for (int k = 0; k < RG / 2; ++k) l2[k] = 0;
+      const float4* s4 = reinterpret_cast<const float4*>(row_s + g * RG);
+      const float4* n4 = reinterpret_cast<const float4*>(neg_m);
+#pragma unroll 1
       for (int x = 0; x < n_seg; ++x, ++i) {
         const int k0 = (unit.tile0 + off + x) * kPaTile, pos = k0 + key;
-        ok = mbar_wait(&sc_full[i % kStages], (uint32_t)(i / kStages) & 1, abort_flag);
-        ok = ok && mbar_wait(&s_full[i & 1], (uint32_t)(i >> 1) & 1, abort_flag);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        tc_fence_after_sync();
-        float w[RG];
-        tmem_ld<RG>(tmem_base + lane_base + (i & 1) * R + g * RG, reinterpret_cast<uint32_t*>(w));
-        const float ks = scales[(i % kStages) * 16 + (key >> p.page_shift)];
-        const float vs = scales[(i % kStages) * 16 + 8 + (key >> p.page_shift)];
-        const float bias = log2f(vs), inv_vs = pos < ent.len ? 1.0f / vs : 0.f;  // behind the end there is no page
-        const float4* s4 = reinterpret_cast<const float4*>(row_s + g * RG);
-        tmem_wait_ld();
-#pragma unroll
-        for (int r = 0; r < RG; r += 4) {
-          const float4 s = s4[r / 4];
-          w[r] = fmaf(w[r] * ks, s.x, bias);
-          w[r + 1] = fmaf(w[r + 1] * ks, s.y, bias);
-          w[r + 2] = fmaf(w[r + 2] * ks, s.z, bias);
-          w[r + 3] = fmaf(w[r + 3] * ks, s.w, bias);
+        ok = warp_wait(ok, &sc_full[i % kStages], (uint32_t)(i / kStages) & 1, abort_flag);
+        ok = warp_wait(ok, &s_full[i & 1], (uint32_t)(i >> 1) & 1, abort_flag);
+        const bool tail = k0 + kPaTile > ent.len;                                             // keys behind the sequence's end
+        // keys before it that not every row sees
+        const bool edge = (p.causal && min(k0 + kPaTile, ent.len) - 1 > unit.pos_a) || (p.window > 0 && k0 <= unit.pos_z - p.window);
+        if (G > 1 && idle) {
+          if (edge) {
+            all_sync<32 * L::kWarps>(1 + G);
+            ++fixes;
+          }
+          warp_arrive(&p_full[i & 1]);
+          continue;
         }
-        const bool tail = k0 + kPaTile > ent.len;                                    // keys behind the sequence's end
-        const bool edge = /* keys before it that not every row sees */ (p.causal && min(k0 + kPaTile, ent.len) - 1 > unit.pos_a) || (p.window > 0 && k0 <= unit.pos_z - p.window);
-        if (tail || edge) {
+        tc_fence_after_sync();
+        const uint32_t t_s = tmem_base + lane_base + (i & 1) * R + g * RG;
+        float w[RG];  // exponents of the weights: s log2e + log2(sv) - reference + kPaShift
+        tmem_ld<RG>(t_s, reinterpret_cast<uint32_t*>(w));
+        const float ks = scales[(i % kStages) * 16 + (key >> p.page_shift)];
+        const uint32_t vs = __float_as_uint(scales[(i % kStages) * 16 + 8 + (key >> p.page_shift)]);
+        const float bias = (float)((int)(vs >> 23) - 127);                                    // log2 of a power of two
+        const float inv_vs = pos < ent.len ? __uint_as_float(0x7f000000u - vs) : 0.f;         // behind the end there is no page
+        const uint64_t ks2 = f2_pack(ks, ks), bias2 = f2_pack(bias, bias);
+        auto hide = [&]() {
           const int* rp = row_pos + g * RG;
 #pragma unroll
           for (int r = 0; r < RG; ++r) {
@@ -626,61 +688,111 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
             const bool seen = pos < ent.len && (!p.causal || pos <= at) && (p.window <= 0 || pos > at - p.window);
             if (!seen) w[r] = -INFINITY;
           }
-        }
-        // ---- maximum of each row: over the warp's keys, then over the group's four warps
-        float mine = -INFINITY;
-#pragma unroll
-        for (int r = 0; r < RG; ++r) {
-          const float top = warp_max(w[r]);
-          if (lane == r) mine = top;
-        }
-        float* mx = max_sh + ((i & 1) * G + g) * 4 * RG;
-        if (lane < RG) mx[(sw & 3) * RG + lane] = mine;
-        group_sync();
-        if (!ok) break;
-        if (lane < RG) {
-          const float m_new = fmaxf(fmaxf(fmaxf(m, mx[lane]), mx[RG + lane]), fmaxf(mx[2 * RG + lane], mx[3 * RG + lane]));
-          const float ref = m_new == -INFINITY ? 0.f : m_new;
-          row_m[lane] = ref - kPaShift;
-          row_a[(i & 1) * L::kWarps * RG + lane] = ex2(m - ref);
-          m = m_new;
-        }
-        __syncwarp();
-        // ---- weights, their sum, and P as two e4m3 terms
-        uint32_t hi[RG / 4], lo[RG / 4];
-        const float4* m4 = reinterpret_cast<const float4*>(row_m);
-        const float4* a4 = reinterpret_cast<const float4*>(row_a + (i & 1) * L::kWarps * RG);
+        };
+        tmem_wait_ld();
 #pragma unroll
         for (int r = 0; r < RG; r += 4) {
-          const float4 mm = m4[r / 4], a = a4[r / 4];
-          const float p0 = ex2(w[r] - mm.x), p1 = ex2(w[r + 1] - mm.y), p2 = ex2(w[r + 2] - mm.z), p3 = ex2(w[r + 3] - mm.w);
-          l[r] = fmaf(l[r], a.x, p0 * inv_vs);
-          l[r + 1] = fmaf(l[r + 1], a.y, p1 * inv_vs);
-          l[r + 2] = fmaf(l[r + 2], a.z, p2 * inv_vs);
-          l[r + 3] = fmaf(l[r + 3], a.w, p3 * inv_vs);
-          const __half2 f01 = __floats2half2_rn(p0, p1), f23 = __floats2half2_rn(p2, p3);
-          const __nv_fp8x2_storage_t h01 = __nv_cvt_halfraw2_to_fp8x2(f01, __NV_SATFINITE, __NV_E4M3);
-          const __nv_fp8x2_storage_t h23 = __nv_cvt_halfraw2_to_fp8x2(f23, __NV_SATFINITE, __NV_E4M3);
-          const __half2 d01 = __hsub2(f01, __half2(__nv_cvt_fp8x2_to_halfraw2(h01, __NV_E4M3)));
-          const __half2 d23 = __hsub2(f23, __half2(__nv_cvt_fp8x2_to_halfraw2(h23, __NV_E4M3)));
-          hi[r / 4] = (uint32_t)h01 | (uint32_t)h23 << 16;
-          lo[r / 4] = (uint32_t)__nv_cvt_halfraw2_to_fp8x2(d01, __NV_SATFINITE, __NV_E4M3) |
-                      (uint32_t)__nv_cvt_halfraw2_to_fp8x2(d23, __NV_SATFINITE, __NV_E4M3) << 16;
+          const float4 s = s4[r / 4], n = n4[r / 4];
+          f2_unpack(f2_fma(f2_mul(f2_pack(w[r], w[r + 1]), ks2), f2_pack(s.x, s.y), f2_add(bias2, f2_pack(n.x, n.y))), w[r], w[r + 1]);
+          f2_unpack(f2_fma(f2_mul(f2_pack(w[r + 2], w[r + 3]), ks2), f2_pack(s.z, s.w), f2_add(bias2, f2_pack(n.z, n.w))), w[r + 2], w[r + 3]);
         }
-        uint8_t* pb = smem + L::kP + (i & 1) * kPaTileBytes + key * 128;
+        if (tail || edge) hide();
+        float top = fmaxf(w[0], w[1]);
+#pragma unroll
+        for (int r = 2; r < RG; r += 2) top = max3(top, w[r], w[r + 1]);
+        if (group_any(1 + g, top > kPaLimit)) {
+          // ---- some row's reference is too low (always so in a unit's first tile): the exact maxima, from the scores again
+          tmem_ld<RG>(t_s, reinterpret_cast<uint32_t*>(w));
+          tmem_wait_ld();
+#pragma unroll
+          for (int r = 0; r < RG; r += 4) {
+            const float4 s = s4[r / 4];
+            w[r] = fmaf(w[r] * ks, s.x, bias);
+            w[r + 1] = fmaf(w[r + 1] * ks, s.y, bias);
+            w[r + 2] = fmaf(w[r + 2] * ks, s.z, bias);
+            w[r + 3] = fmaf(w[r + 3] * ks, s.w, bias);
+          }
+          if (tail || edge) hide();
+          float mine = -INFINITY;
+#pragma unroll
+          for (int r = 0; r < RG; ++r) {
+            const float mx = warp_max(w[r]);
+            if (lane == r) mine = mx;
+          }
+          if (lane < RG) max_sh[(sw & 3) * RG + lane] = mine;
+          group_sync(1 + g);
+          if (lane < RG) {
+            const float m_new = fmaxf(fmaxf(fmaxf(m, max_sh[lane]), max_sh[RG + lane]), fmaxf(max_sh[2 * RG + lane], max_sh[3 * RG + lane]));
+            if ((sw & 3) == 0) {
+              neg_m[lane] = kPaShift - m_new;
+              factor[lane] = m_new == -INFINITY ? 1.0f : ex2(m - m_new);
+            }
+            m = m_new;
+          }
+          group_sync(1 + g);
+          const float4* f4 = reinterpret_cast<const float4*>(factor);
+#pragma unroll
+          for (int r = 0; r < RG; r += 4) {
+            const float4 n = n4[r / 4], f = f4[r / 4];
+            w[r] = w[r] == -INFINITY ? w[r] : w[r] + n.x;
+            w[r + 1] = w[r + 1] == -INFINITY ? w[r + 1] : w[r + 1] + n.y;
+            w[r + 2] = w[r + 2] == -INFINITY ? w[r + 2] : w[r + 2] + n.z;
+            w[r + 3] = w[r + 3] == -INFINITY ? w[r + 3] : w[r + 3] + n.w;
+            l2[r / 2] = f2_mul(l2[r / 2], f2_pack(f.x, f.y));
+            l2[r / 2 + 1] = f2_mul(l2[r / 2 + 1], f2_pack(f.z, f.w));
+          }
+          if (x > 0) {  // what the tensor core has summed so far
+            ok = warp_wait(ok, &o_full[(i - 1) & 1], (uint32_t)((i - 1) >> 1) & 1, abort_flag);
+            tc_fence_after_sync();
+#pragma unroll
+            for (int c = 0; c < RG; c += 16) {
+              uint32_t o[16];
+              tmem_ld16(t_o + c, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int r = 0; r < 16; r += 4) {
+                const float4 f = f4[(c + r) / 4];
+                o[r] = __float_as_uint(__uint_as_float(o[r]) * f.x);
+                o[r + 1] = __float_as_uint(__uint_as_float(o[r + 1]) * f.y);
+                o[r + 2] = __float_as_uint(__uint_as_float(o[r + 2]) * f.z);
+                o[r + 3] = __float_as_uint(__uint_as_float(o[r + 3]) * f.w);
+              }
+              tmem_st16(t_o + c, o);
+            }
+            tmem_wait_st();
+          }
+        }
+        // ---- weights, their sum, and P as two e4m3 terms
+        uint32_t hi[RG / 4], lo[RG / 4];
+        const uint64_t inv2 = f2_pack(inv_vs, inv_vs);
+#pragma unroll
+        for (int r = 0; r < RG; r += 4) {
+          const float p0 = ex2(w[r]), p1 = ex2(w[r + 1]), p2 = ex2(w[r + 2]), p3 = ex2(w[r + 3]);
+          l2[r / 2] = f2_fma(f2_pack(p0, p1), inv2, l2[r / 2]);
+          l2[r / 2 + 1] = f2_fma(f2_pack(p2, p3), inv2, l2[r / 2 + 1]);
+          // first term e4m3; what it leaves, exact in fp16, as e5m2: the upper byte of an fp16, rounded
+          const uint32_t h = pack4_e4m3(p0, p1, p2, p3);
+          const __half2 d01 = __hsub2(__floats2half2_rn(p0, p1), __half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)h, __NV_E4M3)));
+          const __half2 d23 = __hsub2(__floats2half2_rn(p2, p3), __half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(h >> 16), __NV_E4M3)));
+          hi[r / 4] = h;
+          lo[r / 4] = __byte_perm(*reinterpret_cast<const uint32_t*>(&d01) + 0x00800080u, *reinterpret_cast<const uint32_t*>(&d23) + 0x00800080u, 0x7531);
+        }
+        // the buffer of tile i - 2
+        if (i >= 2) ok = warp_wait(ok, &o_full[i & 1], (uint32_t)((i - 2) >> 1) & 1, abort_flag);
+        uint8_t* pb = smem + L::kP + key * 128 + (R <= 32 ? 0 : (i & 1) * L::kPBuf);
 #pragma unroll
         for (int c = 0; c < RG / 16; ++c) {
-          const int chunk = g * (RG / 16) + c;  // 16 rows of the R
-          *reinterpret_cast<uint4*>(pb + ((chunk ^ (key & 7)) << 4)) = make_uint4(hi[4 * c], hi[4 * c + 1], hi[4 * c + 2], hi[4 * c + 3]);
-          *reinterpret_cast<uint4*>(pb + (((chunk + 4) ^ (key & 7)) << 4)) = make_uint4(lo[4 * c], lo[4 * c + 1], lo[4 * c + 2], lo[4 * c + 3]);
+          const int chunk = R <= 32 ? (i & 1) * 2 + c : g * (RG / 16) + c;  // 16 rows of the R
+          const int at0 = (chunk ^ (key & 7)) << 4, at1 = R <= 32 ? ((chunk + 4) ^ (key & 7)) << 4 : L::kPTerm + at0;
+          *reinterpret_cast<uint4*>(pb + at0) = make_uint4(hi[4 * c], hi[4 * c + 1], hi[4 * c + 2], hi[4 * c + 3]);
+          *reinterpret_cast<uint4*>(pb + at1) = make_uint4(lo[4 * c], lo[4 * c + 1], lo[4 * c + 2], lo[4 * c + 3]);
         }
         if (tail || edge) {
           // A weight of zero does not silence a NaN: V of keys behind the end becomes zero, and NaN codes of keys that only
-          // some rows see are taken out of the product and put into the accumulators of the rows that do see them.
+          // some rows see are taken out of the product and come back through the sums of the rows that do see them.
           const int v_fill = 2 * i + 1, v_stage = v_fill % kStages;
-          ok = mbar_wait(&kv_full[v_stage], (uint32_t)(v_fill / kStages) & 1, abort_flag);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
+          ok = warp_wait(ok, &kv_full[v_stage], (uint32_t)(v_fill / kStages) & 1, abort_flag);
+          __syncwarp();
           uint4* vrow = reinterpret_cast<uint4*>(smem + L::kRing + v_stage * kPaTileBytes + key * 128);
           if (g == 0) {
             if (pos >= ent.len) {
@@ -690,19 +802,18 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
             if (edge) {
               uint32_t nan_bits[4] = {0, 0, 0, 0};
               if (pos < ent.len) {
-#pragma unroll 1
+#pragma unroll
                 for (int c = 0; c < 8; ++c) {
                   const uint4 q = vrow[c ^ (key & 7)];
                   const uint32_t wd[4] = {q.x, q.y, q.z, q.w};
                   uint32_t kept[4];
-                  bool any = false;
+                  uint32_t any = 0;
 #pragma unroll
                   for (int k = 0; k < 4; ++k) {
                     const uint32_t is = __vcmpeq4(wd[k] & 0x7f7f7f7fu, 0x7f7f7f7fu);
                     kept[k] = wd[k] & ~is;
-                    any = any || is;
-                    const uint32_t four = (is & 1u) | (is >> 7 & 2u) | (is >> 14 & 4u) | (is >> 21 & 8u);
-                    nan_bits[c >> 1] |= four << ((c & 1) * 16 + k * 4);
+                    any |= is;
+                    nan_bits[c >> 1] |= ((is & 1u) | (is >> 7 & 2u) | (is >> 14 & 4u) | (is >> 21 & 8u)) << ((c & 1) * 16 + k * 4);
                   }
                   if (any) vrow[c ^ (key & 7)] = make_uint4(kept[0], kept[1], kept[2], kept[3]);
                 }
@@ -713,11 +824,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
             }
           }
           if (edge) {
-            __syncwarp();
-            if (lane == 0) mbar_arrive(fix_bar);
-            ok = mbar_wait(fix_bar, fixes & 1, abort_flag);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
+            all_sync<32 * L::kWarps>(1 + G);
             const uint32_t* any = nan_any + (fixes & 1) * 4;
             if (any[0] | any[1] | any[2] | any[3]) {
               // this thread's channel: the rows that see a key whose V is NaN there
@@ -726,10 +833,10 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
               for (int kk = 0; kk < kPaTile; ++kk) {
                 if (!(words[kk * 4] >> lane & 1u)) continue;
                 const int at_key = k0 + kk;
-#pragma unroll
+#pragma unroll 1
                 for (int r = 0; r < RG; ++r) {
                   const int at = row_pos[g * RG + r];
-                  if ((!p.causal || at_key <= at) && (p.window <= 0 || at_key > at - p.window)) acc[r] = __uint_as_float(0x7fffffffu);
+                  if ((!p.causal || at_key <= at) && (p.window <= 0 || at_key > at - p.window)) nan_rows |= 1u << r;
                 }
               }
             }
@@ -738,48 +845,66 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
         }
         fence_proxy_async_smem();
         tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[i & 1]);
-        if (x > 0) {
-          add_output(i - 1);
-          if (!ok) break;
+        warp_arrive(&p_full[i & 1]);
+      }
+      // ---- the accumulator, the sum over the keys, then the result or what another block needs to go on
+      ok = warp_wait(ok, &o_full[(i - 1) & 1], (uint32_t)((i - 1) >> 1) & 1, abort_flag);
+      tc_fence_after_sync();
+      float o[RG];
+      tmem_ld<RG>(t_o, reinterpret_cast<uint32_t*>(o));
+      {
+        float v[RG];
+#pragma unroll
+        for (int k = 0; k < RG / 2; ++k) f2_unpack(l2[k], v[2 * k], v[2 * k + 1]);
+        // halves of the rows change lanes while the sums are formed: lane x ends with row x (RG = 32) or x / 2 (RG = 16)
+        int width = RG;
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) {
+          if (width > 1) {
+            width >>= 1;
+#pragma unroll
+            for (int k = 0; k < RG / 2; ++k)
+              if (k < width) {
+                const float send = lane & d ? v[k] : v[k + width], keep = lane & d ? v[k + width] : v[k];
+                v[k] = keep + __shfl_xor_sync(0xffffffffu, send, d);
+              }
+          } else {
+            v[0] += __shfl_xor_sync(0xffffffffu, v[0], d);
+          }
         }
+        if (RG == 32 || (lane & 1) == 0) max_sh[(sw & 3) * RG + (RG == 32 ? lane : lane >> 1)] = v[0];
       }
-      if (ok) add_output(i - 1);
-      if (!ok) break;
-      // ---- sum over the keys, then the result or what another block needs to go on
-      float mine = 0.f;
-#pragma unroll
-      for (int r = 0; r < RG; ++r) {
-        float s = l[r];
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-        if (lane == r) mine = s;
-      }
-      if (lane < RG) sum_sh[(sw & 3) * RG + lane] = mine;
-      group_sync();
-      if (!ok) break;
+      group_sync(1 + g);
       const int row = g * RG + lane;  // of lanes < RG
-      const float total = lane < RG ? (sum_sh[lane] + sum_sh[RG + lane]) + (sum_sh[2 * RG + lane] + sum_sh[3 * RG + lane]) : 0.f;
+      const float total = lane < RG ? (max_sh[lane] + max_sh[RG + lane]) + (max_sh[2 * RG + lane] + max_sh[3 * RG + lane]) : 0.f;
+      tmem_wait_ld();
+      if (nan_rows) {
+#pragma unroll
+        for (int r = 0; r < RG; ++r)
+          if (nan_rows >> r & 1u) o[r] = __uint_as_float(0x7fffffffu);
+      }
       if (off == 0 && n_seg == unit.tiles) {
         const bool owned = lane < RG && row < unit.rows;
         const int flat = unit.first + (owned ? row : 0), tok = flat / p.group, head = h * p.group + flat - tok * p.group;
-        const float inv = total != 0.f ? 1.0f / total : 0.f;  // nothing seen: zero
-        if (owned && p.lse && (sw & 3) == 0)
-          p.lse[(int64_t)(ent.row0 + tok) * p.hq + head] = total != 0.f ? (m - kPaShift + log2f(total)) * 0.6931471805599453f : -INFINITY;
-        const long long at = (int64_t)(ent.row0 + tok) * p.o_st + (int64_t)head * p.o_sh;
-#pragma unroll
-        for (int r = 0; r < RG; ++r) {
-          const float f = __shfl_sync(0xffffffffu, inv, r);
-          const long long o = __shfl_sync(0xffffffffu, at, r);
-          if (g * RG + r < unit.rows) p.out[o + key] = __float2bfloat16_rn(acc[r] * f);
+        if (owned && ok) {
+          if (p.lse && (sw & 3) == 0)
+            p.lse[(int64_t)(ent.row0 + tok) * p.hq + head] = total != 0.f ? (m - kPaShift + log2f(total)) * 0.6931471805599453f : -INFINITY;
         }
+        if (lane < RG) {
+          inv_sh[lane] = total != 0.f ? 1.0f / total : 0.f;  // nothing seen: zero
+          at_sh[lane] = (int64_t)(ent.row0 + tok) * p.o_st + (int64_t)head * p.o_sh;
+        }
+        __syncwarp();
+#pragma unroll
+        for (int r = 0; r < RG; ++r)
+          if (ok && g * RG + r < unit.rows) p.out[at_sh[r] + key] = __float2bfloat16_rn(o[r] * inv_sh[r]);
+        __syncwarp();
       } else {
         const int64_t slot = 2 * (int64_t)blockIdx.x + (off == 0 ? 1 : 0);
         float* part = p.parts + slot * R * kHeadDim + (int64_t)g * RG * kHeadDim;
 #pragma unroll
         for (int r = 0; r < RG; ++r)
-          if (g * RG + r < unit.rows) part[r * kHeadDim + key] = acc[r];
+          if (g * RG + r < unit.rows) part[r * kHeadDim + key] = o[r];
         if ((sw & 3) == 0 && lane < RG) p.stats[slot * R + row] = make_float2(m, total);
         if (off == 0 && sw == 0 && lane == 0)
           p.headers[blockIdx.x] = {1, b, h, j, (int)((t + unit.tiles - 1) / st.per_block), {0, 0, 0}};
@@ -857,14 +982,14 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
 }
 
 // ---------------------------------------------------------------------------------------------- host side
-// Up to 16 rows per kv head (one token of up to 16 query heads each): the small form, two blocks per SM; else 64 rows.
-static bool small_form(int64_t max_q, int group) { return max_q * group <= 16; }
+// Rows of a block's unit: up to 16 or 32 (query tokens times heads of a group) fit a form of which an SM holds two blocks;
+// more go 96 at a time through the large one.
+static int form_rows(int64_t max_q, int group) { return max_q * group <= 16 ? 16 : max_q * group <= 32 ? 32 : 96; }
+static int form_blocks(const magi_ctx* ctx, int rows) { return ctx->sm_count * (rows == 96 ? 1 : 2); }
 
-static int64_t part_slots(const magi_ctx* ctx, bool small) { return 2 * (int64_t)ctx->sm_count * (small ? 2 : 1); }
-
-static int64_t workspace_bytes(const magi_ctx* ctx, bool small) {
-  const int64_t slots = part_slots(ctx, small);
-  return slots / 2 * (int64_t)sizeof(PaHeader) + slots * (small ? 16 : 64) * (kHeadDim * 4 + 8);
+static int64_t workspace_bytes(const magi_ctx* ctx, int rows) {
+  const int64_t blocks = form_blocks(ctx, rows);
+  return blocks * (int64_t)sizeof(PaHeader) + 2 * blocks * rows * (kHeadDim * 4 + 8);
 }
 
 template <int RG, int G>
@@ -875,7 +1000,7 @@ static int launch_paged(magi_ctx* ctx, const CUtensorMap& tk, const CUtensorMap&
     MAGI_CUDA_OK(ctx, cudaFuncSetAttribute(paged_attn_kernel<RG, G>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kDynamic));
     if (ctx->device < 64) configured[ctx->device] = true;
   }
-  const int blocks = ctx->sm_count * (G == 1 ? 2 : 1);
+  const int blocks = form_blocks(ctx, L::kRows);
   paged_attn_kernel<RG, G><<<blocks, L::kThreads, L::kDynamic, st>>>(tk, tv, k);
   MAGI_CUDA_OK(ctx, cudaGetLastError());
   const int64_t rows = (int64_t)k.max_q * k.group;
@@ -896,7 +1021,7 @@ static int launch_paged(magi_ctx* ctx, const CUtensorMap& tk, const CUtensorMap&
 
 extern "C" int64_t magi_paged_attn_workspace_bytes(magi_ctx* ctx, int32_t max_q, int32_t n_q_heads, int32_t n_kv_heads) {
   if (!ctx || max_q < 0 || n_q_heads <= 0 || n_kv_heads <= 0 || n_q_heads % n_kv_heads) return 0;
-  return magi::workspace_bytes(ctx, magi::small_form(max_q, n_q_heads / n_kv_heads));
+  return magi::workspace_bytes(ctx, magi::form_rows(max_q, n_q_heads / n_kv_heads));
 }
 
 extern "C" int magi_paged_attn_fwd(magi_ctx* ctx, const magi_token_cache* cache, const magi_paged_attn_params* p, void* stream) {
@@ -939,14 +1064,16 @@ extern "C" int magi_paged_attn_fwd(magi_ctx* ctx, const magi_token_cache* cache,
   DeviceScope dev(ctx);
   while ((1 << k.page_shift) < k.c.page_tokens) ++k.page_shift;
   k.rows_total = k.c.n_layers * k.c.n_pages * k.c.n_kv_heads * k.c.page_tokens;
-  const bool small = small_form(p->max_q, k.group);
-  const int64_t slots = part_slots(ctx, small);
+  const int rows = form_rows(p->max_q, k.group);
+  const int64_t blocks = form_blocks(ctx, rows);
   k.headers = static_cast<PaHeader*>(p->workspace);
-  k.parts = reinterpret_cast<float*>(k.headers + slots / 2);
-  k.stats = reinterpret_cast<float2*>(k.parts + slots * (small ? 16 : 64) * kHeadDim);
+  k.parts = reinterpret_cast<float*>(k.headers + blocks);
+  k.stats = reinterpret_cast<float2*>(k.parts + 2 * blocks * rows * kHeadDim);
   CUtensorMap tk, tv;
   if (int rc = make_rows_map(ctx, &tk, cache->k8, k.rows_total, k.c.page_tokens, "paged attn k8")) return rc;
   if (int rc = make_rows_map(ctx, &tv, cache->v8, k.rows_total, k.c.page_tokens, "paged attn v8")) return rc;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  return small ? launch_paged<16, 1>(ctx, tk, tv, k, st) : launch_paged<32, 2>(ctx, tk, tv, k, st);
+  if (rows == 16) return launch_paged<16, 1>(ctx, tk, tv, k, st);
+  if (rows == 32) return launch_paged<32, 1>(ctx, tk, tv, k, st);
+  return launch_paged<32, 3>(ctx, tk, tv, k, st);
 }

@@ -178,9 +178,10 @@ def attention(books, layer, q, seqs, cu, hkv, scale=None, causal=True, window=0)
     owns are NaN in out.
 
     tol bounds what the kernel's own roundings may do to an exact computation:
-      * P as fp16 (2^-11) in two e4m3 terms: each rounding is off by at most 2^-4 of the value, so both by 2^-8, and by no more than
-        2^-10 / 2^8 = 2^-18 of the largest weight at the subnormal end: |do| <= (2^-8 + 2^-11) sum p|v| + 2^-18 sum |v| / l, where l
-        is the sum of the weights relative to the largest;
+      * P as e4m3 plus residual as e5m2: the first rounding leaves at most 2^-4 of the value, the second is off by at most
+        2^-3 of that: 2^-7, and fp16 in between by 2^-11.  Where the first term is subnormal it leaves at most 2^-10, of which
+        the second loses 2^-13, and the largest weight of a row is at least 2^5: 2^-18 of it.
+        |do| <= (2^-7 + 2^-11) sum p|v| + 2^-18 sum |v| / l, where l is the sum of the weights relative to the largest;
       * Q in two e4m3 terms, each row scaled so that its largest entry lies in (224, 448]: 16 (two 4-bit) significand bits
         hold bf16's 8 exactly, except that what lies below 2^-10 / 224 < 2^-17 of the row's largest entry is lost:
         |ds| <= scale * 2^-17 max|q| * sum_d |k_d|, which changes a weight by a factor of at most exp(2 |ds|);
@@ -213,7 +214,7 @@ def attention(books, layer, q, seqs, cu, hkv, scale=None, causal=True, window=0)
                     ds = scale * 2.0 ** -17 * np.abs(qq).max(1, keepdims=True) * np.abs(kk).sum(1).max()
                     a = w @ np.abs(vv) / l
                     out[cu[i] + r, heads], lse[cu[i] + r, heads] = o, (top + np.log(l))[:, 0]
-                    tol[cu[i] + r, heads] = 2.0 ** -8 * np.abs(o) + (2.0 ** -8 + 2.0 ** -11 + 2 * ds + 2.0 ** -14) * a + 2.0 ** -18 * np.abs(vv).sum(0) / l
+                    tol[cu[i] + r, heads] = 2.0 ** -8 * np.abs(o) + (2.0 ** -7 + 2.0 ** -11 + 2 * ds + 2.0 ** -14) * a + 2.0 ** -18 * np.abs(vv).sum(0) / l
                     tol_l[cu[i] + r, heads] = (ds + 2.0 ** -16 + 2.0 ** -20 * np.abs(top))[:, 0]
     return out, lse, tol, tol_l
 

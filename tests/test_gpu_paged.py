@@ -544,3 +544,29 @@ def test_arguments_are_checked():
             bad()
     assert mb.paged_attn(q[:0], c, 0, i32([]))[0].shape == (0, 4, 128)
     assert status() == 0
+
+
+def test_a_long_tail_behind_one_large_weight():
+    """One key takes about half of the softmax, 60000 others share the rest: their weights, 2^-16 of the largest, must not
+    be rounded away.  Values: 0 at the large key, 1 elsewhere."""
+    import magi_b200 as mb
+    n = 60001
+    c = make_cache([n], 128, 1, seed=30, poison=False)
+    ids = c.page_table[0].long()
+    c.k8.view(torch.uint8).zero_()
+    c.v8.view(torch.uint8).fill_(0x38)          # 1.0
+    c.k_scale.fill_(1.0), c.v_scale.fill_(1.0)
+    q = torch.zeros(1, 6, 128, dtype=torch.bfloat16, device="cuda")
+    q[0, :, 0] = 12.0
+    for where in (0, 5000, n - 1):
+        c.k8.view(torch.uint8).zero_()
+        c.v8.view(torch.uint8).fill_(0x38)
+        page, off = int(ids[where // 128]), where % 128
+        c.k8.view(torch.uint8)[0, page, 0, off, 0] = 0x52   # 10.0: the score 12 * 10 / sqrt(128) = 10.607 nats = 15.3 bits
+        c.v8.view(torch.uint8)[0, page, 0, off] = 0
+        out, lse = mb.paged_attn(q, c, 0, i32([0]))
+        big = math.exp(12 * 10 / math.sqrt(128))
+        want = (n - 1) / (n - 1 + big)
+        # every small weight is the same number and rounds the same way, by at most 2^-3 of it (e5m2): the bound of the result
+        assert abs(float(out.double().mean()) - want) <= (2.0 ** -8 + 2.0 ** -3) * want
+        assert abs(float(lse[0, 0]) - math.log(n - 1 + big)) <= 1e-4
