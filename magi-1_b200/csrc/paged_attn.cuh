@@ -1,0 +1,432 @@
+// Shared by the attention kernels over the token-paged cache: how a call is seen on the device, how its 128-key tiles are
+// dealt out to the blocks, the walk over a block's part, the loading warp, and warp-level helpers.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include "paged.cuh"
+#include "ptx_sm100.cuh"
+
+namespace magi {
+using namespace ptx;
+
+constexpr int kPaTile = 128;                   // keys of a tile
+constexpr int kPaTileBytes = kPaTile * kHeadDim;
+constexpr int kPromptRows = 256;               // query rows of a block in the prompt form
+constexpr int kPaNear = 64;                    // entries whose lengths a block keeps in shared memory
+// P = 2^(w - reference + 5).  The reference of a row is the exact maximum when it is set and stays while no weight exceeds
+// e4m3's 448 = 2^8.8, that is until the maximum has grown 14-fold: nearly every tile then needs one vote of the group in
+// place of its maxima, and the tensor core goes on summing in TMEM.  The residual term is e5m2, whose smallest step is 2^-16:
+// a weight is dropped only below 2^-22 of the reference, so a long tail of small weights behind one large one keeps its mass.
+constexpr float kPaShift = 5.0f, kPaLimit = 8.8f;
+
+struct PagedAttnKernelParams {
+  PagedView c;
+  int layer;
+  const __nv_bfloat16* q;
+  int64_t q_st, q_sh;
+  __nv_bfloat16* out;
+  int64_t o_st, o_sh;
+  float* lse;
+  const int32_t* seqs;
+  const int32_t* cu_q;
+  int n, total_q, max_q, hq, group;
+  float scale_log2;
+  int causal, window;
+  int* status;
+  int page_shift;      // log2(page_tokens)
+  int rows_total;      // rows of the tensor maps
+  struct PaHeader* headers;  // [blocks]
+  float* parts;        // [blocks][2][rows][128] accumulators of units that lie in several blocks
+  float2* stats;       // [blocks][2][rows] their maximum and sum
+};
+
+// What a block leaves behind about its last unit, when others continue it.
+struct PaHeader {
+  int open;        // 1: the unit starts in this block and ends in block `last`
+  int b, h, j;     // entry, kv head, row tile
+  int last;
+  int pad[3];
+};
+
+// One entry of the call as the kernels see it; rows and lengths that make no sense count as none.
+struct PaEntry {
+  int seq, len, row0, n_q;
+};
+
+__device__ __forceinline__ PaEntry load_entry(const PagedAttnKernelParams& p, int b, bool* bad) {
+  PaEntry e;
+  e.seq = p.seqs[b];
+  e.row0 = p.cu_q ? p.cu_q[b] : b;
+  e.n_q = p.cu_q ? p.cu_q[b + 1] - e.row0 : 1;
+  e.len = 0;
+  bool wrong = false;
+  if (e.n_q < 0 || e.n_q > p.max_q || e.row0 < 0 || (int64_t)e.row0 + e.n_q > p.total_q) {
+    wrong = true;
+    e.n_q = 0;
+  }
+  if (e.seq >= 0 && e.seq < p.c.max_seqs) {
+    e.len = p.c.lens[e.seq];
+    const int64_t room = (int64_t)p.c.per_row << p.page_shift;
+    if (e.len < 0 || e.len > room) {
+      wrong = true;
+      e.len = 0;
+    }
+  } else {
+    wrong = true;
+    e.seq = 0;
+  }
+  *bad = wrong;
+  return e;
+}
+
+// Row tile j of an entry: query rows (token, head of the group) flattened, kRows at a time.
+struct PaUnit {
+  int first, rows;      // flattened rows [first, first + rows)
+  int pos_a, pos_z;     // positions of its first and last token
+  int tile0, tiles;     // 128-key tiles that some row may see; at least one, so that rows that see nothing are written
+};
+
+template <int kRows>
+__device__ __forceinline__ int unit_tiles(const PagedAttnKernelParams& p, const PaEntry& e, int j, PaUnit* u) {
+  const int first = j * kRows;
+  const int rows = min(kRows, e.n_q * p.group - first);
+  const int pos_a = e.len - e.n_q + first / p.group;
+  const int pos_z = e.len - e.n_q + (first + rows - 1) / p.group;
+  const int end = p.causal ? pos_z + 1 : e.len;
+  const int begin = p.window > 0 ? max(0, pos_a - p.window + 1) : 0;
+  int tile0 = 0, tiles = 1;
+  if (end > begin) {
+    tile0 = begin / kPaTile;
+    tiles = (end + kPaTile - 1) / kPaTile - tile0;
+  }
+  if (u) *u = {first, rows, pos_a, pos_z, tile0, tiles};
+  return tiles;
+}
+
+template <int kRows>
+__device__ __forceinline__ int row_tiles(const PagedAttnKernelParams& p, const PaEntry& e) {
+  return (e.n_q * p.group + kRows - 1) / kRows;
+}
+
+// Where a block's part of the tiles starts; every role walks from there by itself.
+struct PaStart {
+  int64_t t0, t1;       // tiles [t0, t1)
+  int64_t per_block;
+  int b, h, j, off;     // unit and tile within it
+};
+
+__device__ __forceinline__ void tma_load_2d(void* smem_dst, const CUtensorMap* m, uint64_t* bar, int c0, int c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+      ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(c0), "r"(c1)
+      : "memory");
+}
+__device__ __forceinline__ void cp_async_4(void* smem_dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(smem_dst)), "l"(src) : "memory");
+}
+// One arrival on the barrier once this thread's earlier cp.async have landed.
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ uint32_t pack4_e4m3(float a, float b, float c, float d) {
+  return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3) |
+         (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3) << 16;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// Largest value over the warp, NaN left out.
+__device__ __forceinline__ float warp_max(float v) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));  // volatile: not to be moved under a branch
+  return r;
+}
+
+// A whole warp waits, its lanes staying together: lane 0 asks, by predicate and not by branch, and the warp votes.  (32 lanes
+// asking for one barrier are served one after the other, about 200 cycles a question; a branch on the lane leaves lane 0
+// behind on its own, and the warp-wide instructions that follow need all lanes at once.)
+__device__ __forceinline__ bool warp_wait(bool ok, uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  if (!ok) return false;
+  const uint32_t addr = smem_u32(bar), lane = threadIdx.x & 31;
+  long long t0 = 0;
+  while (true) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred l, p;\n\t"
+        "setp.eq.u32 l, %3, 0;\n\t"
+        "setp.ne.u32 p, %3, %3;\n\t"
+        "@l mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %4;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(addr), "r"(parity), "r"(lane), "r"((uint32_t)MAGI_WAIT_HINT_NS)
+        : "memory");
+    if (__any_sync(0xffffffffu, done)) break;
+    const long long now = clock64();
+    if (t0 == 0) t0 = now;
+    const bool late = now - t0 > 1000000000LL;
+    if (__any_sync(0xffffffffu, late)) *abort_flag = 1;
+    __syncwarp();
+    if (__any_sync(0xffffffffu, *abort_flag != 0)) return false;
+  }
+  __syncwarp();  // what lane 0 has seen is there for the others
+  return true;
+}
+// One arrival for the warp, after what all its lanes did before.
+__device__ __forceinline__ void warp_arrive(uint64_t* bar) {
+  __syncwarp();
+  asm volatile(
+      "{\n\t.reg .pred l;\n\t"
+      "setp.eq.u32 l, %1, 0;\n\t"
+      "@l mbarrier.arrive.shared::cta.b64 _, [%0];\n\t}"
+      ::"r"(smem_u32(bar)), "r"(threadIdx.x & 31)
+      : "memory");
+}
+
+// Which tiles are this block's: the tiles of all units in a row, dealt out in equal contiguous parts.  Whole block; scratch
+// needs kPlanScratch bytes.  The caller puts a barrier behind it.
+constexpr int kPlanScratch = (8 + (int)sizeof(PaEntry)) * kPgMaxEntries;
+template <int R, int kThreads>
+__device__ __forceinline__ void plan_tiles(const PagedAttnKernelParams& p, uint8_t* scratch, PaStart* start, PaEntry* near) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hkv = p.c.n_kv_heads;
+  int64_t* sums = reinterpret_cast<int64_t*>(scratch);  // [n] tiles of an entry, then their prefix sums
+  PaEntry* entries = reinterpret_cast<PaEntry*>(scratch + 8 * kPgMaxEntries);
+  const bool single = (int64_t)p.max_q * p.group <= R;                   // one row tile per entry
+  bool any_bad = false;
+  for (int b = threadIdx.x; b < p.n; b += kThreads) {
+    bool bad;
+    const PaEntry e = load_entry(p, b, &bad);
+    any_bad |= bad;
+    entries[b] = e;
+    if (single) sums[b] = e.n_q > 0 ? (int64_t)unit_tiles<R>(p, e, 0, nullptr) * hkv : 0;
+  }
+  if (any_bad && blockIdx.x == 0) *p.status = MAGI_E_RANGE;
+  __syncthreads();
+  if (!single) {
+    for (int b = warp; b < p.n; b += kThreads / 32) {
+      const PaEntry e = entries[b];
+      const int n_j = row_tiles<R>(p, e);
+      int64_t w = 0;
+      for (int j = lane; j < n_j; j += 32) w += unit_tiles<R>(p, e, j, nullptr);
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) w += __shfl_xor_sync(0xffffffffu, w, d);
+      if (lane == 0) sums[b] = w * hkv;
+    }
+    __syncthreads();
+  }
+  if (warp == 0) {
+    int64_t carry = 0;
+    for (int b0 = 0; b0 < p.n; b0 += 32) {
+      int64_t x = b0 + lane < p.n ? sums[b0 + lane] : 0;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, x, d);
+        if (lane >= d) x += y;
+      }
+      if (b0 + lane < p.n) sums[b0 + lane] = carry + x;
+      carry += __shfl_sync(0xffffffffu, x, 31);
+    }
+    __syncwarp();
+    const int64_t total = carry;
+    const int64_t per_block = (total + gridDim.x - 1) / gridDim.x;
+    const int64_t t0 = min((int64_t)blockIdx.x * per_block, total), t1 = min(t0 + per_block, total);
+    if (t0 < t1) {
+      int b = 0;  // first entry whose sum exceeds t0
+      for (int b0 = 0; b0 < p.n; b0 += 32) {
+        const bool over = b0 + lane < p.n && sums[b0 + lane] > t0;
+        const uint32_t m = __ballot_sync(0xffffffffu, over);
+        if (m) {
+          b = b0 + __ffs(m) - 1;
+          break;
+        }
+      }
+      const int64_t before = b > 0 ? sums[b - 1] : 0;
+      const int64_t per_head = (sums[b] - before) / hkv;
+      const int h = (int)((t0 - before) / per_head);
+      int64_t rem = (t0 - before) - h * per_head;
+      int j = 0;
+      if (!single) {
+        const PaEntry e = entries[b];
+        const int n_j = row_tiles<R>(p, e);
+        for (int j0 = 0; j0 < n_j; j0 += 32) {
+          const int64_t mine = j0 + lane < n_j ? unit_tiles<R>(p, e, j0 + lane, nullptr) : 0;
+          int64_t x = mine;
+#pragma unroll
+          for (int d = 1; d < 32; d <<= 1) {
+            const int64_t y = __shfl_up_sync(0xffffffffu, x, d);
+            if (lane >= d) x += y;
+          }
+          const uint32_t m = __ballot_sync(0xffffffffu, x > rem);
+          if (m) {
+            const int f = __ffs(m) - 1;
+            rem -= __shfl_sync(0xffffffffu, x - mine, f);
+            j = j0 + f;
+            break;
+          }
+          rem -= __shfl_sync(0xffffffffu, x, 31);
+        }
+      }
+      for (int i = lane; i < kPaNear; i += 32)
+        if (b + i < p.n) near[i] = entries[b + i];
+      if (lane == 0) *start = {t0, t1, per_block, b, h, j, (int)rem};
+    } else if (lane == 0) {
+      *start = {t0, t0, per_block, 0, 0, 0, 0};
+    }
+    if (lane == 0) p.headers[blockIdx.x].open = 0;
+  }
+}
+
+// The walk over a block's segments (a segment = the tiles of one unit that are its own), the same in every role.
+template <int R>
+struct PaWalk {
+  const PagedAttnKernelParams& p;
+  const PaEntry* near;
+  int64_t t, t1;
+  int b, h, j, off, b0, n_j, n_seg;
+  PaEntry ent;
+  PaUnit unit;
+
+  __device__ __forceinline__ PaWalk(const PagedAttnKernelParams& params, const PaStart& st, const PaEntry* entries)
+      : p(params), near(entries), t(st.t0), t1(st.t1), b(st.b), h(st.h), j(st.j), off(st.off), b0(st.b) {
+    if (t < t1) fetch();
+  }
+  __device__ __forceinline__ void fetch() {
+    if (b - b0 < kPaNear) ent = near[b - b0];
+    else {
+      bool bad;
+      ent = load_entry(p, b, &bad);
+    }
+    n_j = row_tiles<R>(p, ent);
+  }
+  // The current segment: its unit and number of tiles; false behind the last one.
+  __device__ __forceinline__ bool segment() {
+    if (t >= t1) return false;
+    unit_tiles<R>(p, ent, j, &unit);
+    n_seg = (int)min((int64_t)(unit.tiles - off), t1 - t);
+    return true;
+  }
+  __device__ __forceinline__ void advance() {
+    t += n_seg;
+    if (t >= t1) return;
+    off = 0;
+    if (++j < n_j) return;
+    j = 0;
+    if (++h < p.c.n_kv_heads) return;
+    h = 0;
+    do {
+      if (++b >= p.n) return;
+      fetch();
+    } while (n_j == 0);
+  }
+};
+
+// The loading warp: the pages of K and V of every tile into a ring of 16 KB stages (K of tile i is fill 2i, V 2i + 1), the
+// scales of its pages by cp.async into slot i % kSlots.
+template <int R, int kStages, int kSlots>
+__device__ __forceinline__ void load_tiles(const PagedAttnKernelParams& p, PaWalk<R>& w, const CUtensorMap* tm_k, const CUtensorMap* tm_v,
+                                           uint8_t* ring, float* scales, uint64_t* kv_full, uint64_t* kv_empty, uint64_t* sc_full,
+                                           volatile int* abort_flag) {
+  const int lane = threadIdx.x & 31;
+  const int P = p.c.page_tokens, per_tile = kPaTile >> p.page_shift;
+  int fill = 0;
+  bool ok = true;
+  for (; w.segment() && ok; w.advance()) {
+    const int32_t* row = p.c.table + (int64_t)w.ent.seq * p.c.per_row;
+    const int first_page = (w.unit.tile0 + w.off) * per_tile;
+    const int pages = (int)(((int64_t)w.ent.len + P - 1) >> p.page_shift);  // pages that hold tokens
+    int ahead = lane < per_tile && first_page + lane < pages ? row[first_page + lane] : -1;
+    for (int i = 0; i < w.n_seg && ok; ++i) {
+      const int page0 = first_page + i * per_tile;
+      const bool mine = lane < per_tile && page0 + lane < pages;
+      const int id = ahead;
+      const int next = page0 + per_tile + lane;
+      ahead = i + 1 < w.n_seg && lane < per_tile && next < pages ? row[next] : -1;  // in flight while this tile is loaded
+      const bool lost = mine && (id < 0 || id >= p.c.n_pages);
+      if (lost) *p.status = MAGI_E_RANGE;
+      const int n_load = min(per_tile, max(0, pages - page0));
+      // a page that does not exist is read behind the last row, which fills zeros
+      const int64_t block = lost ? 0 : ((int64_t)p.layer * p.c.n_pages + max(id, 0)) * p.c.n_kv_heads + w.h;
+      const int y = lost ? p.rows_total : (int)(block << p.page_shift);
+      const int slot = (fill >> 1) % kSlots;
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv, ++fill) {
+        const int stage = fill % kStages, use = fill / kStages;
+        if (use > 0) ok = warp_wait(ok, &kv_empty[stage], (use & 1) ^ 1, abort_flag);
+        if (!ok) break;
+        if (lane == 0) mbar_expect_tx(&kv_full[stage], n_load << (p.page_shift + 7));
+        __syncwarp();
+        if (mine) tma_load_2d(ring + stage * kPaTileBytes + (lane << (p.page_shift + 7)), kv ? tm_v : tm_k, &kv_full[stage], 0, y);
+        if (kv == 0) {
+          if (mine) {
+            cp_async_4(scales + slot * 16 + lane, p.c.k_scale + block);
+            cp_async_4(scales + slot * 16 + 8 + lane, p.c.v_scale + block);
+          }
+          cp_async_arrive(&sc_full[slot]);
+        }
+        __syncwarp();
+      }
+    }
+  }
+  if (!ok) {  // given up: let the copies in flight land before the block leaves
+    int late = 0;
+    for (int f = max(0, fill - kStages); f < fill; ++f) mbar_wait(&kv_full[f % kStages], (f / kStages) & 1, &late, 100000000LL);
+  }
+  __syncwarp();
+}
+
+// Four bf16 of a query row (a lane's share of its 128 channels) as two e4m3 terms, the row scaled by the power of two that
+// brings its largest entry into (224, 448].  Returns that power's inverse; whole warp, one row.
+__device__ __forceinline__ float split_query(uint2 raw, uint32_t* hi, uint32_t* lo) {
+  float f[4] = {__uint_as_float(raw.x << 16), __uint_as_float(raw.x & 0xffff0000u), __uint_as_float(raw.y << 16), __uint_as_float(raw.y & 0xffff0000u)};
+  const float top = fmaxf(fmaxf(fabsf(f[0]), fabsf(f[1])), fmaxf(fabsf(f[2]), fabsf(f[3])));
+  const bool odd = !(fabsf(f[0]) < INFINITY && fabsf(f[1]) < INFINITY && fabsf(f[2]) < INFINITY && fabsf(f[3]) < INFINITY);
+  const uint32_t bits = __float_as_uint(warp_max(top));
+  // below 2^-92 the entries keep fewer bits: their scores are then below 2^-16 whatever the keys are
+  const int e = max((int)(bits >> 23) - 127 - ((bits & 0x7fffffu) <= 0x600000u ? 8 : 7), -100);
+  const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
+  float res[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) f[k] *= inv;
+  uint32_t h = pack4_e4m3(f[0], f[1], f[2], f[3]);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const __half_raw hr = __nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)(h >> (8 * k)), __NV_E4M3);
+    res[k] = f[k] - __half2float(*reinterpret_cast<const __half*>(&hr));
+  }
+  const bool any_odd = __any_sync(0xffffffffu, odd);  // a row with NaN or infinity has no softmax: NaN throughout
+  *hi = any_odd ? 0x7f7f7f7fu : h;
+  *lo = any_odd ? 0u : pack4_e4m3(res[0], res[1], res[2], res[3]);
+  return __uint_as_float((uint32_t)(127 + e) << 23);
+}
+
+// P of four keys (or rows) as e4m3 and, of what that leaves (exact in fp16), as e5m2: the upper byte of an fp16, rounded.
+__device__ __forceinline__ void split_weights(float p0, float p1, float p2, float p3, uint32_t* hi, uint32_t* lo) {
+  const uint32_t h = pack4_e4m3(p0, p1, p2, p3);
+  const __half2 d01 = __hsub2(__floats2half2_rn(p0, p1), __half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)h, __NV_E4M3)));
+  const __half2 d23 = __hsub2(__floats2half2_rn(p2, p3), __half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(h >> 16), __NV_E4M3)));
+  *hi = h;
+  *lo = __byte_perm(*reinterpret_cast<const uint32_t*>(&d01) + 0x00800080u, *reinterpret_cast<const uint32_t*>(&d23) + 0x00800080u, 0x7531);
+}
+
+// Row `key` of a V tile in shared memory: its NaN codes become zero, their places go to bits (channel c: word c / 32).
+__device__ __forceinline__ void take_nan(uint4* vrow, int key, uint32_t (&bits)[4]) {
+#pragma unroll
+  for (int c = 0; c < 8; ++c) {
+    const uint4 q = vrow[c ^ (key & 7)];
+    const uint32_t wd[4] = {q.x, q.y, q.z, q.w};
+    uint32_t kept[4], any = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t is = __vcmpeq4(wd[k] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+      kept[k] = wd[k] & ~is;
+      any |= is;
+      bits[c >> 1] |= ((is & 1u) | (is >> 7 & 2u) | (is >> 14 & 4u) | (is >> 21 & 8u)) << ((c & 1) * 16 + k * 4);
+    }
+    if (any) vrow[c ^ (key & 7)] = make_uint4(kept[0], kept[1], kept[2], kept[3]);
+  }
+}
+
+}  // namespace magi

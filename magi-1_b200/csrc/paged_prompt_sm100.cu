@@ -1,0 +1,417 @@
+// Attention over the token-paged 8-bit cache, prompt form: more than 32 query rows per kv head, for sm_100a.
+//
+// Same products, precision and work split as the few-row form (paged_attn_sm100.cu), with the rows across: S [128 rows x 128
+// keys] = Q K8^T and O [128 rows x 128 channels] = P V8, a thread owning a row.  Maximum, reference and sum of a row then live
+// in its thread, no vote or barrier is needed between tiles, and the fixed cost of a tile (barriers, tensor memory latency) is
+// spread over 128 elements of each thread: with the keys across it was 32, and a tile of 96 rows took 4900 cycles, of which
+// 900 were tensor core work.
+//
+// A block works on 256 rows (query tokens times the heads of a kv head, flattened), 128 for each of two softmax warpgroups that
+// take turns on the tensor core.  K and V tiles are read once for all 256 rows.  P goes back over S in TMEM, as e4m3 in columns
+// 0-31 and its e5m2 residual in 32-63, and is the A operand of the second product from there.
+//   warp 0 TMA, warp 1 UMMA issuer, warps 4-11 softmax (warpgroup x: rows 128 x ..), warps 2, 3 idle
+//   TMEM columns: S of warpgroup 0, 1 at 0, 128; O at 256, 384
+#include "paged_attn.cuh"
+
+namespace magi {
+
+int launch_prompt_join(magi_ctx* ctx, const PagedAttnKernelParams& k, cudaStream_t st);
+
+struct PromptShared {
+  static constexpr int kStages = 8;
+  static constexpr int kSlots = 8;                             // tiles whose page scales are kept
+  static constexpr int kThreads = 384;
+  static constexpr int kRing = 0;
+  static constexpr int kQ = kRing + kStages * kPaTileBytes;    // [2 terms][2 warpgroups][128 rows][128 bytes]
+  static constexpr int kScales = kQ + 4 * kPaTileBytes;        // [kSlots][2][8]
+  static constexpr int kNan = kScales + kSlots * 64;           // [2][128][4] channels whose V is NaN (boundary tiles)
+  static constexpr int kNanAny = kNan + 2 * kPaTile * 16;      // [2][4] whether a warp's keys have any
+  static constexpr int kNear = kNanAny + 32;
+  static constexpr int kStart = kNear + kPaNear * 16;
+  static constexpr int kBar = kStart + 64;
+  static constexpr int kNumBars = 2 * kStages + kSlots + 9;
+  static constexpr int kMisc = kBar + kNumBars * 8;
+  static constexpr int kDynamic = kMisc + 16 + 1024;
+};
+static_assert(PromptShared::kDynamic <= 232448, "shared memory per block");
+static_assert(PromptShared::kStages * kPaTileBytes >= kPlanScratch, "the plan's scratch is in the ring");
+
+template <int kThreads>
+__device__ __forceinline__ void named_sync(int id) {
+  __syncwarp();
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(kThreads) : "memory");
+}
+
+__global__ void __launch_bounds__(PromptShared::kThreads, 1)
+paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                    const __grid_constant__ PagedAttnKernelParams p) {
+  using L = PromptShared;
+  constexpr int R = kPromptRows, kStages = L::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* kv_full = reinterpret_cast<uint64_t*>(smem + L::kBar);
+  uint64_t* kv_empty = kv_full + kStages;
+  uint64_t* sc_full = kv_empty + kStages;
+  uint64_t* q_full = sc_full + L::kSlots;  // [2] by warpgroup, as the next three
+  uint64_t* s_full = q_full + 2;
+  uint64_t* p_full = s_full + 2;
+  uint64_t* o_full = p_full + 2;
+  uint64_t* drain_bar = o_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kMisc);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kMisc + 4);
+  PaStart* start = reinterpret_cast<PaStart*>(smem + L::kStart);
+  PaEntry* near = reinterpret_cast<PaEntry*>(smem + L::kNear);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&kv_full[s], 1);
+      mbar_init(&kv_empty[s], 1);
+    }
+    for (int s = 0; s < L::kSlots; ++s) mbar_init(&sc_full[s], 32);  // each lane of the loading warp
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(&q_full[x], 4);
+      mbar_init(&s_full[x], 1);
+      mbar_init(&p_full[x], 4);
+      mbar_init(&o_full[x], 1);
+    }
+    mbar_init(drain_bar, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  plan_tiles<R, L::kThreads>(p, smem + L::kRing, start, near);
+  fence_proxy_async_smem();  // the ring goes over to TMA
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_slot;
+  const PaStart st = *start;
+  PaWalk<R> walk(p, st, near);
+
+  if (warp == 0) {
+    if (lane == 0) {
+      tma_prefetch_desc(&tm_k);
+      tma_prefetch_desc(&tm_v);
+    }
+    __syncwarp();
+    load_tiles<R, kStages, L::kSlots>(p, walk, &tm_k, &tm_v, smem + L::kRing, reinterpret_cast<float*>(smem + L::kScales), kv_full, kv_empty, sc_full, abort_flag);
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ UMMA issuer
+    if (lane == 0) {
+      constexpr uint32_t idesc_s = umma_idesc(128, kPaTile, 0, 0, 0, 0);
+      constexpr uint32_t idesc_o = umma_idesc(128, kHeadDim, 0, 0, 0, 1), idesc_r = umma_idesc(128, kHeadDim, 1, 0, 0, 1);  // A e4m3, e5m2
+      constexpr uint32_t desc_hi = (1024u >> 4) | (1u << 14) | (2u << 29);  // 1024 bytes between groups of 8 rows, 128-byte swizzle
+      const uint32_t ring = (smem_u32(smem + L::kRing) >> 4) | (1u << 16);
+      const uint32_t q_lo = (smem_u32(smem + L::kQ) >> 4) | (1u << 16);
+      constexpr uint32_t kTile16 = kPaTileBytes >> 4;
+      bool ok = true;
+      int i = 0;                       // tiles so far
+      int seen[2] = {0, 0}, units[2] = {0, 0};  // tiles and units of each warpgroup
+      auto first = [&](int x, int fill) {  // S of warpgroup x
+        const uint32_t a = q_lo + x * kTile16, b = ring + (fill % kStages) * kTile16, d = tmem_base + x * 128;
+        umma_ss_f8_lh<0>(d, a, b, desc_hi, idesc_s);
+#pragma unroll
+        for (int s = 1; s < 8; ++s)  // 32 channels per instruction; then the residual term
+          umma_ss_f8_lh<1>(d, a + (s & 3) * 2 + (s >> 2) * 2 * kTile16, b + (s & 3) * 2, desc_hi, idesc_s);
+        umma_commit(&s_full[x]);
+      };
+      for (; ok && walk.segment(); walk.advance()) {
+        const int nx = walk.unit.rows > 128 ? 2 : 1;
+        ok = mbar_wait(&kv_full[(2 * i) % kStages], (uint32_t)(2 * i / kStages) & 1, abort_flag);
+        for (int x = 0; x < nx && ok; ++x) {
+          ok = mbar_wait(&q_full[x], units[x]++ & 1, abort_flag);
+          if (!ok) break;
+          tc_fence_after_sync();
+          first(x, 2 * i);
+        }
+        if (ok) umma_commit(&kv_empty[(2 * i) % kStages]);
+        for (int k = 0; k < walk.n_seg && ok; ++k, ++i) {
+          const bool more = k + 1 < walk.n_seg;
+          const int v_fill = 2 * i + 1, k_fill = 2 * i + 2;
+          ok = mbar_wait(&kv_full[v_fill % kStages], (uint32_t)(v_fill / kStages) & 1, abort_flag);
+          if (ok && more) ok = mbar_wait(&kv_full[k_fill % kStages], (uint32_t)(k_fill / kStages) & 1, abort_flag);
+          for (int x = 0; x < nx && ok; ++x) {
+            ok = mbar_wait(&p_full[x], seen[x]++ & 1, abort_flag);
+            if (!ok) break;
+            tc_fence_after_sync();
+            const uint32_t b = ring + (v_fill % kStages) * kTile16, d = tmem_base + 256 + x * 128, a = tmem_base + x * 128;
+            if (k == 0) umma_ts_f8_lh<0>(d, a, b, desc_hi, idesc_o);
+            else umma_ts_f8_lh<1>(d, a, b, desc_hi, idesc_o);
+#pragma unroll
+            for (int s = 1; s < 8; ++s)  // 32 keys per instruction: 8 columns of P, 32 rows of V; then the residual term
+              umma_ts_f8_lh<1>(d, a + s * 8, b + (s & 3) * 256, desc_hi, s < 4 ? idesc_o : idesc_r);
+            if (!more) umma_commit(&o_full[x]);
+            if (x == nx - 1) umma_commit(&kv_empty[v_fill % kStages]);
+            if (more) {
+              first(x, k_fill);
+              if (x == nx - 1) umma_commit(&kv_empty[k_fill % kStages]);
+            }
+          }
+        }
+      }
+      if (!ok) {  // given up: the instructions issued so far still read shared memory and write TMEM
+        int late = 0;
+        umma_commit(drain_bar);
+        mbar_wait(drain_bar, 0, &late, 100000000LL);
+      }
+    }
+    __syncwarp();
+  } else if (warp >= 4) {
+    // ------------------------------------------------------------------ softmax and output
+    // No early exits in here: a warp whose wait gave up goes on without waiting, so that the named barriers always meet.
+    const int x = (warp - 4) >> 2, quarter = warp & 3;
+    const int row = quarter * 32 + lane;  // of the warpgroup's 128; also the key whose V row this thread looks after (x = 0)
+    const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
+    const uint32_t t_s = tmem_base + lane_base + x * 128, t_o = t_s + 256;
+    const float* scales = reinterpret_cast<const float*>(smem + L::kScales);
+    uint4* nan_sh = reinterpret_cast<uint4*>(smem + L::kNan);
+    volatile uint32_t* nan_any = reinterpret_cast<uint32_t*>(smem + L::kNanAny);
+    bool ok = true;
+    int i = 0;                 // tiles of the block so far
+    int seen = 0, units = 0;   // tiles and units of this warpgroup
+    for (; walk.segment(); walk.advance()) {
+      const PaUnit& unit = walk.unit;
+      const PaEntry& ent = walk.ent;
+      const int n_seg = walk.n_seg, off = walk.off;
+      const int nx = unit.rows > 128 ? 2 : 1;
+      if (x >= nx) {  // a short unit leaves the second warpgroup out
+        i += n_seg;
+        continue;
+      }
+      // ---- this warp's 32 query rows as two e4m3 terms
+      float row_scale = 0.f;
+      const int flat = unit.first + x * 128 + row;
+      const int tok = flat / p.group, head = walk.h * p.group + flat - tok * p.group;
+      const bool owned = x * 128 + row < unit.rows;
+      const long long q_at = (int64_t)(ent.row0 + tok) * p.q_st + (int64_t)head * p.q_sh;
+#pragma unroll 1
+      for (int r0 = 0; r0 < 32; r0 += 8) {
+        uint2 raw[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          const long long at = __shfl_sync(0xffffffffu, q_at, r0 + r);
+          raw[r] = make_uint2(0, 0);
+          if (x * 128 + quarter * 32 + r0 + r < unit.rows) raw[r] = *reinterpret_cast<const uint2*>(p.q + at + lane * 4);
+        }
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          uint32_t hi, lo;
+          const float scale = split_query(raw[r], &hi, &lo);
+          const int tr = quarter * 32 + r0 + r;
+          uint8_t* at = smem + L::kQ + x * kPaTileBytes + tr * 128 + (((lane >> 2) ^ (tr & 7)) << 4) + (lane & 3) * 4;
+          *reinterpret_cast<uint32_t*>(at) = hi;
+          *reinterpret_cast<uint32_t*>(at + 2 * kPaTileBytes) = lo;
+          row_scale = lane == r0 + r ? scale : row_scale;
+        }
+      }
+      fence_proxy_async_smem();
+      warp_arrive(&q_full[x]);
+      const float c1 = row_scale * p.scale_log2;
+      const uint64_t c2 = f2_pack(c1, c1);
+      const int at_pos = ent.len - ent.n_q + tok;
+      float m = -INFINITY;                  // reference maximum, at most kPaLimit - kPaShift below the running one
+      uint64_t l2 = 0;                      // sum of the weights, two halves
+      uint32_t nan_ch[4] = {0, 0, 0, 0};    // channels of this row that are NaN (boundary tiles)
+#pragma unroll 1
+      for (int k = 0; k < n_seg; ++k, ++i, ++seen) {
+        const int k0 = (unit.tile0 + off + k) * kPaTile;
+        ok = warp_wait(ok, &sc_full[i % L::kSlots], (uint32_t)(i / L::kSlots) & 1, abort_flag);
+        ok = warp_wait(ok, &s_full[x], seen & 1, abort_flag);
+        tc_fence_after_sync();
+        float s[kPaTile];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32(t_s + c * 32, reinterpret_cast<uint32_t*>(s) + c * 32);
+        const float* sc = scales + (i % L::kSlots) * 16;
+        const bool tail = k0 + kPaTile > ent.len;  // keys behind the sequence's end
+        // keys before it that not every row sees
+        const bool edge = (p.causal && min(k0 + kPaTile, ent.len) - 1 > unit.pos_a) || (p.window > 0 && k0 <= unit.pos_z - p.window);
+        const int last = min(p.causal ? at_pos : ent.len - 1, ent.len - 1) - k0;               // columns [begin, last] are seen
+        const int begin = p.window > 0 ? max(at_pos - p.window + 1 - k0, 0) : 0;
+        auto hide = [&]() {
+#pragma unroll
+          for (int c = 0; c < kPaTile; ++c)
+            if (c > last || c < begin) s[c] = -INFINITY;
+        };
+        // exponents of the weights: s log2e + log2(sv) + plus, the scales by groups of 16 keys (a page is a multiple of that)
+        auto exponents = [&](float plus) {
+#pragma unroll
+          for (int g = 0; g < 8; ++g) {
+            const int pg = (g * 16) >> p.page_shift;
+            const float ks = sc[pg];
+            const float b = (float)((int)(__float_as_uint(sc[8 + pg]) >> 23) - 127) + plus;
+            const uint64_t ks2 = f2_pack(ks, ks), b2 = f2_pack(b, b);
+#pragma unroll
+            for (int c = g * 16; c < g * 16 + 16; c += 2) f2_unpack(f2_fma(f2_mul(f2_pack(s[c], s[c + 1]), ks2), c2, b2), s[c], s[c + 1]);
+          }
+          if (tail || edge) hide();
+        };
+        auto largest = [&]() {
+          float top[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+          for (int c = 4; c < 124; c += 8) {
+            top[0] = max3(top[0], s[c], s[c + 1]);
+            top[1] = max3(top[1], s[c + 2], s[c + 3]);
+            top[2] = max3(top[2], s[c + 4], s[c + 5]);
+            top[3] = max3(top[3], s[c + 6], s[c + 7]);
+          }
+          top[0] = max3(top[0], s[124], s[125]);
+          top[1] = max3(top[1], s[126], s[127]);
+          return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        };
+        tmem_wait_ld();
+        exponents(kPaShift - m);
+        const float over = largest();
+        const bool need = over > kPaLimit;
+        if (__any_sync(0xffffffffu, need)) {
+          // ---- some row's reference is too low (always so in a unit's first tile): its exact maximum, from the scores again
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_ld32(t_s + c * 32, reinterpret_cast<uint32_t*>(s) + c * 32);
+          tmem_wait_ld();
+          exponents(0.f);
+          const float m_new = need ? fmaxf(m, largest()) : m;
+          const float f = need ? ex2(m - m_new) : 1.0f;
+          m = m_new;
+          const float plus = kPaShift - m_new;
+#pragma unroll
+          for (int c = 0; c < kPaTile; ++c) s[c] = s[c] == -INFINITY ? s[c] : s[c] + plus;
+          l2 = f2_mul(l2, f2_pack(f, f));
+          if (k > 0) {  // what the tensor core has summed so far: this tile's scores were issued behind it
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+              uint32_t o[32];
+              tmem_ld32(t_o + c * 32, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int q = 0; q < 32; ++q) o[q] = __float_as_uint(__uint_as_float(o[q]) * f);
+              tmem_st32(t_o + c * 32, o);
+            }
+          }
+        }
+        // ---- weights, their sum, and P as two terms over the scores
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          uint32_t hi[8], lo[8];
+#pragma unroll
+          for (int c4 = 0; c4 < 8; ++c4) {
+            const int c = q * 32 + c4 * 4;
+            const uint32_t vs = __float_as_uint(sc[8 + (c >> 4 << 4 >> p.page_shift)]);
+            const float inv = c <= last ? __uint_as_float(0x7f000000u - vs) : 0.f;  // behind the end there may be no page
+            const uint64_t inv2 = f2_pack(inv, inv);
+            const float p0 = ex2(s[c]), p1 = ex2(s[c + 1]), p2 = ex2(s[c + 2]), p3 = ex2(s[c + 3]);
+            l2 = f2_fma(f2_pack(p0, p1), inv2, l2);
+            l2 = f2_fma(f2_pack(p2, p3), inv2, l2);
+            split_weights(p0, p1, p2, p3, &hi[c4], &lo[c4]);
+          }
+          tmem_st8(t_s + q * 8, hi);
+          tmem_st8(t_s + 32 + q * 8, lo);
+        }
+        if (tail || edge) {
+          // A weight of zero does not silence a NaN: V of keys behind the end becomes zero, and NaN codes of keys that only
+          // some rows see are taken out of the product and come back in the rows that do see them.
+          const int v_fill = 2 * i + 1, buf = i & 1;
+          if (x == 0) {
+            ok = warp_wait(ok, &kv_full[v_fill % kStages], (uint32_t)(v_fill / kStages) & 1, abort_flag);
+            uint4* vrow = reinterpret_cast<uint4*>(smem + L::kRing + (v_fill % kStages) * kPaTileBytes + row * 128);
+            if (k0 + row >= ent.len) {
+#pragma unroll
+              for (int c = 0; c < 8; ++c) vrow[c] = make_uint4(0, 0, 0, 0);
+            }
+            if (edge) {
+              uint32_t bits[4] = {0, 0, 0, 0};
+              if (k0 + row < ent.len) take_nan(vrow, row, bits);
+              nan_sh[buf * kPaTile + row] = make_uint4(bits[0], bits[1], bits[2], bits[3]);
+              nan_any[buf * 4 + quarter] = __any_sync(0xffffffffu, (bits[0] | bits[1] | bits[2] | bits[3]) != 0);  // every lane the same
+            }
+            fence_proxy_async_smem();
+          }
+          if (edge) {
+            if (nx == 2) named_sync<256>(2);
+            else named_sync<128>(1);
+            const volatile uint32_t* any = nan_any + buf * 4;
+            if (any[0] | any[1] | any[2] | any[3]) {
+#pragma unroll 1
+              for (int kk = max(begin, 0); kk <= min(last, kPaTile - 1); ++kk) {
+                const uint4 w = nan_sh[buf * kPaTile + kk];
+                nan_ch[0] |= w.x;
+                nan_ch[1] |= w.y;
+                nan_ch[2] |= w.z;
+                nan_ch[3] |= w.w;
+              }
+              __syncwarp();
+            }
+          }
+        }
+        tmem_wait_st();
+        tc_fence_before_sync();
+        warp_arrive(&p_full[x]);
+      }
+      // ---- the result, or what another block needs to go on
+      ok = warp_wait(ok, &o_full[x], units & 1, abort_flag);
+      ++units;
+      tc_fence_after_sync();
+      float l0, l1;
+      f2_unpack(l2, l0, l1);
+      const float total = l0 + l1;
+      const bool whole = off == 0 && n_seg == unit.tiles;
+      const float inv = whole ? (total != 0.f ? 1.0f / total : 0.f) : 1.0f;  // nothing seen: zero
+      const int64_t slot = (2 * (int64_t)blockIdx.x + (off == 0 ? 1 : 0)) * R + x * 128 + row;
+      __nv_bfloat16* out = p.out + (int64_t)(ent.row0 + (owned ? tok : 0)) * p.o_st + (int64_t)head * p.o_sh;
+      float* part = p.parts + slot * kHeadDim;
+#pragma unroll 1
+      for (int c = 0; c < 4; ++c) {
+        float o[32];
+        tmem_ld32(t_o + c * 32, reinterpret_cast<uint32_t*>(o));
+        tmem_wait_ld();
+        const uint32_t nan_bits = c == 0 ? nan_ch[0] : c == 1 ? nan_ch[1] : c == 2 ? nan_ch[2] : nan_ch[3];
+#pragma unroll
+        for (int q = 0; q < 32; ++q) o[q] = nan_bits >> q & 1u ? __uint_as_float(0x7fffffffu) : o[q] * inv;
+        if (owned && ok) {
+          if (whole) {
+#pragma unroll
+            for (int q = 0; q < 32; q += 8)
+              *reinterpret_cast<uint4*>(out + c * 32 + q) = make_uint4(pack_bf16x2(o[q], o[q + 1]), pack_bf16x2(o[q + 2], o[q + 3]), pack_bf16x2(o[q + 4], o[q + 5]), pack_bf16x2(o[q + 6], o[q + 7]));
+          } else {
+#pragma unroll
+            for (int q = 0; q < 32; q += 4) *reinterpret_cast<float4*>(part + c * 32 + q) = make_float4(o[q], o[q + 1], o[q + 2], o[q + 3]);
+          }
+        }
+        __syncwarp();
+      }
+      if (owned) {
+        if (!whole) p.stats[slot] = make_float2(m, total);
+        else if (p.lse && ok)
+          p.lse[(int64_t)(ent.row0 + tok) * p.hq + head] = total != 0.f ? (m - kPaShift + log2f(total)) * 0.6931471805599453f : -INFINITY;
+      }
+      if (!whole && off == 0 && threadIdx.x == 128)
+        p.headers[blockIdx.x] = {1, walk.b, walk.h, walk.j, (int)((walk.t + unit.tiles - 1) / st.per_block), {0, 0, 0}};
+      __syncwarp();
+    }
+  }
+
+  // ------------------------------------------------------------------ teardown
+  tc_fence_before_sync();
+  __syncthreads();
+  if (*abort_flag && threadIdx.x == 0) *p.status = MAGI_E_TIMEOUT;
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
+int launch_paged_prompt(magi_ctx* ctx, const CUtensorMap& tk, const CUtensorMap& tv, const PagedAttnKernelParams& k, cudaStream_t st) {
+  static bool configured[64] = {};  // per device: opt in to > 48 KB of dynamic shared memory once
+  if (ctx->device >= 64 || !configured[ctx->device]) {
+    MAGI_CUDA_OK(ctx, cudaFuncSetAttribute(paged_prompt_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PromptShared::kDynamic));
+    if (ctx->device < 64) configured[ctx->device] = true;
+  }
+  paged_prompt_kernel<<<ctx->sm_count, PromptShared::kThreads, PromptShared::kDynamic, st>>>(tk, tv, k);
+  MAGI_CUDA_OK(ctx, cudaGetLastError());
+  return launch_prompt_join(ctx, k, st);
+}
+
+}  // namespace magi

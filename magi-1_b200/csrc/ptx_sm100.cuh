@@ -233,6 +233,17 @@ __device__ __forceinline__ void umma_ts_f16_lh(uint32_t d_tmem, uint32_t a_tmem,
       ::"r"(d_tmem), "r"(a_tmem), "r"(b_lo), "r"(desc_hi), "r"(idesc), "n"(kAccumulate)
       : "memory");
 }
+// The same for e4m3 / e5m2 operands (K = 32 per instruction).
+template <int kAccumulate>
+__device__ __forceinline__ void umma_ts_f8_lh(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t desc_hi, uint32_t idesc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\t"
+      "mov.b64 db, {%2, %3};\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], [%1], db, %4, p;\n\t}"
+      ::"r"(d_tmem), "r"(a_tmem), "r"(b_lo), "r"(desc_hi), "r"(idesc), "n"(kAccumulate)
+      : "memory");
+}
 // Pair form: issued by one thread of the even CTA of a pair; M = 256 rows (128 per CTA, each CTA's A tile and half of
 // the B tile at the same shared-memory offset in both), the accumulator at the same tensor-memory address in both.
 template <int kAccumulate>
