@@ -3,12 +3,11 @@
 // Same products, precision and work split as the few-row form (paged_attn_sm100.cu), with the rows across: S [128 rows x 128
 // keys] = Q K8^T and O [128 rows x 128 channels] = P V8, a thread owning a row.  Maximum, reference and sum of a row then live
 // in its thread, no vote or barrier is needed between tiles, and the fixed cost of a tile (barriers, tensor memory latency) is
-// spread over 128 elements of each thread: with the keys across it was 32, and a tile of 96 rows took 4900 cycles, of which
-// 900 were tensor core work.
+// spread over 128 elements of each thread instead of 32.
 //
 // A block works on 256 rows (query tokens times the heads of a kv head, flattened), 128 for each of two softmax warpgroups that
-// take turns on the tensor core.  K and V tiles are read once for all 256 rows.  P goes back over S in TMEM, as e4m3 in columns
-// 0-31 and its e5m2 residual in 32-63, and is the A operand of the second product from there.
+// take turns on the tensor core.  K and V tiles are read once for all 256 rows.  P goes back over S in TMEM (32 keys: 8 columns
+// of e4m3, 8 of the e5m2 residual) and is the A operand of the second product from there.
 //   warp 0 TMA, warp 1 UMMA issuer, warps 4-11 softmax (warpgroup x: rows 128 x ..), warps 2, 3 idle
 //   TMEM columns: S of warpgroup 0, 1 at 0, 128; O at 256, 384
 #include "paged_attn.cuh"
@@ -144,7 +143,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             else umma_ts_f8_lh<1>(d, a, b, desc_hi, idesc_o);
 #pragma unroll
             for (int s = 1; s < 8; ++s)  // 32 keys per instruction: 8 columns of P, 32 rows of V; then the residual term
-              umma_ts_f8_lh<1>(d, a + s * 8, b + (s & 3) * 256, desc_hi, s < 4 ? idesc_o : idesc_r);
+              umma_ts_f8_lh<1>(d, a + (s & 3) * 16 + (s >> 2) * 8, b + (s & 3) * 256, desc_hi, s < 4 ? idesc_o : idesc_r);
             if (!more) umma_commit(&o_full[x]);
             if (x == nx - 1) umma_commit(&kv_empty[v_fill % kStages]);
             if (more) {
@@ -212,10 +211,9 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
       fence_proxy_async_smem();
       warp_arrive(&q_full[x]);
       const float c1 = row_scale * p.scale_log2;
-      const uint64_t c2 = f2_pack(c1, c1);
       const int at_pos = ent.len - ent.n_q + tok;
       float m = -INFINITY;                  // reference maximum, at most kPaLimit - kPaShift below the running one
-      uint64_t l2 = 0;                      // sum of the weights, two halves
+      float l = 0.f;                        // sum of the weights
       uint32_t nan_ch[4] = {0, 0, 0, 0};    // channels of this row that are NaN (boundary tiles)
 #pragma unroll 1
       for (int k = 0; k < n_seg; ++k, ++i, ++seen) {
@@ -223,63 +221,52 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         ok = warp_wait(ok, &sc_full[i % L::kSlots], (uint32_t)(i / L::kSlots) & 1, abort_flag);
         ok = warp_wait(ok, &s_full[x], seen & 1, abort_flag);
         tc_fence_after_sync();
-        float s[kPaTile];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32(t_s + c * 32, reinterpret_cast<uint32_t*>(s) + c * 32);
         const float* sc = scales + (i % L::kSlots) * 16;
         const bool tail = k0 + kPaTile > ent.len;  // keys behind the sequence's end
         // keys before it that not every row sees
         const bool edge = (p.causal && min(k0 + kPaTile, ent.len) - 1 > unit.pos_a) || (p.window > 0 && k0 <= unit.pos_z - p.window);
         const int last = min(p.causal ? at_pos : ent.len - 1, ent.len - 1) - k0;               // columns [begin, last] are seen
         const int begin = p.window > 0 ? max(at_pos - p.window + 1 - k0, 0) : 0;
-        auto hide = [&]() {
-#pragma unroll
-          for (int c = 0; c < kPaTile; ++c)
-            if (c > last || c < begin) s[c] = -INFINITY;
+        // 32 keys at a time, twice over (the scores stay in TMEM in between): the loop bodies then stay small enough for the
+        // instruction cache, and a thread holds 32 scores instead of 128.
+        // w = s log2e + log2(sv) = raw * kc + bias, the scales by groups of 16 keys (a page is a multiple of that)
+        auto factors = [&](int c, float* kc, float* bias, float* inv) {
+          const int pg = c >> p.page_shift;
+          const uint32_t vs = __float_as_uint(sc[8 + pg]);
+          *kc = fminf(sc[pg] * c1, 3.0e38f);  // finite: a raw score of zero stays zero
+          *bias = (float)((int)(vs >> 23) - 127);
+          *inv = c <= last ? __uint_as_float(0x7f000000u - vs) : 0.f;  // behind the end there may be no page
         };
-        // exponents of the weights: s log2e + log2(sv) + plus, the scales by groups of 16 keys (a page is a multiple of that)
-        auto exponents = [&](float plus) {
-#pragma unroll
-          for (int g = 0; g < 8; ++g) {
-            const int pg = (g * 16) >> p.page_shift;
-            const float ks = sc[pg];
-            const float b = (float)((int)(__float_as_uint(sc[8 + pg]) >> 23) - 127) + plus;
-            const uint64_t ks2 = f2_pack(ks, ks), b2 = f2_pack(b, b);
-#pragma unroll
-            for (int c = g * 16; c < g * 16 + 16; c += 2) f2_unpack(f2_fma(f2_mul(f2_pack(s[c], s[c + 1]), ks2), c2, b2), s[c], s[c + 1]);
-          }
-          if (tail || edge) hide();
-        };
-        auto largest = [&]() {
-          float top[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-          for (int c = 4; c < 124; c += 8) {
-            top[0] = max3(top[0], s[c], s[c + 1]);
-            top[1] = max3(top[1], s[c + 2], s[c + 3]);
-            top[2] = max3(top[2], s[c + 4], s[c + 5]);
-            top[3] = max3(top[3], s[c + 6], s[c + 7]);
-          }
-          top[0] = max3(top[0], s[124], s[125]);
-          top[1] = max3(top[1], s[126], s[127]);
-          return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-        };
-        tmem_wait_ld();
-        exponents(kPaShift - m);
-        const float over = largest();
-        const bool need = over > kPaLimit;
-        if (__any_sync(0xffffffffu, need)) {
-          // ---- some row's reference is too low (always so in a unit's first tile): its exact maximum, from the scores again
-#pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_ld32(t_s + c * 32, reinterpret_cast<uint32_t*>(s) + c * 32);
+        float top = -INFINITY;
+#pragma unroll 1
+        for (int c0 = 0; c0 < kPaTile; c0 += 32) {
+          float s[32];
+          tmem_ld32(t_s + c0, reinterpret_cast<uint32_t*>(s));
+          float kc[2], bias[2], inv[2];
+          factors(c0, &kc[0], &bias[0], &inv[0]);
+          factors(c0 + 16, &kc[1], &bias[1], &inv[1]);
           tmem_wait_ld();
-          exponents(0.f);
-          const float m_new = need ? fmaxf(m, largest()) : m;
+          if (tail || edge) {
+#pragma unroll
+            for (int c = 0; c < 32; ++c)
+              if (c0 + c <= last && c0 + c >= begin) top = fmaxf(top, fmaf(s[c], kc[c >> 4], bias[c >> 4]));
+          } else {
+            float t0 = top, t1 = top;
+#pragma unroll
+            for (int c = 0; c < 32; c += 4) {
+              t0 = max3(t0, fmaf(s[c], kc[c >> 4], bias[c >> 4]), fmaf(s[c + 1], kc[c >> 4], bias[c >> 4]));
+              t1 = max3(t1, fmaf(s[c + 2], kc[c >> 4], bias[c >> 4]), fmaf(s[c + 3], kc[c >> 4], bias[c >> 4]));
+            }
+            top = fmaxf(t0, t1);
+          }
+        }
+        const bool need = top > m + (kPaLimit - kPaShift);
+        if (__any_sync(0xffffffffu, need)) {
+          // some row's reference is too low (always so in a unit's first tile): it becomes the maximum
+          const float m_new = need ? top : m;
           const float f = need ? ex2(m - m_new) : 1.0f;
           m = m_new;
-          const float plus = kPaShift - m_new;
-#pragma unroll
-          for (int c = 0; c < kPaTile; ++c) s[c] = s[c] == -INFINITY ? s[c] : s[c] + plus;
-          l2 = f2_mul(l2, f2_pack(f, f));
+          l *= f;
           if (k > 0) {  // what the tensor core has summed so far: this tile's scores were issued behind it
 #pragma unroll 1
             for (int c = 0; c < 4; ++c) {
@@ -292,23 +279,39 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             }
           }
         }
-        // ---- weights, their sum, and P as two terms over the scores
-#pragma unroll
+        // ---- weights, their sum, and P as two terms: keys 32 q .. at columns 16 q .. 16 q + 15, over scores already used
+        const float plus = m == -INFINITY ? 0.f : kPaShift - m;
+#pragma unroll 1
         for (int q = 0; q < 4; ++q) {
-          uint32_t hi[8], lo[8];
+          float s[32];
+          tmem_ld32(t_s + q * 32, reinterpret_cast<uint32_t*>(s));
+          float kc[2], bias[2], inv[2];
+          factors(q * 32, &kc[0], &bias[0], &inv[0]);
+          factors(q * 32 + 16, &kc[1], &bias[1], &inv[1]);
+          bias[0] += plus;
+          bias[1] += plus;
+          tmem_wait_ld();
 #pragma unroll
-          for (int c4 = 0; c4 < 8; ++c4) {
-            const int c = q * 32 + c4 * 4;
-            const uint32_t vs = __float_as_uint(sc[8 + (c >> 4 << 4 >> p.page_shift)]);
-            const float inv = c <= last ? __uint_as_float(0x7f000000u - vs) : 0.f;  // behind the end there may be no page
-            const uint64_t inv2 = f2_pack(inv, inv);
-            const float p0 = ex2(s[c]), p1 = ex2(s[c + 1]), p2 = ex2(s[c + 2]), p3 = ex2(s[c + 3]);
-            l2 = f2_fma(f2_pack(p0, p1), inv2, l2);
-            l2 = f2_fma(f2_pack(p2, p3), inv2, l2);
-            split_weights(p0, p1, p2, p3, &hi[c4], &lo[c4]);
+          for (int c = 0; c < 32; ++c) s[c] = ex2(fmaf(s[c], kc[c >> 4], bias[c >> 4]));
+          if (tail || edge) {
+#pragma unroll
+            for (int c = 0; c < 32; ++c)
+              if (q * 32 + c > last || q * 32 + c < begin) s[c] = 0.f;
           }
-          tmem_st8(t_s + q * 8, hi);
-          tmem_st8(t_s + 32 + q * 8, lo);
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            float a0 = 0.f, a1 = 0.f;
+#pragma unroll
+            for (int c = 0; c < 16; c += 2) {
+              a0 += s[16 * g + c];
+              a1 += s[16 * g + c + 1];
+            }
+            l = fmaf(a0 + a1, inv[g], l);
+          }
+          uint32_t w[16];
+#pragma unroll
+          for (int c4 = 0; c4 < 8; ++c4) split_weights(s[4 * c4], s[4 * c4 + 1], s[4 * c4 + 2], s[4 * c4 + 3], &w[c4], &w[8 + c4]);
+          tmem_st16(t_s + q * 16, w);
         }
         if (tail || edge) {
           // A weight of zero does not silence a NaN: V of keys behind the end becomes zero, and NaN codes of keys that only
@@ -354,9 +357,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
       ok = warp_wait(ok, &o_full[x], units & 1, abort_flag);
       ++units;
       tc_fence_after_sync();
-      float l0, l1;
-      f2_unpack(l2, l0, l1);
-      const float total = l0 + l1;
+      const float total = l;
       const bool whole = off == 0 && n_seg == unit.tiles;
       const float inv = whole ? (total != 0.f ? 1.0f / total : 0.f) : 1.0f;  // nothing seen: zero
       const int64_t slot = (2 * (int64_t)blockIdx.x + (off == 0 ? 1 : 0)) * R + x * 128 + row;
