@@ -5,11 +5,13 @@
 // in its thread, no vote or barrier is needed between tiles, and the fixed cost of a tile (barriers, tensor memory latency) is
 // spread over 128 elements of each thread instead of 32.
 //
-// A block works on 256 rows (query tokens times the heads of a kv head, flattened), 128 for each of two softmax warpgroups that
-// take turns on the tensor core.  K and V tiles are read once for all 256 rows.  P goes back over S in TMEM (32 keys: 8 columns
-// of e4m3, 8 of the e5m2 residual) and is the A operand of the second product from there.
-//   warp 0 TMA, warp 1 UMMA issuer, warps 4-11 softmax (warpgroup x: rows 128 x ..), warps 2, 3 idle
-//   TMEM columns: S of warpgroup 0, 1 at 0, 128; O at 256, 384
+// A block works on 256 rows (query tokens times the heads of a kv head, flattened), two tiles of 128 that take turns on the
+// tensor core.  K and V tiles are read once for all 256 rows.  Two warpgroups share a row tile, 64 keys each (and 64 channels of
+// the result): with one, the latencies of its conversions lay open, 7000 cycles a tile.  They exchange the row maxima through
+// shared memory, one barrier a tile.  P goes back over S in TMEM (32 keys: 8 columns of e4m3, 8 of the e5m2 residual) and is the
+// A operand of the second product from there.
+//   warp 0 TMA, warp 1 UMMA issuer, warps 2, 3 idle, warps 4-19 softmax (warpgroup 2 x + half: row tile x, keys 64 half ..)
+//   TMEM columns: S of row tile 0, 1 at 0, 128; O at 256, 384
 #include "paged_attn.cuh"
 
 namespace magi {
@@ -19,13 +21,15 @@ int launch_prompt_join(magi_ctx* ctx, const PagedAttnKernelParams& k, cudaStream
 struct PromptShared {
   static constexpr int kStages = 8;
   static constexpr int kSlots = 8;                             // tiles whose page scales are kept
-  static constexpr int kThreads = 384;
+  static constexpr int kThreads = 640;
   static constexpr int kRing = 0;
   static constexpr int kQ = kRing + kStages * kPaTileBytes;    // [2 terms][2 warpgroups][128 rows][128 bytes]
   static constexpr int kScales = kQ + 4 * kPaTileBytes;        // [kSlots][2][8]
   static constexpr int kNan = kScales + kSlots * 64;           // [2][128][4] channels whose V is NaN (boundary tiles)
   static constexpr int kNanAny = kNan + 2 * kPaTile * 16;      // [2][4] whether a warp's keys have any
-  static constexpr int kNear = kNanAny + 32;
+  static constexpr int kTop = kNanAny + 32;                    // [2 buffers][2 row tiles][2 halves][128] row maxima, and sums at the end
+  static constexpr int kRowS = kTop + 2 * 4 * 128 * 4;         // [2 row tiles][128] scale of a query row
+  static constexpr int kNear = kRowS + 2 * 128 * 4;
   static constexpr int kStart = kNear + kPaNear * 16;
   static constexpr int kBar = kStart + 64;
   static constexpr int kNumBars = 2 * kStages + kSlots + 9;
@@ -35,6 +39,11 @@ struct PromptShared {
 static_assert(PromptShared::kDynamic <= 232448, "shared memory per block");
 static_assert(PromptShared::kStages * kPaTileBytes >= kPlanScratch, "the plan's scratch is in the ring");
 
+// The two warpgroups of row tile x.
+__device__ __forceinline__ void pair_sync(int x) {
+  __syncwarp();
+  asm volatile("bar.sync %0, 256;" ::"r"(1 + x) : "memory");
+}
 template <int kThreads>
 __device__ __forceinline__ void named_sync(int id) {
   __syncwarp();
@@ -51,7 +60,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
   uint64_t* kv_full = reinterpret_cast<uint64_t*>(smem + L::kBar);
   uint64_t* kv_empty = kv_full + kStages;
   uint64_t* sc_full = kv_empty + kStages;
-  uint64_t* q_full = sc_full + L::kSlots;  // [2] by warpgroup, as the next three
+  uint64_t* q_full = sc_full + L::kSlots;  // [2] by row tile, as the next three
   uint64_t* s_full = q_full + 2;
   uint64_t* p_full = s_full + 2;
   uint64_t* o_full = p_full + 2;
@@ -70,9 +79,9 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     }
     for (int s = 0; s < L::kSlots; ++s) mbar_init(&sc_full[s], 32);  // each lane of the loading warp
     for (int x = 0; x < 2; ++x) {
-      mbar_init(&q_full[x], 4);
+      mbar_init(&q_full[x], 8);
       mbar_init(&s_full[x], 1);
-      mbar_init(&p_full[x], 4);
+      mbar_init(&p_full[x], 8);
       mbar_init(&o_full[x], 1);
     }
     mbar_init(drain_bar, 1);
@@ -101,7 +110,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     load_tiles<R, kStages, L::kSlots>(p, walk, &tm_k, &tm_v, smem + L::kRing, reinterpret_cast<float*>(smem + L::kScales), kv_full, kv_empty, sc_full, abort_flag);
   } else if (warp == 1) {
     // ------------------------------------------------------------------ UMMA issuer
-    if (lane == 0) {
+    if (elect_one()) {
       constexpr uint32_t idesc_s = umma_idesc(128, kPaTile, 0, 0, 0, 0);
       constexpr uint32_t idesc_o = umma_idesc(128, kHeadDim, 0, 0, 0, 1), idesc_r = umma_idesc(128, kHeadDim, 1, 0, 0, 1);  // A e4m3, e5m2
       constexpr uint32_t desc_hi = (1024u >> 4) | (1u << 14) | (2u << 29);  // 1024 bytes between groups of 8 rows, 128-byte swizzle
@@ -110,8 +119,8 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
       constexpr uint32_t kTile16 = kPaTileBytes >> 4;
       bool ok = true;
       int i = 0;                       // tiles so far
-      int seen[2] = {0, 0}, units[2] = {0, 0};  // tiles and units of each warpgroup
-      auto first = [&](int x, int fill) {  // S of warpgroup x
+      int seen[2] = {0, 0}, units[2] = {0, 0};  // key tiles and units of each row tile
+      auto first = [&](int x, int fill) {  // S of row tile x
         const uint32_t a = q_lo + x * kTile16, b = ring + (fill % kStages) * kTile16, d = tmem_base + x * 128;
         umma_ss_f8_lh<0>(d, a, b, desc_hi, idesc_s);
 #pragma unroll
@@ -143,7 +152,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             else umma_ts_f8_lh<1>(d, a, b, desc_hi, idesc_o);
 #pragma unroll
             for (int s = 1; s < 8; ++s)  // 32 keys per instruction: 8 columns of P, 32 rows of V; then the residual term
-              umma_ts_f8_lh<1>(d, a + (s & 3) * 16 + (s >> 2) * 8, b + (s & 3) * 256, desc_hi, s < 4 ? idesc_o : idesc_r);
+              umma_ts_f8_lh<1>(d, a + (s & 3) * 32 + (s >> 2) * 8, b + (s & 3) * 256, desc_hi, s < 4 ? idesc_o : idesc_r);
             if (!more) umma_commit(&o_full[x]);
             if (x == nx - 1) umma_commit(&kv_empty[v_fill % kStages]);
             if (more) {
@@ -163,33 +172,35 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
   } else if (warp >= 4) {
     // ------------------------------------------------------------------ softmax and output
     // No early exits in here: a warp whose wait gave up goes on without waiting, so that the named barriers always meet.
-    const int x = (warp - 4) >> 2, quarter = warp & 3;
-    const int row = quarter * 32 + lane;  // of the warpgroup's 128; also the key whose V row this thread looks after (x = 0)
+    const int x = (warp - 4) >> 3, half = (warp - 4) >> 2 & 1, quarter = warp & 3;
+    const int row = quarter * 32 + lane;  // of the tile's 128; also the key whose V row this thread looks after (x = half = 0)
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
     const uint32_t t_s = tmem_base + lane_base + x * 128, t_o = t_s + 256;
     const float* scales = reinterpret_cast<const float*>(smem + L::kScales);
     uint4* nan_sh = reinterpret_cast<uint4*>(smem + L::kNan);
     volatile uint32_t* nan_any = reinterpret_cast<uint32_t*>(smem + L::kNanAny);
+    float* top_mine = reinterpret_cast<float*>(smem + L::kTop) + (x * 2 + half) * 128 + row;
+    const float* top_other = reinterpret_cast<const float*>(smem + L::kTop) + (x * 2 + (half ^ 1)) * 128 + row;
+    float* row_s = reinterpret_cast<float*>(smem + L::kRowS) + x * 128;
     bool ok = true;
     int i = 0;                 // tiles of the block so far
-    int seen = 0, units = 0;   // tiles and units of this warpgroup
+    int seen = 0, units = 0;   // key tiles and units of this row tile
     for (; walk.segment(); walk.advance()) {
       const PaUnit& unit = walk.unit;
       const PaEntry& ent = walk.ent;
       const int n_seg = walk.n_seg, off = walk.off;
       const int nx = unit.rows > 128 ? 2 : 1;
-      if (x >= nx) {  // a short unit leaves the second warpgroup out
+      if (x >= nx) {  // a short unit leaves the second row tile out
         i += n_seg;
         continue;
       }
-      // ---- this warp's 32 query rows as two e4m3 terms
-      float row_scale = 0.f;
+      // ---- 16 query rows per warp as two e4m3 terms
       const int flat = unit.first + x * 128 + row;
       const int tok = flat / p.group, head = walk.h * p.group + flat - tok * p.group;
       const bool owned = x * 128 + row < unit.rows;
       const long long q_at = (int64_t)(ent.row0 + tok) * p.q_st + (int64_t)head * p.q_sh;
 #pragma unroll 1
-      for (int r0 = 0; r0 < 32; r0 += 8) {
+      for (int r0 = half * 16; r0 < half * 16 + 16; r0 += 8) {
         uint2 raw[8];
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
@@ -205,12 +216,13 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
           uint8_t* at = smem + L::kQ + x * kPaTileBytes + tr * 128 + (((lane >> 2) ^ (tr & 7)) << 4) + (lane & 3) * 4;
           *reinterpret_cast<uint32_t*>(at) = hi;
           *reinterpret_cast<uint32_t*>(at + 2 * kPaTileBytes) = lo;
-          row_scale = lane == r0 + r ? scale : row_scale;
+          row_s[tr] = scale;  // every lane the same
         }
       }
       fence_proxy_async_smem();
       warp_arrive(&q_full[x]);
-      const float c1 = row_scale * p.scale_log2;
+      ok = warp_wait(ok, &q_full[x], units & 1, abort_flag);  // the other half's row scales
+      const float c1 = row_s[row] * p.scale_log2;
       const int at_pos = ent.len - ent.n_q + tok;
       float m = -INFINITY;                  // reference maximum, at most kPaLimit - kPaShift below the running one
       float l = 0.f;                        // sum of the weights
@@ -239,7 +251,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         };
         float top = -INFINITY;
 #pragma unroll 1
-        for (int c0 = 0; c0 < kPaTile; c0 += 32) {
+        for (int c0 = half * 64; c0 < half * 64 + 64; c0 += 32) {
           float s[32];
           tmem_ld32(t_s + c0, reinterpret_cast<uint32_t*>(s));
           float kc[2], bias[2], inv[2];
@@ -260,6 +272,9 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             top = fmaxf(t0, t1);
           }
         }
+        top_mine[(seen & 1) * 512] = top;
+        pair_sync(x);
+        top = fmaxf(top, top_other[(seen & 1) * 512]);
         const bool need = top > m + (kPaLimit - kPaShift);
         if (__any_sync(0xffffffffu, need)) {
           // some row's reference is too low (always so in a unit's first tile): it becomes the maximum
@@ -269,7 +284,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
           l *= f;
           if (k > 0) {  // what the tensor core has summed so far: this tile's scores were issued behind it
 #pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
+            for (int c = half * 2; c < half * 2 + 2; ++c) {
               uint32_t o[32];
               tmem_ld32(t_o + c * 32, o);
               tmem_wait_ld();
@@ -279,10 +294,10 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             }
           }
         }
-        // ---- weights, their sum, and P as two terms: keys 32 q .. at columns 16 q .. 16 q + 15, over scores already used
+        // ---- weights, their sum, and P as two terms: keys 32 q .. at the first 16 of their scores' columns
         const float plus = m == -INFINITY ? 0.f : kPaShift - m;
 #pragma unroll 1
-        for (int q = 0; q < 4; ++q) {
+        for (int q = half * 2; q < half * 2 + 2; ++q) {
           float s[32];
           tmem_ld32(t_s + q * 32, reinterpret_cast<uint32_t*>(s));
           float kc[2], bias[2], inv[2];
@@ -311,13 +326,13 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
           uint32_t w[16];
 #pragma unroll
           for (int c4 = 0; c4 < 8; ++c4) split_weights(s[4 * c4], s[4 * c4 + 1], s[4 * c4 + 2], s[4 * c4 + 3], &w[c4], &w[8 + c4]);
-          tmem_st16(t_s + q * 16, w);
+          tmem_st16(t_s + q * 32, w);
         }
         if (tail || edge) {
           // A weight of zero does not silence a NaN: V of keys behind the end becomes zero, and NaN codes of keys that only
           // some rows see are taken out of the product and come back in the rows that do see them.
           const int v_fill = 2 * i + 1, buf = i & 1;
-          if (x == 0) {
+          if (x == 0 && half == 0) {
             ok = warp_wait(ok, &kv_full[v_fill % kStages], (uint32_t)(v_fill / kStages) & 1, abort_flag);
             uint4* vrow = reinterpret_cast<uint4*>(smem + L::kRing + (v_fill % kStages) * kPaTileBytes + row * 128);
             if (k0 + row >= ent.len) {
@@ -333,8 +348,8 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             fence_proxy_async_smem();
           }
           if (edge) {
-            if (nx == 2) named_sync<256>(2);
-            else named_sync<128>(1);
+            if (nx == 2) named_sync<512>(4);
+            else named_sync<256>(3);
             const volatile uint32_t* any = nan_any + buf * 4;
             if (any[0] | any[1] | any[2] | any[3]) {
 #pragma unroll 1
@@ -357,14 +372,17 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
       ok = warp_wait(ok, &o_full[x], units & 1, abort_flag);
       ++units;
       tc_fence_after_sync();
-      const float total = l;
+      top_mine[0] = l;  // the maxima of the last tile have been read by both halves before its scores were consumed ...
+      pair_sync(x);
+      const float total = l + top_other[0];
+      pair_sync(x);     // ... and the sums before the next tile's maxima
       const bool whole = off == 0 && n_seg == unit.tiles;
       const float inv = whole ? (total != 0.f ? 1.0f / total : 0.f) : 1.0f;  // nothing seen: zero
       const int64_t slot = (2 * (int64_t)blockIdx.x + (off == 0 ? 1 : 0)) * R + x * 128 + row;
       __nv_bfloat16* out = p.out + (int64_t)(ent.row0 + (owned ? tok : 0)) * p.o_st + (int64_t)head * p.o_sh;
       float* part = p.parts + slot * kHeadDim;
 #pragma unroll 1
-      for (int c = 0; c < 4; ++c) {
+      for (int c = half * 2; c < half * 2 + 2; ++c) {
         float o[32];
         tmem_ld32(t_o + c * 32, reinterpret_cast<uint32_t*>(o));
         tmem_wait_ld();
@@ -383,7 +401,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         }
         __syncwarp();
       }
-      if (owned) {
+      if (owned && half == 0) {
         if (!whole) p.stats[slot] = make_float2(m, total);
         else if (p.lse && ok)
           p.lse[(int64_t)(ent.row0 + tok) * p.hq + head] = total != 0.f ? (m - kPaShift + log2f(total)) * 0.6931471805599453f : -INFINITY;
