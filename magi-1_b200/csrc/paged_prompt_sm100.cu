@@ -12,6 +12,8 @@
 // A operand of the second product from there.
 //   warp 0 TMA, warp 1 UMMA issuer, warps 2, 3 idle, warps 4-19 softmax (warpgroup 2 x + half: row tile x, keys 64 half ..)
 //   TMEM columns: S of row tile 0, 1 at 0, 128; O at 256, 384
+#include <type_traits>
+
 #include "paged_attn.cuh"
 
 namespace magi {
@@ -50,6 +52,8 @@ __device__ __forceinline__ void named_sync(int id) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(kThreads) : "memory");
 }
 
+// kGroup: consecutive keys that share a page, and so scales, for sure (page_tokens, at most 32).
+template <int kGroup>
 __global__ void __launch_bounds__(PromptShared::kThreads, 1)
 paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                     const __grid_constant__ PagedAttnKernelParams p) {
@@ -239,39 +243,49 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         const bool edge = (p.causal && min(k0 + kPaTile, ent.len) - 1 > unit.pos_a) || (p.window > 0 && k0 <= unit.pos_z - p.window);
         const int last = min(p.causal ? at_pos : ent.len - 1, ent.len - 1) - k0;               // columns [begin, last] are seen
         const int begin = p.window > 0 ? max(at_pos - p.window + 1 - k0, 0) : 0;
-        // 32 keys at a time, twice over (the scores stay in TMEM in between): the loop bodies then stay small enough for the
-        // instruction cache, and a thread holds 32 scores instead of 128.
-        // w = s log2e + log2(sv) = raw * kc + bias, the scales by groups of 16 keys (a page is a multiple of that)
-        auto factors = [&](int c, float* kc, float* bias, float* inv) {
-          const int pg = c >> p.page_shift;
+        // 32 keys at a time, twice over: the scores stay in TMEM in between, so that a thread holds 32 of them and not all.
+        // w = s log2e + log2(sv) = raw * kc + bias; the sum adds P / sv.
+        constexpr int kGroups = 64 / kGroup;
+        float kc[kGroups], bias[kGroups], inv[kGroups];
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+          const int c = half * 64 + g * kGroup, pg = c >> p.page_shift;
           const uint32_t vs = __float_as_uint(sc[8 + pg]);
-          *kc = fminf(sc[pg] * c1, 3.0e38f);  // finite: a raw score of zero stays zero
-          *bias = (float)((int)(vs >> 23) - 127);
-          *inv = c <= last ? __uint_as_float(0x7f000000u - vs) : 0.f;  // behind the end there may be no page
-        };
-        float top = -INFINITY;
-#pragma unroll 1
-        for (int c0 = half * 64; c0 < half * 64 + 64; c0 += 32) {
-          float s[32];
-          tmem_ld32(t_s + c0, reinterpret_cast<uint32_t*>(s));
-          float kc[2], bias[2], inv[2];
-          factors(c0, &kc[0], &bias[0], &inv[0]);
-          factors(c0 + 16, &kc[1], &bias[1], &inv[1]);
-          tmem_wait_ld();
-          if (tail || edge) {
-#pragma unroll
-            for (int c = 0; c < 32; ++c)
-              if (c0 + c <= last && c0 + c >= begin) top = fmaxf(top, fmaf(s[c], kc[c >> 4], bias[c >> 4]));
-          } else {
-            float t0 = top, t1 = top;
-#pragma unroll
-            for (int c = 0; c < 32; c += 4) {
-              t0 = max3(t0, fmaf(s[c], kc[c >> 4], bias[c >> 4]), fmaf(s[c + 1], kc[c >> 4], bias[c >> 4]));
-              t1 = max3(t1, fmaf(s[c + 2], kc[c >> 4], bias[c >> 4]), fmaf(s[c + 3], kc[c >> 4], bias[c >> 4]));
-            }
-            top = fmaxf(t0, t1);
-          }
+          kc[g] = fminf(sc[pg] * c1, 3.0e38f);  // finite: a raw score of zero stays zero
+          bias[g] = __uint_as_float(0x4b000000u | vs >> 23) - 8388735.0f;  // its exponent: 2^23 + (e + 127) - (2^23 + 127)
+          inv[g] = c <= last ? __uint_as_float(0x7f000000u - vs) : 0.f;     // behind the end there may be no page
         }
+        // Both passes exist twice, with and without the comparison of every key with the row's border.
+        auto find_top = [&](auto masked) {
+          float top = -INFINITY;
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+          uint64_t s2[16];
+          tmem_ld32(t_s + half * 64 + q * 32, reinterpret_cast<uint32_t*>(s2));
+          tmem_wait_ld();
+          float t0 = top, t1 = top;
+#pragma unroll
+          for (int c = 0; c < 32; c += 4) {
+            const int g = (q * 32 + c) / kGroup;
+            const uint64_t kc2 = f2_pack(kc[g], kc[g]), b2 = f2_pack(bias[g], bias[g]);
+            float w0, w1, w2, w3;
+            f2_unpack(f2_fma(s2[c / 2], kc2, b2), w0, w1);
+            f2_unpack(f2_fma(s2[c / 2 + 1], kc2, b2), w2, w3);
+            if constexpr (decltype(masked)::value) {
+              const int at = half * 64 + q * 32 + c;
+              w0 = at <= last && at >= begin ? w0 : -INFINITY;
+              w1 = at + 1 <= last && at + 1 >= begin ? w1 : -INFINITY;
+              w2 = at + 2 <= last && at + 2 >= begin ? w2 : -INFINITY;
+              w3 = at + 3 <= last && at + 3 >= begin ? w3 : -INFINITY;
+            }
+            t0 = max3(t0, w0, w1);
+            t1 = max3(t1, w2, w3);
+          }
+          top = fmaxf(t0, t1);
+          }
+          return top;
+        };
+        float top = tail || edge ? find_top(std::true_type()) : find_top(std::false_type());
         top_mine[(seen & 1) * 512] = top;
         pair_sync(x);
         top = fmaxf(top, top_other[(seen & 1) * 512]);
@@ -296,38 +310,48 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         }
         // ---- weights, their sum, and P as two terms: keys 32 q .. at the first 16 of their scores' columns
         const float plus = m == -INFINITY ? 0.f : kPaShift - m;
-#pragma unroll 1
-        for (int q = half * 2; q < half * 2 + 2; ++q) {
-          float s[32];
-          tmem_ld32(t_s + q * 32, reinterpret_cast<uint32_t*>(s));
-          float kc[2], bias[2], inv[2];
-          factors(q * 32, &kc[0], &bias[0], &inv[0]);
-          factors(q * 32 + 16, &kc[1], &bias[1], &inv[1]);
-          bias[0] += plus;
-          bias[1] += plus;
+        auto weigh = [&](auto masked) {
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+          uint64_t s2[16];
+          tmem_ld32(t_s + half * 64 + q * 32, reinterpret_cast<uint32_t*>(s2));
           tmem_wait_ld();
-#pragma unroll
-          for (int c = 0; c < 32; ++c) s[c] = ex2(fmaf(s[c], kc[c >> 4], bias[c >> 4]));
-          if (tail || edge) {
-#pragma unroll
-            for (int c = 0; c < 32; ++c)
-              if (q * 32 + c > last || q * 32 + c < begin) s[c] = 0.f;
-          }
-#pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            float a0 = 0.f, a1 = 0.f;
-#pragma unroll
-            for (int c = 0; c < 16; c += 2) {
-              a0 += s[16 * g + c];
-              a1 += s[16 * g + c + 1];
-            }
-            l = fmaf(a0 + a1, inv[g], l);
-          }
           uint32_t w[16];
+          uint64_t sum[32 / kGroup];
 #pragma unroll
-          for (int c4 = 0; c4 < 8; ++c4) split_weights(s[4 * c4], s[4 * c4 + 1], s[4 * c4 + 2], s[4 * c4 + 3], &w[c4], &w[8 + c4]);
-          tmem_st16(t_s + q * 32, w);
-        }
+          for (int g = 0; g < 32 / kGroup; ++g) sum[g] = 0;
+#pragma unroll
+          for (int c = 0; c < 32; c += 4) {
+            const int g = (q * 32 + c) / kGroup;
+            const uint64_t kc2 = f2_pack(kc[g], kc[g]), b2 = f2_pack(bias[g] + plus, bias[g] + plus);
+            float p0, p1, p2, p3;
+            f2_unpack(f2_fma(s2[c / 2], kc2, b2), p0, p1);
+            f2_unpack(f2_fma(s2[c / 2 + 1], kc2, b2), p2, p3);
+            p0 = ex2(p0);
+            p1 = ex2(p1);
+            p2 = ex2(p2);
+            p3 = ex2(p3);
+            if constexpr (decltype(masked)::value) {
+              const int at = half * 64 + q * 32 + c;
+              p0 = at <= last && at >= begin ? p0 : 0.f;
+              p1 = at + 1 <= last && at + 1 >= begin ? p1 : 0.f;
+              p2 = at + 2 <= last && at + 2 >= begin ? p2 : 0.f;
+              p3 = at + 3 <= last && at + 3 >= begin ? p3 : 0.f;
+            }
+            sum[c / kGroup] = f2_add(sum[c / kGroup], f2_add(f2_pack(p0, p1), f2_pack(p2, p3)));
+            split_weights(p0, p1, p2, p3, &w[c / 4], &w[8 + c / 4]);
+          }
+          tmem_st16(t_s + half * 64 + q * 32, w);
+#pragma unroll
+          for (int g = 0; g < 32 / kGroup; ++g) {
+            float a0, a1;
+            f2_unpack(sum[g], a0, a1);
+            l = fmaf(a0 + a1, inv[q * 32 / kGroup + g], l);
+          }
+          }
+        };
+        if (tail || edge) weigh(std::true_type());
+        else weigh(std::false_type());
         if (tail || edge) {
           // A weight of zero does not silence a NaN: V of keys behind the end becomes zero, and NaN codes of keys that only
           // some rows see are taken out of the product and come back in the rows that do see them.
@@ -425,10 +449,12 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
 int launch_paged_prompt(magi_ctx* ctx, const CUtensorMap& tk, const CUtensorMap& tv, const PagedAttnKernelParams& k, cudaStream_t st) {
   static bool configured[64] = {};  // per device: opt in to > 48 KB of dynamic shared memory once
   if (ctx->device >= 64 || !configured[ctx->device]) {
-    MAGI_CUDA_OK(ctx, cudaFuncSetAttribute(paged_prompt_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PromptShared::kDynamic));
+    MAGI_CUDA_OK(ctx, cudaFuncSetAttribute(paged_prompt_kernel<16>, cudaFuncAttributeMaxDynamicSharedMemorySize, PromptShared::kDynamic));
+    MAGI_CUDA_OK(ctx, cudaFuncSetAttribute(paged_prompt_kernel<32>, cudaFuncAttributeMaxDynamicSharedMemorySize, PromptShared::kDynamic));
     if (ctx->device < 64) configured[ctx->device] = true;
   }
-  paged_prompt_kernel<<<ctx->sm_count, PromptShared::kThreads, PromptShared::kDynamic, st>>>(tk, tv, k);
+  const auto kernel = k.c.page_tokens == 16 ? paged_prompt_kernel<16> : paged_prompt_kernel<32>;
+  kernel<<<ctx->sm_count, PromptShared::kThreads, PromptShared::kDynamic, st>>>(tk, tv, k);
   MAGI_CUDA_OK(ctx, cudaGetLastError());
   return launch_prompt_join(ctx, k, st);
 }
