@@ -146,34 +146,20 @@ __device__ __forceinline__ float warp_max(float v) {
   return r;
 }
 
-// A whole warp waits, its lanes staying together: lane 0 asks, by predicate and not by branch, and the warp votes.  (32 lanes
-// asking for one barrier are served one after the other, about 200 cycles a question; a branch on the lane leaves lane 0
-// behind on its own, and the warp-wide instructions that follow need all lanes at once.)
-__device__ __forceinline__ bool warp_wait(bool ok, uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
-  if (!ok) return false;
-  const uint32_t addr = smem_u32(bar), lane = threadIdx.x & 31;
-  long long t0 = 0;
-  while (true) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred l, p;\n\t"
-        "setp.eq.u32 l, %3, 0;\n\t"
-        "setp.ne.u32 p, %3, %3;\n\t"
-        "@l mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %4;\n\t"
-        "selp.b32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(addr), "r"(parity), "r"(lane), "r"((uint32_t)MAGI_WAIT_HINT_NS)
-        : "memory");
-    if (__any_sync(0xffffffffu, done)) break;
-    const long long now = clock64();
-    if (t0 == 0) t0 = now;
-    const bool late = now - t0 > 1000000000LL;
-    if (__any_sync(0xffffffffu, late)) *abort_flag = 1;
+// A whole warp waits, its lanes staying together (the warp-wide instructions that follow need all lanes at once, and a branch
+// on the lane left lane 0 behind on its own): all ask, the warp votes.  Bounded; gives up at once where another warp did.
+__device__ __forceinline__ bool warp_wait_long(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  const long long t0 = clock64();
+  while (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) {
+    if (__any_sync(0xffffffffu, clock64() - t0 > 1000000000LL)) *abort_flag = 1;
     __syncwarp();
     if (__any_sync(0xffffffffu, *abort_flag != 0)) return false;
   }
-  __syncwarp();  // what lane 0 has seen is there for the others
   return true;
+}
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  return warp_wait_long(bar, parity, abort_flag);
 }
 // One arrival for the warp, after what all its lanes did before.
 __device__ __forceinline__ void warp_arrive(uint64_t* bar) {
@@ -354,7 +340,7 @@ __device__ __forceinline__ void load_tiles(const PagedAttnKernelParams& p, PaWal
 #pragma unroll
       for (int kv = 0; kv < 2; ++kv, ++fill) {
         const int stage = fill % kStages, use = fill / kStages;
-        if (use > 0) ok = warp_wait(ok, &kv_empty[stage], (use & 1) ^ 1, abort_flag);
+        if (use > 0) ok = warp_wait(&kv_empty[stage], (use & 1) ^ 1, abort_flag);
         if (!ok) break;
         if (lane == 0) mbar_expect_tx(&kv_full[stage], n_load << (p.page_shift + 7));
         __syncwarp();

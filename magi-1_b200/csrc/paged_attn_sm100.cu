@@ -221,7 +221,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
     __syncwarp();
   } else {
     // ------------------------------------------------------------------ softmax and output
-    // No early exits in here: a warp whose wait gave up goes on without waiting, so that the named barriers always meet.
+    // No early exits in here: a warp whose wait gave up goes on, so that the named barriers always meet.
     const int sw = warp - 2;
     const int quarter = warp & 3;             // TMEM lanes of this warp
     const int key = quarter * 32 + lane;      // key of the tile; channel of the output
@@ -235,7 +235,6 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
     int64_t* at_sh = reinterpret_cast<int64_t*>(smem + L::kAt) + sw * R;
     uint4* nan_sh = reinterpret_cast<uint4*>(smem + L::kNan);
     volatile uint32_t* nan_any = reinterpret_cast<uint32_t*>(smem + L::kNanAny);
-    bool ok = true;
     int i = 0, units = 0;
     for (; walk.segment(); walk.advance()) {
       const PaUnit& unit = walk.unit;
@@ -271,7 +270,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       }
       fence_proxy_async_smem();
       warp_arrive(q_full);
-      ok = warp_wait(ok, q_full, units & 1, abort_flag);  // the other warps' row scales and positions
+      warp_wait(q_full, units & 1, abort_flag);  // the other warps' row scales and positions
       float m = -INFINITY;    // lane r < R: reference maximum of row r, at most kPaLimit - kPaShift below the running one
       uint32_t nan_rows = 0;  // rows whose result in this thread's channel is NaN (boundary tiles)
       uint64_t l2[R / 2];    // sums over this thread's keys, rows in pairs
@@ -282,8 +281,8 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
 #pragma unroll 1
       for (int x = 0; x < n_seg; ++x, ++i) {
         const int k0 = (unit.tile0 + off + x) * kPaTile, pos = k0 + key;
-        ok = warp_wait(ok, &sc_full[i % L::kSlots], (uint32_t)(i / L::kSlots) & 1, abort_flag);
-        ok = warp_wait(ok, &s_full[i & 1], (uint32_t)(i >> 1) & 1, abort_flag);
+        warp_wait(&sc_full[i % L::kSlots], (uint32_t)(i / L::kSlots) & 1, abort_flag);
+        warp_wait(&s_full[i & 1], (uint32_t)(i >> 1) & 1, abort_flag);
         const bool tail = k0 + kPaTile > ent.len;                                             // keys behind the sequence's end
         // keys before it that not every row sees
         const bool edge = (p.causal && min(k0 + kPaTile, ent.len) - 1 > unit.pos_a) || (p.window > 0 && k0 <= unit.pos_z - p.window);
@@ -358,7 +357,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
             l2[r / 2 + 1] = f2_mul(l2[r / 2 + 1], f2_pack(f.z, f.w));
           }
           if (x > 0) {  // what the tensor core has summed so far
-            ok = warp_wait(ok, &o_full[(i - 1) & 1], (uint32_t)((i - 1) >> 1) & 1, abort_flag);
+            warp_wait(&o_full[(i - 1) & 1], (uint32_t)((i - 1) >> 1) & 1, abort_flag);
             tc_fence_after_sync();
 #pragma unroll
             for (int c = 0; c < R; c += 16) {
@@ -389,7 +388,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
           split_weights(p0, p1, p2, p3, &hi[r / 4], &lo[r / 4]);
         }
         // the buffer of tile i - 2
-        if (i >= 2) ok = warp_wait(ok, &o_full[i & 1], (uint32_t)((i - 2) >> 1) & 1, abort_flag);
+        if (i >= 2) warp_wait(&o_full[i & 1], (uint32_t)((i - 2) >> 1) & 1, abort_flag);
         uint8_t* pb = smem + L::kP + key * 128;
 #pragma unroll
         for (int c = 0; c < R / 16; ++c) {
@@ -401,7 +400,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
           // A weight of zero does not silence a NaN: V of keys behind the end becomes zero, and NaN codes of keys that only
           // some rows see are taken out of the product and come back through the sums of the rows that do see them.
           const int v_fill = 2 * i + 1, v_stage = v_fill % kStages;
-          ok = warp_wait(ok, &kv_full[v_stage], (uint32_t)(v_fill / kStages) & 1, abort_flag);
+          warp_wait(&kv_full[v_stage], (uint32_t)(v_fill / kStages) & 1, abort_flag);
           __syncwarp();
           uint4* vrow = reinterpret_cast<uint4*>(smem + L::kRing + v_stage * kPaTileBytes + key * 128);
           if (pos >= ent.len) {
@@ -436,7 +435,8 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
         warp_arrive(&p_full[i & 1]);
       }
       // ---- the accumulator, the sum over the keys, then the result or what another block needs to go on
-      ok = warp_wait(ok, &o_full[(i - 1) & 1], (uint32_t)((i - 1) >> 1) & 1, abort_flag);
+      warp_wait(&o_full[(i - 1) & 1], (uint32_t)((i - 1) >> 1) & 1, abort_flag);
+      const bool ok = *abort_flag == 0;
       tc_fence_after_sync();
       float o[R];
       tmem_ld<R>(t_o, reinterpret_cast<uint32_t*>(o));

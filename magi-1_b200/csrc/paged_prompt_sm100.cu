@@ -175,7 +175,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     __syncwarp();
   } else if (warp >= 4) {
     // ------------------------------------------------------------------ softmax and output
-    // No early exits in here: a warp whose wait gave up goes on without waiting, so that the named barriers always meet.
+    // No early exits in here: a warp whose wait gave up goes on, so that the named barriers always meet.
     const int x = (warp - 4) >> 3, half = (warp - 4) >> 2 & 1, quarter = warp & 3;
     const int row = quarter * 32 + lane;  // of the tile's 128; also the key whose V row this thread looks after (x = half = 0)
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
@@ -186,7 +186,6 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     float* top_mine = reinterpret_cast<float*>(smem + L::kTop) + (x * 2 + half) * 128 + row;
     const float* top_other = reinterpret_cast<const float*>(smem + L::kTop) + (x * 2 + (half ^ 1)) * 128 + row;
     float* row_s = reinterpret_cast<float*>(smem + L::kRowS) + x * 128;
-    bool ok = true;
     int i = 0;                 // tiles of the block so far
     int seen = 0, units = 0;   // key tiles and units of this row tile
     for (; walk.segment(); walk.advance()) {
@@ -225,7 +224,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
       }
       fence_proxy_async_smem();
       warp_arrive(&q_full[x]);
-      ok = warp_wait(ok, &q_full[x], units & 1, abort_flag);  // the other half's row scales
+      warp_wait(&q_full[x], units & 1, abort_flag);  // the other half's row scales
       const float c1 = row_s[row] * p.scale_log2;
       const int at_pos = ent.len - ent.n_q + tok;
       float m = -INFINITY;                  // reference maximum, at most kPaLimit - kPaShift below the running one
@@ -234,13 +233,14 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
 #pragma unroll 1
       for (int k = 0; k < n_seg; ++k, ++i, ++seen) {
         const int k0 = (unit.tile0 + off + k) * kPaTile;
-        ok = warp_wait(ok, &sc_full[i % L::kSlots], (uint32_t)(i / L::kSlots) & 1, abort_flag);
-        ok = warp_wait(ok, &s_full[x], seen & 1, abort_flag);
+        warp_wait(&sc_full[i % L::kSlots], (uint32_t)(i / L::kSlots) & 1, abort_flag);
+        warp_wait(&s_full[x], seen & 1, abort_flag);
         tc_fence_after_sync();
         const float* sc = scales + (i % L::kSlots) * 16;
         const bool tail = k0 + kPaTile > ent.len;  // keys behind the sequence's end
         // keys before it that not every row sees
         const bool edge = (p.causal && min(k0 + kPaTile, ent.len) - 1 > unit.pos_a) || (p.window > 0 && k0 <= unit.pos_z - p.window);
+        const bool border = __any_sync(0xffffffffu, tail || edge);  // the vote lets the branches on it be uniform ones
         const int last = min(p.causal ? at_pos : ent.len - 1, ent.len - 1) - k0;               // columns [begin, last] are seen
         const int begin = p.window > 0 ? max(at_pos - p.window + 1 - k0, 0) : 0;
         // 32 keys at a time, twice over: the scores stay in TMEM in between, so that a thread holds 32 of them and not all.
@@ -257,35 +257,27 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         }
         // Both passes exist twice, with and without the comparison of every key with the row's border.
         auto find_top = [&](auto masked) {
-          float top = -INFINITY;
+          float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
-          uint64_t s2[16];
-          tmem_ld32(t_s + half * 64 + q * 32, reinterpret_cast<uint32_t*>(s2));
-          tmem_wait_ld();
-          float t0 = top, t1 = top;
+            float s[32];
+            tmem_ld32(t_s + half * 64 + q * 32, reinterpret_cast<uint32_t*>(s));
+            tmem_wait_ld();
 #pragma unroll
-          for (int c = 0; c < 32; c += 4) {
-            const int g = (q * 32 + c) / kGroup;
-            const uint64_t kc2 = f2_pack(kc[g], kc[g]), b2 = f2_pack(bias[g], bias[g]);
-            float w0, w1, w2, w3;
-            f2_unpack(f2_fma(s2[c / 2], kc2, b2), w0, w1);
-            f2_unpack(f2_fma(s2[c / 2 + 1], kc2, b2), w2, w3);
-            if constexpr (decltype(masked)::value) {
-              const int at = half * 64 + q * 32 + c;
-              w0 = at <= last && at >= begin ? w0 : -INFINITY;
-              w1 = at + 1 <= last && at + 1 >= begin ? w1 : -INFINITY;
-              w2 = at + 2 <= last && at + 2 >= begin ? w2 : -INFINITY;
-              w3 = at + 3 <= last && at + 3 >= begin ? w3 : -INFINITY;
+            for (int c = 0; c < 32; ++c) {
+              const int g = (q * 32 + c) / kGroup, at = half * 64 + q * 32 + c;
+              s[c] = fmaf(s[c], kc[g], bias[g]);
+              if constexpr (decltype(masked)::value) s[c] = at <= last && at >= begin ? s[c] : -INFINITY;
             }
-            t0 = max3(t0, w0, w1);
-            t1 = max3(t1, w2, w3);
+#pragma unroll
+            for (int c = 0; c < 32; c += 4) {
+              t0 = max3(t0, s[c], s[c + 1]);
+              t1 = max3(t1, s[c + 2], s[c + 3]);
+            }
           }
-          top = fmaxf(t0, t1);
-          }
-          return top;
+          return fmaxf(t0, t1);
         };
-        float top = tail || edge ? find_top(std::true_type()) : find_top(std::false_type());
+        float top = border ? find_top(std::true_type()) : find_top(std::false_type());
         top_mine[(seen & 1) * 512] = top;
         pair_sync(x);
         top = fmaxf(top, top_other[(seen & 1) * 512]);
@@ -313,51 +305,39 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         auto weigh = [&](auto masked) {
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
-          uint64_t s2[16];
-          tmem_ld32(t_s + half * 64 + q * 32, reinterpret_cast<uint32_t*>(s2));
-          tmem_wait_ld();
-          uint32_t w[16];
-          uint64_t sum[32 / kGroup];
+            float s[32];
+            tmem_ld32(t_s + half * 64 + q * 32, reinterpret_cast<uint32_t*>(s));
+            tmem_wait_ld();
+            uint32_t w[16];
 #pragma unroll
-          for (int g = 0; g < 32 / kGroup; ++g) sum[g] = 0;
+            for (int g = 0; g < 32 / kGroup; ++g) {
+              const float k = kc[q * 32 / kGroup + g], b = bias[q * 32 / kGroup + g] + plus;
+              float a0 = 0.f, a1 = 0.f;
 #pragma unroll
-          for (int c = 0; c < 32; c += 4) {
-            const int g = (q * 32 + c) / kGroup;
-            const uint64_t kc2 = f2_pack(kc[g], kc[g]), b2 = f2_pack(bias[g] + plus, bias[g] + plus);
-            float p0, p1, p2, p3;
-            f2_unpack(f2_fma(s2[c / 2], kc2, b2), p0, p1);
-            f2_unpack(f2_fma(s2[c / 2 + 1], kc2, b2), p2, p3);
-            p0 = ex2(p0);
-            p1 = ex2(p1);
-            p2 = ex2(p2);
-            p3 = ex2(p3);
-            if constexpr (decltype(masked)::value) {
-              const int at = half * 64 + q * 32 + c;
-              p0 = at <= last && at >= begin ? p0 : 0.f;
-              p1 = at + 1 <= last && at + 1 >= begin ? p1 : 0.f;
-              p2 = at + 2 <= last && at + 2 >= begin ? p2 : 0.f;
-              p3 = at + 3 <= last && at + 3 >= begin ? p3 : 0.f;
+              for (int c = g * kGroup; c < (g + 1) * kGroup; c += 4) {
+#pragma unroll
+                for (int e = c; e < c + 4; ++e) {
+                  s[e] = ex2(fmaf(s[e], k, b));
+                  const int at = half * 64 + q * 32 + e;
+                  if constexpr (decltype(masked)::value) s[e] = at <= last && at >= begin ? s[e] : 0.f;
+                }
+                a0 += s[c] + s[c + 1];
+                a1 += s[c + 2] + s[c + 3];
+                split_weights(s[c], s[c + 1], s[c + 2], s[c + 3], &w[c / 4], &w[8 + c / 4]);
+              }
+              l = fmaf(a0 + a1, inv[q * 32 / kGroup + g], l);
             }
-            sum[c / kGroup] = f2_add(sum[c / kGroup], f2_add(f2_pack(p0, p1), f2_pack(p2, p3)));
-            split_weights(p0, p1, p2, p3, &w[c / 4], &w[8 + c / 4]);
-          }
-          tmem_st16(t_s + half * 64 + q * 32, w);
-#pragma unroll
-          for (int g = 0; g < 32 / kGroup; ++g) {
-            float a0, a1;
-            f2_unpack(sum[g], a0, a1);
-            l = fmaf(a0 + a1, inv[q * 32 / kGroup + g], l);
-          }
+            tmem_st16(t_s + half * 64 + q * 32, w);
           }
         };
-        if (tail || edge) weigh(std::true_type());
+        if (border) weigh(std::true_type());
         else weigh(std::false_type());
-        if (tail || edge) {
+        if (border) {
           // A weight of zero does not silence a NaN: V of keys behind the end becomes zero, and NaN codes of keys that only
           // some rows see are taken out of the product and come back in the rows that do see them.
           const int v_fill = 2 * i + 1, buf = i & 1;
           if (x == 0 && half == 0) {
-            ok = warp_wait(ok, &kv_full[v_fill % kStages], (uint32_t)(v_fill / kStages) & 1, abort_flag);
+            warp_wait(&kv_full[v_fill % kStages], (uint32_t)(v_fill / kStages) & 1, abort_flag);
             uint4* vrow = reinterpret_cast<uint4*>(smem + L::kRing + (v_fill % kStages) * kPaTileBytes + row * 128);
             if (k0 + row >= ent.len) {
 #pragma unroll
@@ -393,7 +373,8 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         warp_arrive(&p_full[x]);
       }
       // ---- the result, or what another block needs to go on
-      ok = warp_wait(ok, &o_full[x], units & 1, abort_flag);
+      warp_wait(&o_full[x], units & 1, abort_flag);
+      const bool ok = *abort_flag == 0;
       ++units;
       tc_fence_after_sync();
       top_mine[0] = l;  // the maxima of the last tile have been read by both halves before its scores were consumed ...
