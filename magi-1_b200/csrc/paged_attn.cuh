@@ -32,6 +32,8 @@ struct PagedAttnKernelParams {
   const int32_t* seqs;
   const int32_t* cu_q;
   int n, total_q, max_q, hq, group;
+  uint32_t group_mul;  // see by_group()
+  int group_shift;
   float scale_log2;
   int causal, window;
   int* status;
@@ -41,6 +43,19 @@ struct PagedAttnKernelParams {
   float* parts;        // [blocks][2][rows][128] accumulators of units that lie in several blocks
   float2* stats;       // [blocks][2][rows] their maximum and sum
 };
+
+// n / group for 0 <= n < 2^31, by a product with floor(2^(31 + l) / group) + 1, l = ceil(log2 group) (Granlund and Montgomery's
+// division by an invariant): the walk from unit to unit divides often, and every warp does it.
+__device__ __forceinline__ int by_group(const PagedAttnKernelParams& p, int n) {
+  return p.group_shift < 0 ? n : (int)(__umulhi((uint32_t)n, p.group_mul) >> p.group_shift);
+}
+inline void set_group(PagedAttnKernelParams* p, int group) {
+  int l = 0;
+  while ((1ll << l) < group) ++l;
+  p->group = group;
+  p->group_shift = l - 1;
+  p->group_mul = l > 0 ? (uint32_t)((1ull << (31 + l)) / (unsigned)group + 1) : 0u;
+}
 
 // What a block leaves behind about its last unit, when others continue it.
 struct PaHeader {
@@ -92,8 +107,8 @@ template <int kRows>
 __device__ __forceinline__ int unit_tiles(const PagedAttnKernelParams& p, const PaEntry& e, int j, PaUnit* u) {
   const int first = j * kRows;
   const int rows = min(kRows, e.n_q * p.group - first);
-  const int pos_a = e.len - e.n_q + first / p.group;
-  const int pos_z = e.len - e.n_q + (first + rows - 1) / p.group;
+  const int pos_a = e.len - e.n_q + by_group(p, first);
+  const int pos_z = e.len - e.n_q + by_group(p, first + rows - 1);
   const int end = p.causal ? pos_z + 1 : e.len;
   const int begin = p.window > 0 ? max(0, pos_a - p.window + 1) : 0;
   int tile0 = 0, tiles = 1;
@@ -366,25 +381,21 @@ __device__ __forceinline__ void load_tiles(const PagedAttnKernelParams& p, PaWal
 // Four bf16 of a query row (a lane's share of its 128 channels) as two e4m3 terms, the row scaled by the power of two that
 // brings its largest entry into (224, 448].  Returns that power's inverse; whole warp, one row.
 __device__ __forceinline__ float split_query(uint2 raw, uint32_t* hi, uint32_t* lo) {
-  float f[4] = {__uint_as_float(raw.x << 16), __uint_as_float(raw.x & 0xffff0000u), __uint_as_float(raw.y << 16), __uint_as_float(raw.y & 0xffff0000u)};
-  const float top = fmaxf(fmaxf(fabsf(f[0]), fabsf(f[1])), fmaxf(fabsf(f[2]), fabsf(f[3])));
-  const bool odd = !(fabsf(f[0]) < INFINITY && fabsf(f[1]) < INFINITY && fabsf(f[2]) < INFINITY && fabsf(f[3]) < INFINITY);
-  const uint32_t bits = __float_as_uint(warp_max(top));
+  // magnitudes of bf16 compare as whole numbers; NaN and infinity are the largest
+  const uint32_t a = raw.x & 0x7fff7fffu, b = raw.y & 0x7fff7fffu;
+  const uint32_t top = __reduce_max_sync(0xffffffffu, max(max(a & 0xffffu, a >> 16), max(b & 0xffffu, b >> 16)));
   // below 2^-92 the entries keep fewer bits: their scores are then below 2^-16 whatever the keys are
-  const int e = max((int)(bits >> 23) - 127 - ((bits & 0x7fffffu) <= 0x600000u ? 8 : 7), -100);
+  const int e = max((int)(top >> 7) - 127 - ((top & 0x7fu) <= 0x60u ? 8 : 7), -100);
   const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
-  float res[4];
-#pragma unroll
-  for (int k = 0; k < 4; ++k) f[k] *= inv;
-  uint32_t h = pack4_e4m3(f[0], f[1], f[2], f[3]);
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const __half_raw hr = __nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)(h >> (8 * k)), __NV_E4M3);
-    res[k] = f[k] - __half2float(*reinterpret_cast<const __half*>(&hr));
-  }
-  const bool any_odd = __any_sync(0xffffffffu, odd);  // a row with NaN or infinity has no softmax: NaN throughout
-  *hi = any_odd ? 0x7f7f7f7fu : h;
-  *lo = any_odd ? 0u : pack4_e4m3(res[0], res[1], res[2], res[3]);
+  const float f0 = __uint_as_float(raw.x << 16) * inv, f1 = __uint_as_float(raw.x & 0xffff0000u) * inv;
+  const float f2 = __uint_as_float(raw.y << 16) * inv, f3 = __uint_as_float(raw.y & 0xffff0000u) * inv;
+  const uint32_t h = pack4_e4m3(f0, f1, f2, f3);
+  // what the first term leaves: at most eight significant bits, exact in fp16 (and zero below its 2^-25)
+  const float2 d01 = __half22float2(__hsub2(__floats2half2_rn(f0, f1), __half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)h, __NV_E4M3))));
+  const float2 d23 = __half22float2(__hsub2(__floats2half2_rn(f2, f3), __half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(h >> 16), __NV_E4M3))));
+  const bool odd = top >= 0x7f80u;  // a row with NaN or infinity has no softmax: NaN throughout
+  *hi = odd ? 0x7f7f7f7fu : h;
+  *lo = odd ? 0u : pack4_e4m3(d01.x, d01.y, d23.x, d23.y);
   return __uint_as_float((uint32_t)(127 + e) << 23);
 }
 

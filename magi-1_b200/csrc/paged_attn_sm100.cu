@@ -250,7 +250,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
 #pragma unroll
         for (int x = 0; x < kMine; ++x) {
           const int r = sw + x * 4, flat = unit.first + r;
-          toks[x] = flat / p.group;
+          toks[x] = by_group(p, flat);
           raw[x] = make_uint2(0, 0);
           if (r < unit.rows)
             raw[x] = *reinterpret_cast<const uint2*>(p.q + (int64_t)(ent.row0 + toks[x]) * p.q_st + (int64_t)(h * p.group + flat - toks[x] * p.group) * p.q_sh + lane * 4);
@@ -473,7 +473,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       }
       if (off == 0 && n_seg == unit.tiles) {
         const bool owned = lane < R && row < unit.rows;
-        const int flat = unit.first + (owned ? row : 0), tok = flat / p.group, head = h * p.group + flat - tok * p.group;
+        const int flat = unit.first + (owned ? row : 0), tok = by_group(p, flat), head = h * p.group + flat - tok * p.group;
         if (owned && ok) {
           if (p.lse && sw == 0)
             p.lse[(int64_t)(ent.row0 + tok) * p.hq + head] = total != 0.f ? (m - kPaShift + log2f(total)) * 0.6931471805599453f : -INFINITY;
@@ -512,7 +512,8 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
 }
 
 // Joins the parts of a unit that several blocks worked on, in the order of the keys: block (i, y) works on the unit that
-// main block i left open.  kWide: its eight warps share one row (few rows in many parts), else each has a row of its own.
+// main block i left open.  kWide: its eight warps share one row (few rows in many parts), else each has a row of its own (and
+// the parts lie [channel / 4][row][4], as the prompt form's threads, a row each, store them side by side).
 template <int R, bool kWide>
 __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__ PagedAttnKernelParams p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -539,7 +540,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
   for (int k = kWide ? warp : 0; k < n_parts; k += kWide ? 8 : 1) {
     const int64_t s = slot(k);
     const float2 ml = p.stats[s];
-    const float4 o = *reinterpret_cast<const float4*>(p.parts + s * kHeadDim + lane * 4);
+    const float4 o = *reinterpret_cast<const float4*>(p.parts + (kWide ? s * kHeadDim + lane * 4 : (s - r) * kHeadDim + (lane * R + r) * 4));
     const float f = ex2(ml.x - ref);
     sum = fmaf(ml.y, f, sum);
     acc.x = fmaf(o.x, f, acc.x);
@@ -565,7 +566,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
     }
   }
   const float inv = sum != 0.f ? 1.0f / sum : 0.f;
-  const int flat = u.first + r, tok = flat / p.group, head = hd.h * p.group + flat - tok * p.group;
+  const int flat = u.first + r, tok = by_group(p, flat), head = hd.h * p.group + flat - tok * p.group;
   *reinterpret_cast<uint2*>(p.out + (int64_t)(e.row0 + tok) * p.o_st + (int64_t)head * p.o_sh + lane * 4) =
       make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
   if (p.lse && lane == 0)
@@ -659,7 +660,7 @@ extern "C" int magi_paged_attn_fwd(magi_ctx* ctx, const magi_token_cache* cache,
   k.total_q = p->total_q;
   k.max_q = p->max_q;
   k.hq = p->n_q_heads;
-  k.group = p->n_q_heads / k.c.n_kv_heads;
+  set_group(&k, p->n_q_heads / k.c.n_kv_heads);
   k.scale_log2 = (p->softmax_scale > 0.f ? p->softmax_scale : 1.0f / sqrtf((float)kHeadDim)) * 1.4426950408889634f;
   k.causal = p->causal;
   k.window = p->window;

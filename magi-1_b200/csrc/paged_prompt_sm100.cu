@@ -199,7 +199,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
       }
       // ---- 16 query rows per warp as two e4m3 terms
       const int flat = unit.first + x * 128 + row;
-      const int tok = flat / p.group, head = walk.h * p.group + flat - tok * p.group;
+      const int tok = by_group(p, flat), head = walk.h * p.group + flat - tok * p.group;
       const bool owned = x * 128 + row < unit.rows;
       const long long q_at = (int64_t)(ent.row0 + tok) * p.q_st + (int64_t)head * p.q_sh;
 #pragma unroll 1
@@ -255,29 +255,35 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
           bias[g] = __uint_as_float(0x4b000000u | vs >> 23) - 8388735.0f;  // its exponent: 2^23 + (e + 127) - (2^23 + 127)
           inv[g] = c <= last ? __uint_as_float(0x7f000000u - vs) : 0.f;     // behind the end there may be no page
         }
-        // Both passes exist twice, with and without the comparison of every key with the row's border.
-        auto find_top = [&](auto masked) {
-          float t0 = -INFINITY, t1 = -INFINITY;
+        // Columns that every row of this warp sees; those beyond are compared with each row's own border, 16 at a time (the
+        // rows of a warp stand a few positions apart, so one group of 16 or two in a tile).
+        const int all_last = __reduce_min_sync(0xffffffffu, last), all_begin = __reduce_max_sync(0xffffffffu, begin);
+        auto clear = [&](int at) { return at + 15 <= all_last && at >= all_begin; };
+        float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            float s[32];
-            tmem_ld32(t_s + half * 64 + q * 32, reinterpret_cast<uint32_t*>(s));
-            tmem_wait_ld();
+        for (int q = 0; q < 2; ++q) {
+          float s[32];
+          tmem_ld32(t_s + half * 64 + q * 32, reinterpret_cast<uint32_t*>(s));
+          tmem_wait_ld();
 #pragma unroll
-            for (int c = 0; c < 32; ++c) {
-              const int g = (q * 32 + c) / kGroup, at = half * 64 + q * 32 + c;
-              s[c] = fmaf(s[c], kc[g], bias[g]);
-              if constexpr (decltype(masked)::value) s[c] = at <= last && at >= begin ? s[c] : -INFINITY;
-            }
+          for (int c = 0; c < 32; ++c) s[c] = fmaf(s[c], kc[(q * 32 + c) / kGroup], bias[(q * 32 + c) / kGroup]);
+          if (border) {
 #pragma unroll
-            for (int c = 0; c < 32; c += 4) {
-              t0 = max3(t0, s[c], s[c + 1]);
-              t1 = max3(t1, s[c + 2], s[c + 3]);
+            for (int u = 0; u < 2; ++u) {
+              const int at = half * 64 + q * 32 + u * 16;
+              if (!clear(at)) {
+#pragma unroll
+                for (int c = 0; c < 16; ++c) s[u * 16 + c] = at + c <= last && at + c >= begin ? s[u * 16 + c] : -INFINITY;
+              }
             }
           }
-          return fmaxf(t0, t1);
-        };
-        float top = border ? find_top(std::true_type()) : find_top(std::false_type());
+#pragma unroll
+          for (int c = 0; c < 32; c += 4) {
+            t0 = max3(t0, s[c], s[c + 1]);
+            t1 = max3(t1, s[c + 2], s[c + 3]);
+          }
+        }
+        float top = fmaxf(t0, t1);
         top_mine[(seen & 1) * 512] = top;
         pair_sync(x);
         top = fmaxf(top, top_other[(seen & 1) * 512]);
@@ -302,36 +308,37 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         }
         // ---- weights, their sum, and P as two terms: keys 32 q .. at the first 16 of their scores' columns
         const float plus = m == -INFINITY ? 0.f : kPaShift - m;
-        auto weigh = [&](auto masked) {
 #pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            float s[32];
-            tmem_ld32(t_s + half * 64 + q * 32, reinterpret_cast<uint32_t*>(s));
-            tmem_wait_ld();
-            uint32_t w[16];
+        for (int q = 0; q < 2; ++q) {
+          float s[32];
+          tmem_ld32(t_s + half * 64 + q * 32, reinterpret_cast<uint32_t*>(s));
+          tmem_wait_ld();
+          uint32_t w[16];
 #pragma unroll
-            for (int g = 0; g < 32 / kGroup; ++g) {
-              const float k = kc[q * 32 / kGroup + g], b = bias[q * 32 / kGroup + g] + plus;
-              float a0 = 0.f, a1 = 0.f;
+          for (int u = 0; u < 2; ++u) {
+            const int at = half * 64 + q * 32 + u * 16, g = (q * 32 + u * 16) / kGroup;
+            const float k = kc[g], b = bias[g] + plus;
+            float a0 = 0.f, a1 = 0.f;
+            auto sixteen = [&](auto masked) {  // exponentials and conversions run in different pipes: four keys of each in turn
 #pragma unroll
-              for (int c = g * kGroup; c < (g + 1) * kGroup; c += 4) {
+              for (int c = 0; c < 16; c += 4) {
+                float p[4];
 #pragma unroll
-                for (int e = c; e < c + 4; ++e) {
-                  s[e] = ex2(fmaf(s[e], k, b));
-                  const int at = half * 64 + q * 32 + e;
-                  if constexpr (decltype(masked)::value) s[e] = at <= last && at >= begin ? s[e] : 0.f;
+                for (int e = 0; e < 4; ++e) {
+                  p[e] = ex2(fmaf(s[u * 16 + c + e], k, b));
+                  if constexpr (decltype(masked)::value) p[e] = at + c + e <= last && at + c + e >= begin ? p[e] : 0.f;
                 }
-                a0 += s[c] + s[c + 1];
-                a1 += s[c + 2] + s[c + 3];
-                split_weights(s[c], s[c + 1], s[c + 2], s[c + 3], &w[c / 4], &w[8 + c / 4]);
+                a0 += p[0] + p[1];
+                a1 += p[2] + p[3];
+                split_weights(p[0], p[1], p[2], p[3], &w[u * 4 + c / 4], &w[8 + u * 4 + c / 4]);
               }
-              l = fmaf(a0 + a1, inv[q * 32 / kGroup + g], l);
-            }
-            tmem_st16(t_s + half * 64 + q * 32, w);
+            };
+            if (border && !clear(at)) sixteen(std::true_type());
+            else sixteen(std::false_type());
+            l = fmaf(a0 + a1, inv[g], l);
           }
-        };
-        if (border) weigh(std::true_type());
-        else weigh(std::false_type());
+          tmem_st16(t_s + half * 64 + q * 32, w);
+        }
         if (border) {
           // A weight of zero does not silence a NaN: V of keys behind the end becomes zero, and NaN codes of keys that only
           // some rows see are taken out of the product and come back in the rows that do see them.
@@ -385,7 +392,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
       const float inv = whole ? (total != 0.f ? 1.0f / total : 0.f) : 1.0f;  // nothing seen: zero
       const int64_t slot = (2 * (int64_t)blockIdx.x + (off == 0 ? 1 : 0)) * R + x * 128 + row;
       __nv_bfloat16* out = p.out + (int64_t)(ent.row0 + (owned ? tok : 0)) * p.o_st + (int64_t)head * p.o_sh;
-      float* part = p.parts + slot * kHeadDim;
+      float* part = p.parts + (slot - x * 128 - row) * kHeadDim + (x * 128 + row) * 4;  // [channel / 4][row][4]
 #pragma unroll 1
       for (int c = half * 2; c < half * 2 + 2; ++c) {
         float o[32];
@@ -401,7 +408,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
               *reinterpret_cast<uint4*>(out + c * 32 + q) = make_uint4(pack_bf16x2(o[q], o[q + 1]), pack_bf16x2(o[q + 2], o[q + 3]), pack_bf16x2(o[q + 4], o[q + 5]), pack_bf16x2(o[q + 6], o[q + 7]));
           } else {
 #pragma unroll
-            for (int q = 0; q < 32; q += 4) *reinterpret_cast<float4*>(part + c * 32 + q) = make_float4(o[q], o[q + 1], o[q + 2], o[q + 3]);
+            for (int q = 0; q < 32; q += 4) *reinterpret_cast<float4*>(part + (c * 32 + q) * R) = make_float4(o[q], o[q + 1], o[q + 2], o[q + 3]);
           }
         }
         __syncwarp();
