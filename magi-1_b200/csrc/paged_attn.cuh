@@ -187,10 +187,11 @@ __device__ __forceinline__ void warp_arrive(uint64_t* bar) {
       : "memory");
 }
 
-// Which tiles are this block's: the tiles of all units in a row, dealt out in equal contiguous parts.  Whole block; scratch
+// Which tiles are this block's: the tiles of all units in a row, dealt out in contiguous parts of equal weight.  A unit weighs
+// its tiles and kCost more for what it takes to begin and end one, as if it had so many empty tiles in front.  Whole block; scratch
 // needs kPlanScratch bytes.  The caller puts a barrier behind it.
 constexpr int kPlanScratch = (8 + (int)sizeof(PaEntry)) * kPgMaxEntries;
-template <int R, int kThreads>
+template <int R, int kThreads, int kCost>
 __device__ __forceinline__ void plan_tiles(const PagedAttnKernelParams& p, uint8_t* scratch, PaStart* start, PaEntry* near) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hkv = p.c.n_kv_heads;
   int64_t* sums = reinterpret_cast<int64_t*>(scratch);  // [n] tiles of an entry, then their prefix sums
@@ -202,7 +203,7 @@ __device__ __forceinline__ void plan_tiles(const PagedAttnKernelParams& p, uint8
     const PaEntry e = load_entry(p, b, &bad);
     any_bad |= bad;
     entries[b] = e;
-    if (single) sums[b] = e.n_q > 0 ? (int64_t)unit_tiles<R>(p, e, 0, nullptr) * hkv : 0;
+    if (single) sums[b] = e.n_q > 0 ? (int64_t)(unit_tiles<R>(p, e, 0, nullptr) + kCost) * hkv : 0;
   }
   if (any_bad && blockIdx.x == 0) *p.status = MAGI_E_RANGE;
   __syncthreads();
@@ -211,7 +212,7 @@ __device__ __forceinline__ void plan_tiles(const PagedAttnKernelParams& p, uint8
       const PaEntry e = entries[b];
       const int n_j = row_tiles<R>(p, e);
       int64_t w = 0;
-      for (int j = lane; j < n_j; j += 32) w += unit_tiles<R>(p, e, j, nullptr);
+      for (int j = lane; j < n_j; j += 32) w += unit_tiles<R>(p, e, j, nullptr) + kCost;
 #pragma unroll
       for (int d = 16; d > 0; d >>= 1) w += __shfl_xor_sync(0xffffffffu, w, d);
       if (lane == 0) sums[b] = w * hkv;
@@ -253,7 +254,7 @@ __device__ __forceinline__ void plan_tiles(const PagedAttnKernelParams& p, uint8
         const PaEntry e = entries[b];
         const int n_j = row_tiles<R>(p, e);
         for (int j0 = 0; j0 < n_j; j0 += 32) {
-          const int64_t mine = j0 + lane < n_j ? unit_tiles<R>(p, e, j0 + lane, nullptr) : 0;
+          const int64_t mine = j0 + lane < n_j ? unit_tiles<R>(p, e, j0 + lane, nullptr) + kCost : 0;
           int64_t x = mine;
 #pragma unroll
           for (int d = 1; d < 32; d <<= 1) {
@@ -281,17 +282,19 @@ __device__ __forceinline__ void plan_tiles(const PagedAttnKernelParams& p, uint8
 }
 
 // The walk over a block's segments (a segment = the tiles of one unit that are its own), the same in every role.
-template <int R>
+template <int R, int kCost>
 struct PaWalk {
   const PagedAttnKernelParams& p;
   const PaEntry* near;
-  int64_t t, t1;
-  int b, h, j, off, b0, n_j, n_seg;
+  int64_t t, t1;        // weight: the segment's start, the block's end
+  int b, h, j, at;      // unit, and where in its weight the segment starts
+  int b0, n_j, weight;  // weight of the segment
+  int first, n_seg;     // its tiles [first, first + n_seg) of the unit's
   PaEntry ent;
   PaUnit unit;
 
   __device__ __forceinline__ PaWalk(const PagedAttnKernelParams& params, const PaStart& st, const PaEntry* entries)
-      : p(params), near(entries), t(st.t0), t1(st.t1), b(st.b), h(st.h), j(st.j), off(st.off), b0(st.b) {
+      : p(params), near(entries), t(st.t0), t1(st.t1), b(st.b), h(st.h), j(st.j), at(st.off), b0(st.b) {
     if (t < t1) fetch();
   }
   __device__ __forceinline__ void fetch() {
@@ -302,17 +305,25 @@ struct PaWalk {
     }
     n_j = row_tiles<R>(p, ent);
   }
-  // The current segment: its unit and number of tiles; false behind the last one.
+  // The current segment; false behind the last one.
   __device__ __forceinline__ bool segment() {
-    if (t >= t1) return false;
-    unit_tiles<R>(p, ent, j, &unit);
-    n_seg = (int)min((int64_t)(unit.tiles - off), t1 - t);
-    return true;
+    while (t < t1) {
+      unit_tiles<R>(p, ent, j, &unit);
+      weight = (int)min((int64_t)(unit.tiles + kCost - at), t1 - t);
+      first = max(at - kCost, 0);
+      n_seg = max(at + weight - kCost, 0) - first;
+      if (n_seg > 0) return true;
+      advance();  // none of the unit's tiles are in this block
+    }
+    return false;
   }
+  __device__ __forceinline__ bool whole() const { return first == 0 && n_seg == unit.tiles; }
+  // The block that the unit's last tile is in.
+  __device__ __forceinline__ int last_block(int64_t per_block) const { return (int)((t - at + unit.tiles + kCost - 1) / per_block); }
   __device__ __forceinline__ void advance() {
-    t += n_seg;
+    t += weight;
     if (t >= t1) return;
-    off = 0;
+    at = 0;
     if (++j < n_j) return;
     j = 0;
     if (++h < p.c.n_kv_heads) return;
@@ -326,8 +337,8 @@ struct PaWalk {
 
 // The loading warp: the pages of K and V of every tile into a ring of 16 KB stages (K of tile i is fill 2i, V 2i + 1), the
 // scales of its pages by cp.async into slot i % kSlots.
-template <int R, int kStages, int kSlots>
-__device__ __forceinline__ void load_tiles(const PagedAttnKernelParams& p, PaWalk<R>& w, const CUtensorMap* tm_k, const CUtensorMap* tm_v,
+template <int R, int kCost, int kStages, int kSlots>
+__device__ __forceinline__ void load_tiles(const PagedAttnKernelParams& p, PaWalk<R, kCost>& w, const CUtensorMap* tm_k, const CUtensorMap* tm_v,
                                            uint8_t* ring, float* scales, uint64_t* kv_full, uint64_t* kv_empty, uint64_t* sc_full,
                                            volatile int* abort_flag) {
   const int lane = threadIdx.x & 31;
@@ -336,7 +347,7 @@ __device__ __forceinline__ void load_tiles(const PagedAttnKernelParams& p, PaWal
   bool ok = true;
   for (; w.segment() && ok; w.advance()) {
     const int32_t* row = p.c.table + (int64_t)w.ent.seq * p.c.per_row;
-    const int first_page = (w.unit.tile0 + w.off) * per_tile;
+    const int first_page = (w.unit.tile0 + w.first) * per_tile;
     const int pages = (int)(((int64_t)w.ent.len + P - 1) >> p.page_shift);  // pages that hold tokens
     int ahead = lane < per_tile && first_page + lane < pages ? row[first_page + lane] : -1;
     for (int i = 0; i < w.n_seg && ok; ++i) {

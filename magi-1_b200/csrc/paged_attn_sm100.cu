@@ -37,6 +37,7 @@ struct PaShared {
   static constexpr int kStages = R == 16 ? 5 : 4;
   static constexpr int kBlocksPerSm = 2;
   static constexpr int kSlots = 8;                             // tiles whose page scales are kept
+  static constexpr int kCost = 1;                              // beginning and ending a unit, in tiles
   static constexpr int kThreads = 32 * 6;
   static constexpr int kRing = 0;
   // P, a byte per (key, row) and term, two buffers: all four share the 128-byte rows [key] of one tile (term 0 of buffer 0 and
@@ -140,7 +141,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
     tmem_alloc(tmem_slot, L::kTmemCols);
     tmem_relinquish();
   }
-  plan_tiles<R, L::kThreads>(p, smem + L::kRing, start, near);
+  plan_tiles<R, L::kThreads, L::kCost>(p, smem + L::kRing, start, near);
   fence_proxy_async_smem();  // the ring goes over to TMA
   tc_fence_before_sync();
   __syncthreads();
@@ -148,7 +149,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
   const uint32_t tmem_base = *tmem_slot;
   const PaStart st = *start;
 
-  PaWalk<R> walk(p, st, near);
+  PaWalk<R, L::kCost> walk(p, st, near);
 
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer
@@ -156,7 +157,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       tma_prefetch_desc(&tm_k);
       tma_prefetch_desc(&tm_v);
     }
-    load_tiles<R, kStages, L::kSlots>(p, walk, &tm_k, &tm_v, smem + L::kRing, reinterpret_cast<float*>(smem + L::kScales), kv_full, kv_empty, sc_full, abort_flag);
+    load_tiles<R, L::kCost, kStages, L::kSlots>(p, walk, &tm_k, &tm_v, smem + L::kRing, reinterpret_cast<float*>(smem + L::kScales), kv_full, kv_empty, sc_full, abort_flag);
   } else if (warp == 1) {
     // ------------------------------------------------------------------ UMMA issuer
     if (lane == 0) {
@@ -239,7 +240,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
     for (; walk.segment(); walk.advance()) {
       const PaUnit& unit = walk.unit;
       const PaEntry& ent = walk.ent;
-      const int n_seg = walk.n_seg, off = walk.off, h = walk.h;
+      const int n_seg = walk.n_seg, first = walk.first, h = walk.h;
       float* row_s = reinterpret_cast<float*>(smem + L::kRowS) + (units & 1) * R;
       int* row_pos = reinterpret_cast<int*>(smem + L::kRowPos) + (units & 1) * R;
       // ---- query rows of the unit as two e4m3 terms, each row scaled by a power of two so that its largest entry is in (224, 448]
@@ -280,7 +281,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       const float4* n4 = reinterpret_cast<const float4*>(neg_m);
 #pragma unroll 1
       for (int x = 0; x < n_seg; ++x, ++i) {
-        const int k0 = (unit.tile0 + off + x) * kPaTile, pos = k0 + key;
+        const int k0 = (unit.tile0 + first + x) * kPaTile, pos = k0 + key;
         warp_wait(&sc_full[i % L::kSlots], (uint32_t)(i / L::kSlots) & 1, abort_flag);
         warp_wait(&s_full[i & 1], (uint32_t)(i >> 1) & 1, abort_flag);
         const bool tail = k0 + kPaTile > ent.len;                                             // keys behind the sequence's end
@@ -471,7 +472,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
         for (int r = 0; r < R; ++r)
           if (nan_rows >> r & 1u) o[r] = __uint_as_float(0x7fffffffu);
       }
-      if (off == 0 && n_seg == unit.tiles) {
+      if (walk.whole()) {
         const bool owned = lane < R && row < unit.rows;
         const int flat = unit.first + (owned ? row : 0), tok = by_group(p, flat), head = h * p.group + flat - tok * p.group;
         if (owned && ok) {
@@ -488,14 +489,13 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
           if (ok && r < unit.rows) p.out[at_sh[r] + key] = __float2bfloat16_rn(o[r] * inv_sh[r]);
         __syncwarp();
       } else {
-        const int64_t slot = 2 * (int64_t)blockIdx.x + (off == 0 ? 1 : 0);
+        const int64_t slot = 2 * (int64_t)blockIdx.x + (first == 0 ? 1 : 0);
         float* part = p.parts + slot * R * kHeadDim;
 #pragma unroll
         for (int r = 0; r < R; ++r)
           if (r < unit.rows) part[r * kHeadDim + key] = o[r];
         if (sw == 0 && lane < R) p.stats[slot * R + row] = make_float2(m, total);
-        if (off == 0 && sw == 0 && lane == 0)
-          p.headers[blockIdx.x] = {1, walk.b, h, walk.j, (int)((walk.t + unit.tiles - 1) / st.per_block), {0, 0, 0}};
+        if (first == 0 && sw == 0 && lane == 0) p.headers[blockIdx.x] = {1, walk.b, h, walk.j, walk.last_block(st.per_block), {0, 0, 0}};
       }
       ++units;
     }

@@ -23,6 +23,7 @@ int launch_prompt_join(magi_ctx* ctx, const PagedAttnKernelParams& k, cudaStream
 struct PromptShared {
   static constexpr int kStages = 8;
   static constexpr int kSlots = 8;                             // tiles whose page scales are kept
+  static constexpr int kCost = 3;                              // beginning and ending a unit, in tiles
   static constexpr int kThreads = 640;
   static constexpr int kRing = 0;
   static constexpr int kQ = kRing + kStages * kPaTileBytes;    // [2 terms][2 warpgroups][128 rows][128 bytes]
@@ -46,12 +47,6 @@ __device__ __forceinline__ void pair_sync(int x) {
   __syncwarp();
   asm volatile("bar.sync %0, 256;" ::"r"(1 + x) : "memory");
 }
-template <int kThreads>
-__device__ __forceinline__ void named_sync(int id) {
-  __syncwarp();
-  asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(kThreads) : "memory");
-}
-
 // kGroup: consecutive keys that share a page, and so scales, for sure (page_tokens, at most 32).
 template <int kGroup>
 __global__ void __launch_bounds__(PromptShared::kThreads, 1)
@@ -96,14 +91,14 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
-  plan_tiles<R, L::kThreads>(p, smem + L::kRing, start, near);
+  plan_tiles<R, L::kThreads, L::kCost>(p, smem + L::kRing, start, near);
   fence_proxy_async_smem();  // the ring goes over to TMA
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_slot;
   const PaStart st = *start;
-  PaWalk<R> walk(p, st, near);
+  PaWalk<R, L::kCost> walk(p, st, near);
 
   if (warp == 0) {
     if (lane == 0) {
@@ -111,7 +106,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
       tma_prefetch_desc(&tm_v);
     }
     __syncwarp();
-    load_tiles<R, kStages, L::kSlots>(p, walk, &tm_k, &tm_v, smem + L::kRing, reinterpret_cast<float*>(smem + L::kScales), kv_full, kv_empty, sc_full, abort_flag);
+    load_tiles<R, L::kCost, kStages, L::kSlots>(p, walk, &tm_k, &tm_v, smem + L::kRing, reinterpret_cast<float*>(smem + L::kScales), kv_full, kv_empty, sc_full, abort_flag);
   } else if (warp == 1) {
     // ------------------------------------------------------------------ UMMA issuer
     if (elect_one()) {
@@ -124,7 +119,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
       bool ok = true;
       int i = 0;                       // tiles so far
       int seen[2] = {0, 0}, units[2] = {0, 0};  // key tiles and units of each row tile
-      auto first = [&](int x, int fill) {  // S of row tile x
+      auto scores = [&](int x, int fill) {  // S of row tile x
         const uint32_t a = q_lo + x * kTile16, b = ring + (fill % kStages) * kTile16, d = tmem_base + x * 128;
         umma_ss_f8_lh<0>(d, a, b, desc_hi, idesc_s);
 #pragma unroll
@@ -139,7 +134,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
           ok = mbar_wait(&q_full[x], units[x]++ & 1, abort_flag);
           if (!ok) break;
           tc_fence_after_sync();
-          first(x, 2 * i);
+          scores(x, 2 * i);
         }
         if (ok) umma_commit(&kv_empty[(2 * i) % kStages]);
         for (int k = 0; k < walk.n_seg && ok; ++k, ++i) {
@@ -160,7 +155,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             if (!more) umma_commit(&o_full[x]);
             if (x == nx - 1) umma_commit(&kv_empty[v_fill % kStages]);
             if (more) {
-              first(x, k_fill);
+              scores(x, k_fill);
               if (x == nx - 1) umma_commit(&kv_empty[k_fill % kStages]);
             }
           }
@@ -191,7 +186,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     for (; walk.segment(); walk.advance()) {
       const PaUnit& unit = walk.unit;
       const PaEntry& ent = walk.ent;
-      const int n_seg = walk.n_seg, off = walk.off;
+      const int n_seg = walk.n_seg, first = walk.first;
       const int nx = unit.rows > 128 ? 2 : 1;
       if (x >= nx) {  // a short unit leaves the second row tile out
         i += n_seg;
@@ -202,17 +197,17 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
       const int tok = by_group(p, flat), head = walk.h * p.group + flat - tok * p.group;
       const bool owned = x * 128 + row < unit.rows;
       const long long q_at = (int64_t)(ent.row0 + tok) * p.q_st + (int64_t)head * p.q_sh;
-#pragma unroll 1
-      for (int r0 = half * 16; r0 < half * 16 + 16; r0 += 8) {
-        uint2 raw[8];
+      {
+        const int r0 = half * 16;
+        uint2 raw[16];  // all in flight at once
 #pragma unroll
-        for (int r = 0; r < 8; ++r) {
+        for (int r = 0; r < 16; ++r) {
           const long long at = __shfl_sync(0xffffffffu, q_at, r0 + r);
           raw[r] = make_uint2(0, 0);
           if (x * 128 + quarter * 32 + r0 + r < unit.rows) raw[r] = *reinterpret_cast<const uint2*>(p.q + at + lane * 4);
         }
 #pragma unroll
-        for (int r = 0; r < 8; ++r) {
+        for (int r = 0; r < 16; ++r) {
           uint32_t hi, lo;
           const float scale = split_query(raw[r], &hi, &lo);
           const int tr = quarter * 32 + r0 + r;
@@ -232,7 +227,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
       uint32_t nan_ch[4] = {0, 0, 0, 0};    // channels of this row that are NaN (boundary tiles)
 #pragma unroll 1
       for (int k = 0; k < n_seg; ++k, ++i, ++seen) {
-        const int k0 = (unit.tile0 + off + k) * kPaTile;
+        const int k0 = (unit.tile0 + first + k) * kPaTile;
         warp_wait(&sc_full[i % L::kSlots], (uint32_t)(i / L::kSlots) & 1, abort_flag);
         warp_wait(&s_full[x], seen & 1, abort_flag);
         tc_fence_after_sync();
@@ -245,43 +240,47 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         const int begin = p.window > 0 ? max(at_pos - p.window + 1 - k0, 0) : 0;
         // 32 keys at a time, twice over: the scores stay in TMEM in between, so that a thread holds 32 of them and not all.
         // w = s log2e + log2(sv) = raw * kc + bias; the sum adds P / sv.
-        constexpr int kGroups = 64 / kGroup;
-        float kc[kGroups], bias[kGroups], inv[kGroups];
+        constexpr int kPer = 32 / kGroup;
+        auto factors = [&](int at, float (&kc)[kPer], float (&bias)[kPer], float (&inv)[kPer]) {
 #pragma unroll
-        for (int g = 0; g < kGroups; ++g) {
-          const int c = half * 64 + g * kGroup, pg = c >> p.page_shift;
-          const uint32_t vs = __float_as_uint(sc[8 + pg]);
-          kc[g] = fminf(sc[pg] * c1, 3.0e38f);  // finite: a raw score of zero stays zero
-          bias[g] = __uint_as_float(0x4b000000u | vs >> 23) - 8388735.0f;  // its exponent: 2^23 + (e + 127) - (2^23 + 127)
-          inv[g] = c <= last ? __uint_as_float(0x7f000000u - vs) : 0.f;     // behind the end there may be no page
-        }
-        // Columns that every row of this warp sees; those beyond are compared with each row's own border, 16 at a time (the
-        // rows of a warp stand a few positions apart, so one group of 16 or two in a tile).
+          for (int g = 0; g < kPer; ++g) {
+            const int pg = (at + g * kGroup) >> p.page_shift;
+            const uint32_t vs = __float_as_uint(sc[8 + pg]);
+            kc[g] = fminf(sc[pg] * c1, 3.0e38f);  // finite: a raw score of zero stays zero
+            bias[g] = __uint_as_float(0x4b000000u | vs >> 23) - 8388735.0f;  // its exponent: 2^23 + (e + 127) - (2^23 + 127)
+            inv[g] = at + g * kGroup <= last ? __uint_as_float(0x7f000000u - vs) : 0.f;  // behind the end there may be no page
+          }
+        };
+        // At the borders: columns that no row of this warp sees are left out, those that all rows see are like any other.
         const int all_last = __reduce_min_sync(0xffffffffu, last), all_begin = __reduce_max_sync(0xffffffffu, begin);
-        auto clear = [&](int at) { return at + 15 <= all_last && at >= all_begin; };
+        const int any_last = __reduce_max_sync(0xffffffffu, last), any_begin = __reduce_min_sync(0xffffffffu, begin);
+        auto hidden = [&](int at) { return at > any_last || at + 31 < any_begin; };
+        auto mixed = [&](int at) { return at + 31 > all_last || at < all_begin; };
         float t0 = -INFINITY, t1 = -INFINITY;
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          float s[32];
-          tmem_ld32(t_s + half * 64 + q * 32, reinterpret_cast<uint32_t*>(s));
+        auto find_top = [&](int at) {
+          float s[32], kc[kPer], bias[kPer], inv[kPer];
+          tmem_ld32(t_s + at, reinterpret_cast<uint32_t*>(s));
+          factors(at, kc, bias, inv);
           tmem_wait_ld();
 #pragma unroll
-          for (int c = 0; c < 32; ++c) s[c] = fmaf(s[c], kc[(q * 32 + c) / kGroup], bias[(q * 32 + c) / kGroup]);
-          if (border) {
+          for (int c = 0; c < 32; ++c) s[c] = fmaf(s[c], kc[c / kGroup], bias[c / kGroup]);
+          if (border && mixed(at)) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              const int at = half * 64 + q * 32 + u * 16;
-              if (!clear(at)) {
-#pragma unroll
-                for (int c = 0; c < 16; ++c) s[u * 16 + c] = at + c <= last && at + c >= begin ? s[u * 16 + c] : -INFINITY;
-              }
-            }
+            for (int c = 0; c < 32; ++c) s[c] = at + c <= last && at + c >= begin ? s[c] : -INFINITY;
           }
 #pragma unroll
           for (int c = 0; c < 32; c += 4) {
             t0 = max3(t0, s[c], s[c + 1]);
             t1 = max3(t1, s[c + 2], s[c + 3]);
           }
+        };
+        if (!border) {
+          find_top(half * 64);
+          find_top(half * 64 + 32);
+        } else {
+#pragma unroll 1
+          for (int at = half * 64; at < half * 64 + 64; at += 32)
+            if (!hidden(at)) find_top(at);
         }
         float top = fmaxf(t0, t1);
         top_mine[(seen & 1) * 512] = top;
@@ -306,38 +305,55 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             }
           }
         }
-        // ---- weights, their sum, and P as two terms: keys 32 q .. at the first 16 of their scores' columns
+        // ---- weights, their sum, and P as two terms: 32 keys at the first 16 of their scores' columns
         const float plus = m == -INFINITY ? 0.f : kPaShift - m;
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          float s[32];
-          tmem_ld32(t_s + half * 64 + q * 32, reinterpret_cast<uint32_t*>(s));
-          tmem_wait_ld();
+        auto weigh_keys = [&](int at) {
           uint32_t w[16];
+          float s[32], kc[kPer], bias[kPer], inv[kPer], sum[2 * kPer];
+          tmem_ld32(t_s + at, reinterpret_cast<uint32_t*>(s));
+          factors(at, kc, bias, inv);
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const int at = half * 64 + q * 32 + u * 16, g = (q * 32 + u * 16) / kGroup;
-            const float k = kc[g], b = bias[g] + plus;
-            float a0 = 0.f, a1 = 0.f;
-            auto sixteen = [&](auto masked) {  // exponentials and conversions run in different pipes: four keys of each in turn
-#pragma unroll
-              for (int c = 0; c < 16; c += 4) {
-                float p[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  p[e] = ex2(fmaf(s[u * 16 + c + e], k, b));
-                  if constexpr (decltype(masked)::value) p[e] = at + c + e <= last && at + c + e >= begin ? p[e] : 0.f;
-                }
-                a0 += p[0] + p[1];
-                a1 += p[2] + p[3];
-                split_weights(p[0], p[1], p[2], p[3], &w[u * 4 + c / 4], &w[8 + u * 4 + c / 4]);
-              }
-            };
-            if (border && !clear(at)) sixteen(std::true_type());
-            else sixteen(std::false_type());
-            l = fmaf(a0 + a1, inv[g], l);
+          for (int g = 0; g < kPer; ++g) {
+            bias[g] += plus;
+            sum[2 * g] = sum[2 * g + 1] = 0.f;
           }
-          tmem_st16(t_s + half * 64 + q * 32, w);
+          tmem_wait_ld();
+          auto weigh = [&](auto masked) {  // exponentials and conversions run in different pipes: four keys of each in turn
+#pragma unroll
+            for (int c = 0; c < 32; c += 4) {
+              const int g = c / kGroup;
+              float p[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                p[e] = ex2(fmaf(s[c + e], kc[g], bias[g]));
+                if constexpr (decltype(masked)::value) p[e] = at + c + e <= last && at + c + e >= begin ? p[e] : 0.f;
+              }
+              sum[2 * g] += p[0] + p[1];
+              sum[2 * g + 1] += p[2] + p[3];
+              split_weights(p[0], p[1], p[2], p[3], &w[c / 4], &w[8 + c / 4]);
+            }
+          };
+          if (border && mixed(at)) weigh(std::true_type());
+          else weigh(std::false_type());
+#pragma unroll
+          for (int g = 0; g < kPer; ++g) l = fmaf(sum[2 * g] + sum[2 * g + 1], inv[g], l);
+          tmem_st16(t_s + at, w);
+        };
+        if (!border) {
+          weigh_keys(half * 64);
+          weigh_keys(half * 64 + 32);
+        } else {
+#pragma unroll 1
+          for (int at = half * 64; at < half * 64 + 64; at += 32) {
+            if (hidden(at)) {
+              uint32_t w[16];
+#pragma unroll
+              for (int c = 0; c < 16; ++c) w[c] = 0;
+              tmem_st16(t_s + at, w);
+            } else {
+              weigh_keys(at);
+            }
+          }
         }
         if (border) {
           // A weight of zero does not silence a NaN: V of keys behind the end becomes zero, and NaN codes of keys that only
@@ -359,8 +375,14 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             fence_proxy_async_smem();
           }
           if (edge) {
-            if (nx == 2) named_sync<512>(4);
-            else named_sync<256>(3);
+            // row tile 0 goes on when its two halves are through; row tile 1, which runs behind it, waits for its list
+            if (x == 0) {
+              pair_sync(0);
+              if (nx == 2 && half == 0) asm volatile("bar.arrive 3, 384;" ::: "memory");
+            } else {
+              __syncwarp();
+              asm volatile("bar.sync 3, 384;" ::: "memory");
+            }
             const volatile uint32_t* any = nan_any + buf * 4;
             if (any[0] | any[1] | any[2] | any[3]) {
 #pragma unroll 1
@@ -388,9 +410,9 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
       pair_sync(x);
       const float total = l + top_other[0];
       pair_sync(x);     // ... and the sums before the next tile's maxima
-      const bool whole = off == 0 && n_seg == unit.tiles;
+      const bool whole = walk.whole();
       const float inv = whole ? (total != 0.f ? 1.0f / total : 0.f) : 1.0f;  // nothing seen: zero
-      const int64_t slot = (2 * (int64_t)blockIdx.x + (off == 0 ? 1 : 0)) * R + x * 128 + row;
+      const int64_t slot = (2 * (int64_t)blockIdx.x + (first == 0 ? 1 : 0)) * R + x * 128 + row;
       __nv_bfloat16* out = p.out + (int64_t)(ent.row0 + (owned ? tok : 0)) * p.o_st + (int64_t)head * p.o_sh;
       float* part = p.parts + (slot - x * 128 - row) * kHeadDim + (x * 128 + row) * 4;  // [channel / 4][row][4]
 #pragma unroll 1
@@ -418,8 +440,8 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         else if (p.lse && ok)
           p.lse[(int64_t)(ent.row0 + tok) * p.hq + head] = total != 0.f ? (m - kPaShift + log2f(total)) * 0.6931471805599453f : -INFINITY;
       }
-      if (!whole && off == 0 && threadIdx.x == 128)
-        p.headers[blockIdx.x] = {1, walk.b, walk.h, walk.j, (int)((walk.t + unit.tiles - 1) / st.per_block), {0, 0, 0}};
+      if (!whole && first == 0 && threadIdx.x == 128)
+        p.headers[blockIdx.x] = {1, walk.b, walk.h, walk.j, walk.last_block(st.per_block), {0, 0, 0}};
       __syncwarp();
     }
   }
