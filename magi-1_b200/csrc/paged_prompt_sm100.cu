@@ -23,7 +23,7 @@ int launch_prompt_join(magi_ctx* ctx, const PagedAttnKernelParams& k, cudaStream
 struct PromptShared {
   static constexpr int kStages = 8;
   static constexpr int kSlots = 8;                             // tiles whose page scales are kept
-  static constexpr int kCost = 3;                              // beginning and ending a unit, in tiles
+  static constexpr int kCost = 4;                              // beginning and ending a unit, in tiles
   static constexpr int kThreads = 640;
   static constexpr int kRing = 0;
   static constexpr int kQ = kRing + kStages * kPaTileBytes;    // [2 terms][2 warpgroups][128 rows][128 bytes]
@@ -198,23 +198,32 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
       const bool owned = x * 128 + row < unit.rows;
       const long long q_at = (int64_t)(ent.row0 + tok) * p.q_st + (int64_t)head * p.q_sh;
       {
-        const int r0 = half * 16;
-        uint2 raw[16];  // all in flight at once
+        uint2 raw[8];
+        auto fetch = [&](int r0) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const long long at = __shfl_sync(0xffffffffu, q_at, r0 + r);
-          raw[r] = make_uint2(0, 0);
-          if (x * 128 + quarter * 32 + r0 + r < unit.rows) raw[r] = *reinterpret_cast<const uint2*>(p.q + at + lane * 4);
-        }
+          for (int r = 0; r < 8; ++r) {
+            const long long at = __shfl_sync(0xffffffffu, q_at, r0 + r);
+            raw[r] = make_uint2(0, 0);
+            if (x * 128 + quarter * 32 + r0 + r < unit.rows) raw[r] = *reinterpret_cast<const uint2*>(p.q + at + lane * 4);
+          }
+        };
+        fetch(half * 16);
+#pragma unroll 1
+        for (int r0 = half * 16; r0 < half * 16 + 16; r0 += 8) {
+          uint2 now[8];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          uint32_t hi, lo;
-          const float scale = split_query(raw[r], &hi, &lo);
-          const int tr = quarter * 32 + r0 + r;
-          uint8_t* at = smem + L::kQ + x * kPaTileBytes + tr * 128 + (((lane >> 2) ^ (tr & 7)) << 4) + (lane & 3) * 4;
-          *reinterpret_cast<uint32_t*>(at) = hi;
-          *reinterpret_cast<uint32_t*>(at + 2 * kPaTileBytes) = lo;
-          row_s[tr] = scale;  // every lane the same
+          for (int r = 0; r < 8; ++r) now[r] = raw[r];
+          if (r0 == half * 16) fetch(r0 + 8);  // in flight while the first eight are split
+#pragma unroll
+          for (int r = 0; r < 8; ++r) {
+            uint32_t hi, lo;
+            const float scale = split_query(now[r], &hi, &lo);
+            const int tr = quarter * 32 + r0 + r;
+            uint8_t* at = smem + L::kQ + x * kPaTileBytes + tr * 128 + (((lane >> 2) ^ (tr & 7)) << 4) + (lane & 3) * 4;
+            *reinterpret_cast<uint32_t*>(at) = hi;
+            *reinterpret_cast<uint32_t*>(at + 2 * kPaTileBytes) = lo;
+            row_s[tr] = scale;  // every lane the same
+          }
         }
       }
       fence_proxy_async_smem();
@@ -375,13 +384,15 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             fence_proxy_async_smem();
           }
           if (edge) {
-            // row tile 0 goes on when its two halves are through; row tile 1, which runs behind it, waits for its list
+            // Row tile 0 goes on when its two halves are through; row tile 1, which runs behind it, waits for its list.  Row tile 0
+            // can be a tile ahead (its next scores are issued before row tile 1's weights are waited for), so the barrier and
+            // the list go by the tile's parity.
             if (x == 0) {
               pair_sync(0);
-              if (nx == 2 && half == 0) asm volatile("bar.arrive 3, 384;" ::: "memory");
+              if (nx == 2 && half == 0) asm volatile("bar.arrive %0, 384;" ::"r"(3 + buf) : "memory");
             } else {
               __syncwarp();
-              asm volatile("bar.sync 3, 384;" ::: "memory");
+              asm volatile("bar.sync %0, 384;" ::"r"(3 + buf) : "memory");
             }
             const volatile uint32_t* any = nan_any + buf * 4;
             if (any[0] | any[1] | any[2] | any[3]) {
