@@ -23,7 +23,7 @@ int launch_prompt_join(magi_ctx* ctx, const PagedAttnKernelParams& k, cudaStream
 struct PromptShared {
   static constexpr int kStages = 8;
   static constexpr int kSlots = 8;                             // tiles whose page scales are kept
-  static constexpr int kCost = 4;                              // beginning and ending a unit, in tiles
+  static constexpr int kCost = 5;                              // beginning and ending a unit, in tiles
   static constexpr int kThreads = 640;
   static constexpr int kRing = 0;
   static constexpr int kQ = kRing + kStages * kPaTileBytes;    // [2 terms][2 warpgroups][128 rows][128 bytes]
