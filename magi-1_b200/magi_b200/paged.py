@@ -17,21 +17,23 @@ from .ops import HEAD_DIM, KERNEL_LAUNCHES, Context
 
 MAX_ENTRIES = 1024
 _INT32_MAX = 2 ** 31 - 1
+_ATTN_BYTES, _ROTARY_BYTES = C.sizeof(PagedAttnParams), C.sizeof(RotaryParams)
 
 
 def _on(stream, device):
-    """(torch stream the call runs on, its raw handle) - the device's current stream unless one is given."""
-    s = stream if stream is not None else torch.cuda.current_stream(device)
-    if s.device != device:
-        raise ValueError(f"stream belongs to {s.device}, the tensors to {device}")
-    return s, C.c_void_p(s.cuda_stream)
+    """Raw handle of the stream the call runs on: the device's current one unless one is given."""
+    if stream is None:
+        return torch._C._cuda_getCurrentRawStream(device.index)
+    if stream.device != device:
+        raise ValueError(f"stream belongs to {stream.device}, the tensors to {device}")
+    return stream.cuda_stream
 
 
-def _empty_on(s, shape, dtype, device):
-    """torch.empty whose memory belongs to stream s (the caching allocator hands it on in that stream's order)."""
-    if s == torch.cuda.current_stream(device):
+def _empty_on(stream, shape, dtype, device):
+    """torch.empty whose memory belongs to `stream` (the caching allocator hands it on in that stream's order)."""
+    if stream is None:
         return torch.empty(shape, dtype=dtype, device=device)
-    with torch.cuda.stream(s):
+    with torch.cuda.stream(stream):
         return torch.empty(shape, dtype=dtype, device=device)
 
 
@@ -102,6 +104,8 @@ class TokenPagedKVCache:
         for name in ("k8", "v8", "k_scale", "v_scale", "page_table", "seq_lens", "page_refs"):
             setattr(c, name, getattr(self, name).data_ptr())
         c.workspace = self._workspace.data_ptr()
+        self._view_ref = C.byref(c)
+        self._attn_bytes = {}  # workspace sizes by call shape
 
     @property
     def nbytes(self) -> int:
@@ -120,9 +124,9 @@ class TokenPagedKVCache:
         each entry's first new token (int32; -1 throughout when the call is refused), which append takes as `starts`."""
         seqs = self._entries(seqs, "seqs")
         n_new = self._entries(n_new, "n_new", seqs.shape[0])
-        s, raw = _on(stream, self.device)
-        starts = _empty_on(s, (seqs.shape[0],), torch.int32, self.device)
-        check(lib.magi_token_cache_reserve(self.ctx.handle, C.byref(self._view), seqs.data_ptr(), n_new.data_ptr(), seqs.shape[0],
+        raw = _on(stream, self.device)
+        starts = _empty_on(stream, (seqs.shape[0],), torch.int32, self.device)
+        check(lib.magi_token_cache_reserve(self.ctx.handle, self._view_ref, seqs.data_ptr(), n_new.data_ptr(), seqs.shape[0],
                                            starts.data_ptr(), raw), self.ctx.handle)
         KERNEL_LAUNCHES[0] += 1
         return starts
@@ -143,8 +147,8 @@ class TokenPagedKVCache:
             cu_new = _index(cu_new, "cu_new", self.device, seqs.shape[0] + 1)
         elif k.shape[0] != seqs.shape[0] or max_new != 1:
             raise ValueError("without cu_new every entry has one token")
-        _, raw = _on(stream, self.device)
-        check(lib.magi_token_cache_append(self.ctx.handle, C.byref(self._view), int(layer), seqs.data_ptr(), starts.data_ptr(),
+        raw = _on(stream, self.device)
+        check(lib.magi_token_cache_append(self.ctx.handle, self._view_ref, int(layer), seqs.data_ptr(), starts.data_ptr(),
                                           cu_new.data_ptr() if cu_new is not None else None, seqs.shape[0], int(max_new), k.shape[0],
                                           k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), raw),
               self.ctx.handle)
@@ -153,8 +157,8 @@ class TokenPagedKVCache:
     def _branch(self, src, dst, share, stream):
         src = self._entries(src, "src")
         dst = self._entries(dst, "dst", src.shape[0])
-        _, raw = _on(stream, self.device)
-        check(lib.magi_token_cache_branch(self.ctx.handle, C.byref(self._view), src.data_ptr(), dst.data_ptr(), src.shape[0], share, raw),
+        raw = _on(stream, self.device)
+        check(lib.magi_token_cache_branch(self.ctx.handle, self._view_ref, src.data_ptr(), dst.data_ptr(), src.shape[0], share, raw),
               self.ctx.handle)
         KERNEL_LAUNCHES[0] += 2
 
@@ -170,15 +174,15 @@ class TokenPagedKVCache:
     def free(self, seqs: torch.Tensor, stream=None) -> None:
         """Empty the sequences; pages that nobody holds any more become free."""
         seqs = self._entries(seqs, "seqs")
-        _, raw = _on(stream, self.device)
-        check(lib.magi_token_cache_free(self.ctx.handle, C.byref(self._view), seqs.data_ptr(), seqs.shape[0], raw), self.ctx.handle)
+        raw = _on(stream, self.device)
+        check(lib.magi_token_cache_free(self.ctx.handle, self._view_ref, seqs.data_ptr(), seqs.shape[0], raw), self.ctx.handle)
         KERNEL_LAUNCHES[0] += 1
 
     def compact(self, stream=None) -> None:
         """Move the pages in use to the lowest numbers (the i-th one beyond their count to the i-th free one below it) and
         rewrite the tables: afterwards the upper part of every layer's pool is unused."""
-        _, raw = _on(stream, self.device)
-        check(lib.magi_token_cache_compact(self.ctx.handle, C.byref(self._view), raw), self.ctx.handle)
+        raw = _on(stream, self.device)
+        check(lib.magi_token_cache_compact(self.ctx.handle, self._view_ref, raw), self.ctx.handle)
         KERNEL_LAUNCHES[0] += 2
 
 
@@ -201,31 +205,33 @@ def paged_attn(q: torch.Tensor, cache: TokenPagedKVCache, layer: int, seqs: torc
         raise ValueError("without cu_q every entry has one query row")
     if q.shape[1] % cache.n_kv_heads:
         raise ValueError("the query heads must be a multiple of the cache's kv heads")
-    if not 0 <= int(window) <= _INT32_MAX or not 0 <= int(max_q) <= _INT32_MAX:
+    layer, window, max_q = int(layer), int(window), int(max_q)
+    if not 0 <= window <= _INT32_MAX or not 0 <= max_q <= _INT32_MAX:
         raise ValueError("window and max_q must be non-negative 32-bit numbers")
-    s, raw = _on(stream, dev)
+    raw = _on(stream, dev)
+    rows, heads, _ = shape = q.shape
+    stride_t, stride_h, _ = q.stride()
     if out is None:
-        out = _empty_on(s, q.shape, torch.bfloat16, dev)
+        out = _empty_on(stream, shape, torch.bfloat16, dev)
+        out_t, out_h = heads * HEAD_DIM, HEAD_DIM
     else:
-        _rows(out, "out", dev, q.shape[1])
-        if out.shape[0] < q.shape[0]:
+        _rows(out, "out", dev, heads)
+        if out.shape[0] < rows:
             raise ValueError("out must have at least q's rows")
         _one_place_each(out, "out")
-    lse = _empty_on(s, q.shape[:2], torch.float32, dev) if return_lse else None
-    ws = _empty_on(s, (lib.magi_paged_attn_workspace_bytes(cache.ctx.handle, int(max_q), q.shape[1], cache.n_kv_heads),), torch.uint8, dev)
-    p = PagedAttnParams()
-    p.struct_size = C.sizeof(PagedAttnParams)
-    p.layer = int(layer)
-    p.q, p.q_stride_t, p.q_stride_h = q.data_ptr(), q.stride(0), q.stride(1)
-    p.out, p.o_stride_t, p.o_stride_h = out.data_ptr(), out.stride(0), out.stride(1)
-    p.lse = lse.data_ptr() if lse is not None else None
-    p.seqs = seqs.data_ptr()
-    p.cu_q = cu_q.data_ptr() if cu_q is not None else None
-    p.n, p.total_q, p.max_q, p.n_q_heads = seqs.shape[0], q.shape[0], int(max_q), q.shape[1]
-    p.softmax_scale = float(softmax_scale) if softmax_scale else 0.0
-    p.causal, p.window = int(bool(causal)), int(window)
-    p.workspace = ws.data_ptr()
-    check(lib.magi_paged_attn_fwd(cache.ctx.handle, C.byref(cache._view), C.byref(p), raw), cache.ctx.handle)
+        out_t, out_h, _ = out.stride()
+    lse = _empty_on(stream, (rows, heads), torch.float32, dev) if return_lse else None
+    handle = cache.ctx.handle
+    nbytes = cache._attn_bytes.get((max_q, heads))
+    if nbytes is None:
+        nbytes = cache._attn_bytes[max_q, heads] = lib.magi_paged_attn_workspace_bytes(handle, max_q, heads, cache.n_kv_heads)
+    ws = _empty_on(stream, nbytes, torch.uint8, dev)
+    p = PagedAttnParams(
+        struct_size=_ATTN_BYTES, layer=layer, q=q.data_ptr(), q_stride_t=stride_t, q_stride_h=stride_h, out=out.data_ptr(),
+        o_stride_t=out_t, o_stride_h=out_h, lse=lse.data_ptr() if return_lse else None, seqs=seqs.data_ptr(),
+        cu_q=cu_q.data_ptr() if cu_q is not None else None, n=seqs.shape[0], total_q=rows, max_q=max_q, n_q_heads=heads,
+        softmax_scale=softmax_scale or 0.0, causal=bool(causal), window=window, workspace=ws.data_ptr())
+    check(lib.magi_paged_attn_fwd(handle, cache._view_ref, C.byref(p), raw), handle)
     KERNEL_LAUNCHES[0] += 2  # attention and join
     return out, lse
 
@@ -292,9 +298,9 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, lay
     if not isinstance(inv_freq, torch.Tensor) or inv_freq.device != dev or inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 \
             or not inv_freq.is_contiguous() or 2 * inv_freq.shape[0] > D:
         raise ValueError(f"inv_freq must be a contiguous fp64 tensor of at most head_dim / 2 entries on {dev}")
-    s, raw = _on(stream, dev)
+    raw = _on(stream, dev)
     if out is None:
-        out = _empty_on(s, (T, H, D), x.dtype, dev)
+        out = _empty_on(stream, (T, H, D), x.dtype, dev)
     elif out.device != dev or out.dtype != x.dtype or out.shape != x.shape or (D > 1 and out.stride(2) != 1):
         raise ValueError("out must have x's shape, dtype and device and a contiguous last dim")
     elif out.data_ptr() == x.data_ptr() and out.stride() != x.stride():
@@ -303,15 +309,12 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, lay
         _one_place_each(out, "out")
     if T == 0 or H == 0 or D == 0:
         return out
-    p = RotaryParams()
-    p.struct_size = C.sizeof(RotaryParams)
-    p.dtype = _ROTARY_DTYPES[x.dtype]
-    p.x, p.x_stride_t, p.x_stride_h = x.data_ptr(), x.stride(0), x.stride(1)
-    p.out, p.out_stride_t, p.out_stride_h = out.data_ptr(), out.stride(0), out.stride(1)
-    p.positions, p.positions_are_int64 = positions.data_ptr(), int(positions.dtype == torch.int64)
-    p.T, p.H, p.head_dim, p.rot_dim = T, H, D, 2 * inv_freq.shape[0]
-    p.interleaved, p.inverse, p.mscale = int(layout == "interleaved"), int(bool(inverse)), float(mscale)
-    p.inv_freq = inv_freq.data_ptr()
+    (x_t, x_h, _), (out_t, out_h, _) = x.stride(), out.stride()
+    p = RotaryParams(
+        struct_size=_ROTARY_BYTES, dtype=_ROTARY_DTYPES[x.dtype], x=x.data_ptr(), x_stride_t=x_t, x_stride_h=x_h, out=out.data_ptr(),
+        out_stride_t=out_t, out_stride_h=out_h, positions=positions.data_ptr(), positions_are_int64=positions.dtype is torch.int64,
+        T=T, H=H, head_dim=D, rot_dim=2 * inv_freq.shape[0], interleaved=layout == "interleaved", inverse=bool(inverse), mscale=mscale,
+        inv_freq=inv_freq.data_ptr())
     ctx = Context.get(dev)
     check(lib.magi_rotary_fwd(ctx.handle, C.byref(p), raw), ctx.handle)
     KERNEL_LAUNCHES[0] += 1
