@@ -37,8 +37,9 @@ struct PaShared {
   static constexpr int kStages = R == 16 ? 5 : 4;
   static constexpr int kBlocksPerSm = 2;
   static constexpr int kSlots = 8;                             // tiles whose page scales are kept
-  static constexpr int kCost = 1;                              // beginning and ending a unit, in tiles
-  static constexpr int kThreads = 32 * 6;
+  static constexpr int kCost = 4;                              // beginning and ending a unit, in tiles
+  static constexpr int kGroups = R / 16;                       // of four softmax warps, 16 rows each
+  static constexpr int kThreads = 64 + 128 * kGroups;
   static constexpr int kRing = 0;
   // P, a byte per (key, row) and term, two buffers: all four share the 128-byte rows [key] of one tile (term 0 of buffer 0 and
   // 1, then term 1 of both, 32 bytes each)
@@ -49,12 +50,12 @@ struct PaShared {
   static constexpr int kNegM = kMax + 4 * R * 4;               // [R]
   static constexpr int kFactor = kNegM + R * 4;                // [R]
   static constexpr int kRowS = kFactor + R * 4;                // [2][R] scale of a query row
-  static constexpr int kRowPos = kRowS + 2 * R * 4;            // [2][R] its position
-  static constexpr int kInv = kRowPos + 2 * R * 4;             // [4][R]
+  static constexpr int kRowKeys = kRowS + 2 * R * 4;           // [2][R] the keys it sees: first one, how many
+  static constexpr int kInv = kRowKeys + 2 * R * 8;            // [4][R]
   static constexpr int kAt = kInv + 4 * R * 4;                 // [4][R] where a row of the result starts
-  static constexpr int kNan = kAt + 4 * R * 8;                 // [128][4] channels whose V is NaN (boundary tiles)
-  static constexpr int kNanAny = kNan + kPaTile * 16;          // [4] whether a warp's keys have any
-  static constexpr int kNear = kNanAny + 16;                   // [kPaNear] entries
+  static constexpr int kNan = kAt + 4 * R * 8;                 // [kGroups][128][4] channels whose V is NaN (boundary tiles)
+  static constexpr int kNanAny = kNan + kGroups * kPaTile * 16;  // [4] whether a warp's keys have any
+  static constexpr int kNear = kNanAny + kGroups * 16;         // [kPaNear] entries
   static constexpr int kStart = kNear + kPaNear * 16;
   static constexpr int kBar = kStart + 64;
   static constexpr int kNumBars = 2 * kStages + kSlots + 8;
@@ -75,28 +76,23 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
       : "r"(taddr)
       : "memory");
 }
-template <int N>
-__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t* r) {
-  if constexpr (N == 16) tmem_ld16(taddr, r);
-  else tmem_ld32(taddr, r);
-}
-// Barriers of the four softmax warps.  A warp counts once only if its lanes arrive together.
-__device__ __forceinline__ bool softmax_any(bool v) {
+// Barriers of the four softmax warps of group g.  A warp counts once only if its lanes arrive together.
+__device__ __forceinline__ bool group_any(int g, bool v) {
   uint32_t r;
   __syncwarp();
   asm volatile(
       "{\n\t.reg .pred a, b;\n\t"
       "setp.ne.u32 a, %1, 0;\n\t"
-      "bar.red.or.pred b, 1, 128, a;\n\t"
+      "bar.red.or.pred b, %2, 128, a;\n\t"
       "selp.u32 %0, 1, 0, b;\n\t}"
       : "=r"(r)
-      : "r"((uint32_t)v)
+      : "r"((uint32_t)v), "r"(1 + g)
       : "memory");
   return r != 0;
 }
-__device__ __forceinline__ void softmax_sync() {
+__device__ __forceinline__ void group_sync(int g) {
   __syncwarp();
-  asm volatile("bar.sync 1, 128;" ::: "memory");
+  asm volatile("bar.sync %0, 128;" ::"r"(1 + g) : "memory");
 }
 template <int R>
 __global__ void __launch_bounds__(PaShared<R>::kThreads, PaShared<R>::kBlocksPerSm)
@@ -129,10 +125,10 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
     for (int s = 0; s < L::kSlots; ++s) mbar_init(&sc_full[s], 32);  // each lane of the loading warp
     for (int x = 0; x < 2; ++x) {
       mbar_init(&s_full[x], 1);
-      mbar_init(&p_full[x], 4);
+      mbar_init(&p_full[x], 4 * L::kGroups);
       mbar_init(&o_full[x], 1);
     }
-    mbar_init(q_full, 4);
+    mbar_init(q_full, 4 * L::kGroups);
     mbar_init(drain_bar, 1);
     *abort_flag = 0;
     fence_mbar_init();
@@ -160,7 +156,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
     load_tiles<R, L::kCost, kStages, L::kSlots>(p, walk, &tm_k, &tm_v, smem + L::kRing, reinterpret_cast<float*>(smem + L::kScales), kv_full, kv_empty, sc_full, abort_flag);
   } else if (warp == 1) {
     // ------------------------------------------------------------------ UMMA issuer
-    if (lane == 0) {
+    if (elect_one()) {
       constexpr uint32_t idesc_s = umma_idesc(kPaTile, R, 0, 0, 0, 0);
       constexpr uint32_t idesc_o = umma_idesc(kHeadDim, R, 0, 0, 1, 1), idesc_r = umma_idesc(kHeadDim, R, 0, 1, 1, 1);  // B e4m3, e5m2
       constexpr uint32_t desc_hi = (1024u >> 4) | (1u << 14) | (2u << 29);  // 1024 bytes between groups of 8 rows, 128-byte swizzle
@@ -223,34 +219,33 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
   } else {
     // ------------------------------------------------------------------ softmax and output
     // No early exits in here: a warp whose wait gave up goes on, so that the named barriers always meet.
-    const int sw = warp - 2;
+    constexpr int RG = 16;                    // rows of a group
+    const int sw = warp - 2, g = sw >> 2, wq = sw & 3;
     const int quarter = warp & 3;             // TMEM lanes of this warp
     const int key = quarter * 32 + lane;      // key of the tile; channel of the output
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
-    const uint32_t t_o = tmem_base + lane_base + 2 * R;
+    const uint32_t t_o = tmem_base + lane_base + 2 * R + g * RG;
     const float* scales = reinterpret_cast<const float*>(smem + L::kScales);
-    float* max_sh = reinterpret_cast<float*>(smem + L::kMax);
-    float* neg_m = reinterpret_cast<float*>(smem + L::kNegM);     // kPaShift - reference maximum of a row
-    float* factor = reinterpret_cast<float*>(smem + L::kFactor);
-    float* inv_sh = reinterpret_cast<float*>(smem + L::kInv) + sw * R;
-    int64_t* at_sh = reinterpret_cast<int64_t*>(smem + L::kAt) + sw * R;
-    uint4* nan_sh = reinterpret_cast<uint4*>(smem + L::kNan);
-    volatile uint32_t* nan_any = reinterpret_cast<uint32_t*>(smem + L::kNanAny);
+    float* max_sh = reinterpret_cast<float*>(smem + L::kMax) + g * 4 * RG;
+    float* neg_m = reinterpret_cast<float*>(smem + L::kNegM) + g * RG;  // kPaShift - reference maximum of a row
+    float* factor = reinterpret_cast<float*>(smem + L::kFactor) + g * RG;
+    float* inv_sh = reinterpret_cast<float*>(smem + L::kInv) + sw * RG;
+    int64_t* at_sh = reinterpret_cast<int64_t*>(smem + L::kAt) + sw * RG;
     int i = 0, units = 0;
     for (; walk.segment(); walk.advance()) {
       const PaUnit& unit = walk.unit;
       const PaEntry& ent = walk.ent;
       const int n_seg = walk.n_seg, first = walk.first, h = walk.h;
       float* row_s = reinterpret_cast<float*>(smem + L::kRowS) + (units & 1) * R;
-      int* row_pos = reinterpret_cast<int*>(smem + L::kRowPos) + (units & 1) * R;
+      int2* row_keys = reinterpret_cast<int2*>(smem + L::kRowKeys) + (units & 1) * R;
       // ---- query rows of the unit as two e4m3 terms, each row scaled by a power of two so that its largest entry is in (224, 448]
       {
-        constexpr int kMine = R / 4;
+        constexpr int kMine = 4, kWarps = 4 * L::kGroups;
         uint2 raw[kMine];
         int toks[kMine];
 #pragma unroll
         for (int x = 0; x < kMine; ++x) {
-          const int r = sw + x * 4, flat = unit.first + r;
+          const int r = sw + x * kWarps, flat = unit.first + r;
           toks[x] = by_group(p, flat);
           raw[x] = make_uint2(0, 0);
           if (r < unit.rows)
@@ -258,26 +253,26 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
         }
 #pragma unroll
         for (int x = 0; x < kMine; ++x) {
-          const int r = sw + x * 4;
+          const int r = sw + x * kWarps;
           uint32_t hi, lo;
           const float scale = split_query(raw[x], &hi, &lo);
-          const int at = r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4;
-          *reinterpret_cast<uint32_t*>(smem + L::kQ + at) = hi;
-          *reinterpret_cast<uint32_t*>(smem + L::kQ + R * 128 + at) = lo;
+          uint8_t* to = smem + L::kQ + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4;
+          *reinterpret_cast<uint32_t*>(to) = hi;
+          *reinterpret_cast<uint32_t*>(to + R * 128) = lo;
           row_s[r] = scale * p.scale_log2;  // every lane the same
-          row_pos[r] = ent.len - ent.n_q + toks[x];
+          const int at = ent.len - ent.n_q + toks[x], from = p.window > 0 ? max(at - p.window + 1, 0) : 0;
+          row_keys[r] = make_int2(from, max((p.causal ? min(at + 1, ent.len) : ent.len) - from, 0));
         }
-        if (sw == 0 && lane < R) neg_m[lane] = INFINITY;
       }
       fence_proxy_async_smem();
       warp_arrive(q_full);
       warp_wait(q_full, units & 1, abort_flag);  // the other warps' row scales and positions
-      float m = -INFINITY;    // lane r < R: reference maximum of row r, at most kPaLimit - kPaShift below the running one
+      float m = -INFINITY;    // lane r < RG: reference maximum of row r of the group, at most kPaLimit - kPaShift below the running one
       uint32_t nan_rows = 0;  // rows whose result in this thread's channel is NaN (boundary tiles)
-      uint64_t l2[R / 2];    // sums over this thread's keys, rows in pairs
+      uint64_t l2[RG / 2];    // sums over this thread's keys, rows in pairs
 #pragma unroll
-      for (int k = 0; k < R / 2; ++k) l2[k] = 0;
-      const float4* s4 = reinterpret_cast<const float4*>(row_s);
+      for (int k = 0; k < RG / 2; ++k) l2[k] = 0;
+      const float4* s4 = reinterpret_cast<const float4*>(row_s + g * RG);
       const float4* n4 = reinterpret_cast<const float4*>(neg_m);
 #pragma unroll 1
       for (int x = 0; x < n_seg; ++x, ++i) {
@@ -288,40 +283,46 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
         // keys before it that not every row sees
         const bool edge = (p.causal && min(k0 + kPaTile, ent.len) - 1 > unit.pos_a) || (p.window > 0 && k0 <= unit.pos_z - p.window);
         tc_fence_after_sync();
-        const uint32_t t_s = tmem_base + lane_base + (i & 1) * R;
-        float w[R];  // exponents of the weights: s log2e + log2(sv) - reference + kPaShift
-        tmem_ld<R>(t_s, reinterpret_cast<uint32_t*>(w));
+        const uint32_t t_s = tmem_base + lane_base + (i & 1) * R + g * RG;
+        float w[RG];  // exponents of the weights: s log2e + log2(sv) - reference + kPaShift
+        tmem_ld16(t_s, reinterpret_cast<uint32_t*>(w));
         const float ks = scales[(i % L::kSlots) * 16 + (key >> p.page_shift)];
         const uint32_t vs = __float_as_uint(scales[(i % L::kSlots) * 16 + 8 + (key >> p.page_shift)]);
         const float bias = (float)((int)(vs >> 23) - 127);                                    // log2 of a power of two
         const float inv_vs = pos < ent.len ? __uint_as_float(0x7f000000u - vs) : 0.f;         // behind the end there is no page
         const uint64_t ks2 = f2_pack(ks, ks), bias2 = f2_pack(bias, bias);
         auto hide = [&]() {
-          const int* rp = row_pos;
+          const int4* keys = reinterpret_cast<const int4*>(row_keys + g * RG);
 #pragma unroll
-          for (int r = 0; r < R; ++r) {
-            const int at = rp[r];
-            const bool seen = pos < ent.len && (!p.causal || pos <= at) && (p.window <= 0 || pos > at - p.window);
-            if (!seen) w[r] = -INFINITY;
+          for (int r = 0; r < RG; r += 2) {
+            const int4 k = keys[r / 2];
+            if ((uint32_t)(pos - k.x) >= (uint32_t)k.y) w[r] = -INFINITY;
+            if ((uint32_t)(pos - k.z) >= (uint32_t)k.w) w[r + 1] = -INFINITY;
           }
         };
         tmem_wait_ld();
+        bool low = x == 0;  // some row's reference is too low (there is none in a unit's first tile)
+        if (!low) {
 #pragma unroll
-        for (int r = 0; r < R; r += 4) {
-          const float4 s = s4[r / 4], n = n4[r / 4];
-          f2_unpack(f2_fma(f2_mul(f2_pack(w[r], w[r + 1]), ks2), f2_pack(s.x, s.y), f2_add(bias2, f2_pack(n.x, n.y))), w[r], w[r + 1]);
-          f2_unpack(f2_fma(f2_mul(f2_pack(w[r + 2], w[r + 3]), ks2), f2_pack(s.z, s.w), f2_add(bias2, f2_pack(n.z, n.w))), w[r + 2], w[r + 3]);
+          for (int r = 0; r < RG; r += 4) {
+            const float4 s = s4[r / 4], n = n4[r / 4];
+            f2_unpack(f2_fma(f2_mul(f2_pack(w[r], w[r + 1]), ks2), f2_pack(s.x, s.y), f2_add(bias2, f2_pack(n.x, n.y))), w[r], w[r + 1]);
+            f2_unpack(f2_fma(f2_mul(f2_pack(w[r + 2], w[r + 3]), ks2), f2_pack(s.z, s.w), f2_add(bias2, f2_pack(n.z, n.w))), w[r + 2], w[r + 3]);
+          }
+          if (tail || edge) hide();
+          float top = fmaxf(w[0], w[1]);
+#pragma unroll
+          for (int r = 2; r < RG; r += 2) top = max3(top, w[r], w[r + 1]);
+          low = group_any(g, top > kPaLimit);
         }
-        if (tail || edge) hide();
-        float top = fmaxf(w[0], w[1]);
+        if (low) {
+          // ---- the exact maxima, from the scores again
+          if (x > 0) {
+            tmem_ld16(t_s, reinterpret_cast<uint32_t*>(w));
+            tmem_wait_ld();
+          }
 #pragma unroll
-        for (int r = 2; r < R; r += 2) top = max3(top, w[r], w[r + 1]);
-        if (softmax_any(top > kPaLimit)) {
-          // ---- some row's reference is too low (always so in a unit's first tile): the exact maxima, from the scores again
-          tmem_ld<R>(t_s, reinterpret_cast<uint32_t*>(w));
-          tmem_wait_ld();
-#pragma unroll
-          for (int r = 0; r < R; r += 4) {
+          for (int r = 0; r < RG; r += 4) {
             const float4 s = s4[r / 4];
             w[r] = fmaf(w[r] * ks, s.x, bias);
             w[r + 1] = fmaf(w[r + 1] * ks, s.y, bias);
@@ -331,58 +332,55 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
           if (tail || edge) hide();
           float mine = -INFINITY;
 #pragma unroll
-          for (int r = 0; r < R; ++r) {
+          for (int r = 0; r < RG; ++r) {
             const float mx = warp_max(w[r]);
             if (lane == r) mine = mx;
           }
-          if (lane < R) max_sh[sw * R + lane] = mine;
-          softmax_sync();
-          if (lane < R) {
-            const float m_new = fmaxf(fmaxf(fmaxf(m, max_sh[lane]), max_sh[R + lane]), fmaxf(max_sh[2 * R + lane], max_sh[3 * R + lane]));
-            if (sw == 0) {
+          if (lane < RG) max_sh[wq * RG + lane] = mine;
+          group_sync(g);
+          if (lane < RG) {
+            const float m_new = fmaxf(fmaxf(fmaxf(m, max_sh[lane]), max_sh[RG + lane]), fmaxf(max_sh[2 * RG + lane], max_sh[3 * RG + lane]));
+            if (wq == 0) {
               neg_m[lane] = kPaShift - m_new;
               factor[lane] = m_new == -INFINITY ? 1.0f : ex2(m - m_new);
             }
             m = m_new;
           }
-          softmax_sync();
+          group_sync(g);
           const float4* f4 = reinterpret_cast<const float4*>(factor);
 #pragma unroll
-          for (int r = 0; r < R; r += 4) {
-            const float4 n = n4[r / 4], f = f4[r / 4];
+          for (int r = 0; r < RG; r += 4) {
+            const float4 n = n4[r / 4];
             w[r] = w[r] == -INFINITY ? w[r] : w[r] + n.x;
             w[r + 1] = w[r + 1] == -INFINITY ? w[r + 1] : w[r + 1] + n.y;
             w[r + 2] = w[r + 2] == -INFINITY ? w[r + 2] : w[r + 2] + n.z;
             w[r + 3] = w[r + 3] == -INFINITY ? w[r + 3] : w[r + 3] + n.w;
-            l2[r / 2] = f2_mul(l2[r / 2], f2_pack(f.x, f.y));
-            l2[r / 2 + 1] = f2_mul(l2[r / 2 + 1], f2_pack(f.z, f.w));
           }
-          if (x > 0) {  // what the tensor core has summed so far
+          if (x > 0) {  // what has been summed so far, here and by the tensor core
             warp_wait(&o_full[(i - 1) & 1], (uint32_t)((i - 1) >> 1) & 1, abort_flag);
             tc_fence_after_sync();
+            uint32_t o[RG];
+            tmem_ld16(t_o, o);
+            tmem_wait_ld();
 #pragma unroll
-            for (int c = 0; c < R; c += 16) {
-              uint32_t o[16];
-              tmem_ld16(t_o + c, o);
-              tmem_wait_ld();
-#pragma unroll
-              for (int r = 0; r < 16; r += 4) {
-                const float4 f = f4[(c + r) / 4];
-                o[r] = __float_as_uint(__uint_as_float(o[r]) * f.x);
-                o[r + 1] = __float_as_uint(__uint_as_float(o[r + 1]) * f.y);
-                o[r + 2] = __float_as_uint(__uint_as_float(o[r + 2]) * f.z);
-                o[r + 3] = __float_as_uint(__uint_as_float(o[r + 3]) * f.w);
-              }
-              tmem_st16(t_o + c, o);
+            for (int r = 0; r < RG; r += 4) {
+              const float4 f = f4[r / 4];
+              l2[r / 2] = f2_mul(l2[r / 2], f2_pack(f.x, f.y));
+              l2[r / 2 + 1] = f2_mul(l2[r / 2 + 1], f2_pack(f.z, f.w));
+              o[r] = __float_as_uint(__uint_as_float(o[r]) * f.x);
+              o[r + 1] = __float_as_uint(__uint_as_float(o[r + 1]) * f.y);
+              o[r + 2] = __float_as_uint(__uint_as_float(o[r + 2]) * f.z);
+              o[r + 3] = __float_as_uint(__uint_as_float(o[r + 3]) * f.w);
             }
+            tmem_st16(t_o, o);
             tmem_wait_st();
           }
         }
         // ---- weights, their sum, and P as two e4m3 terms
-        uint32_t hi[R / 4], lo[R / 4];
+        uint32_t hi[RG / 4], lo[RG / 4];
         const uint64_t inv2 = f2_pack(inv_vs, inv_vs);
 #pragma unroll
-        for (int r = 0; r < R; r += 4) {
+        for (int r = 0; r < RG; r += 4) {
           const float p0 = ex2(w[r]), p1 = ex2(w[r + 1]), p2 = ex2(w[r + 2]), p3 = ex2(w[r + 3]);
           l2[r / 2] = f2_fma(f2_pack(p0, p1), inv2, l2[r / 2]);
           l2[r / 2 + 1] = f2_fma(f2_pack(p2, p3), inv2, l2[r / 2 + 1]);
@@ -391,40 +389,44 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
         // the buffer of tile i - 2
         if (i >= 2) warp_wait(&o_full[i & 1], (uint32_t)((i - 2) >> 1) & 1, abort_flag);
         uint8_t* pb = smem + L::kP + key * 128;
-#pragma unroll
-        for (int c = 0; c < R / 16; ++c) {
-          const int chunk = (i & 1) * 2 + c;  // 16 rows
-          *reinterpret_cast<uint4*>(pb + ((chunk ^ (key & 7)) << 4)) = make_uint4(hi[4 * c], hi[4 * c + 1], hi[4 * c + 2], hi[4 * c + 3]);
-          *reinterpret_cast<uint4*>(pb + (((chunk + 4) ^ (key & 7)) << 4)) = make_uint4(lo[4 * c], lo[4 * c + 1], lo[4 * c + 2], lo[4 * c + 3]);
-        }
+        const int chunk = (i & 1) * 2 + g;  // 16 rows
+        *reinterpret_cast<uint4*>(pb + ((chunk ^ (key & 7)) << 4)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<uint4*>(pb + (((chunk + 4) ^ (key & 7)) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         if (tail || edge) {
           // A weight of zero does not silence a NaN: V of keys behind the end becomes zero, and NaN codes of keys that only
-          // some rows see are taken out of the product and come back through the sums of the rows that do see them.
-          const int v_fill = 2 * i + 1, v_stage = v_fill % kStages;
-          warp_wait(&kv_full[v_stage], (uint32_t)(v_fill / kStages) & 1, abort_flag);
-          __syncwarp();
-          uint4* vrow = reinterpret_cast<uint4*>(smem + L::kRing + v_stage * kPaTileBytes + key * 128);
-          if (pos >= ent.len) {
+          // some rows see are taken out of the product and come back through the sums of the rows that do see them.  The first
+          // group does that; the second can be a tile behind it, not two, so the lists go by the tile's parity.
+          const int v_fill = 2 * i + 1, v_stage = v_fill % kStages, buf = i & (L::kGroups - 1);
+          uint4* nan_sh = reinterpret_cast<uint4*>(smem + L::kNan) + buf * kPaTile;
+          volatile uint32_t* nan_any = reinterpret_cast<uint32_t*>(smem + L::kNanAny) + buf * 4;
+          if (g == 0) {
+            warp_wait(&kv_full[v_stage], (uint32_t)(v_fill / kStages) & 1, abort_flag);
+            __syncwarp();
+            uint4* vrow = reinterpret_cast<uint4*>(smem + L::kRing + v_stage * kPaTileBytes + key * 128);
+            if (pos >= ent.len) {
 #pragma unroll
-            for (int c = 0; c < 8; ++c) vrow[c] = make_uint4(0, 0, 0, 0);
+              for (int c = 0; c < 8; ++c) vrow[c] = make_uint4(0, 0, 0, 0);
+            }
+            if (edge) {
+              uint32_t bits[4] = {0, 0, 0, 0};
+              if (pos < ent.len) take_nan(vrow, key, bits);
+              nan_sh[key] = make_uint4(bits[0], bits[1], bits[2], bits[3]);
+              nan_any[wq] = __any_sync(0xffffffffu, (bits[0] | bits[1] | bits[2] | bits[3]) != 0);  // every lane the same
+            }
           }
           if (edge) {
-            uint32_t bits[4] = {0, 0, 0, 0};
-            if (pos < ent.len) take_nan(vrow, key, bits);
-            nan_sh[key] = make_uint4(bits[0], bits[1], bits[2], bits[3]);
-            nan_any[sw] = __any_sync(0xffffffffu, (bits[0] | bits[1] | bits[2] | bits[3]) != 0);  // every lane the same
-            softmax_sync();
+            __syncwarp();
+            asm volatile("bar.sync 3, %0;" ::"n"(128 * L::kGroups) : "memory");
             if (nan_any[0] | nan_any[1] | nan_any[2] | nan_any[3]) {
               // this thread's channel: the rows that see a key whose V is NaN there
               const uint32_t* words = reinterpret_cast<const uint32_t*>(nan_sh) + quarter;
 #pragma unroll 1
               for (int kk = 0; kk < kPaTile; ++kk) {
                 if (!(words[kk * 4] >> lane & 1u)) continue;
-                const int at_key = k0 + kk;
 #pragma unroll 1
-                for (int r = 0; r < R; ++r) {
-                  const int at = row_pos[r];
-                  if ((!p.causal || at_key <= at) && (p.window <= 0 || at_key > at - p.window)) nan_rows |= 1u << r;
+                for (int r = 0; r < RG; ++r) {
+                  const int2 k = row_keys[g * RG + r];
+                  if ((uint32_t)(k0 + kk - k.x) < (uint32_t)k.y) nan_rows |= 1u << r;
                 }
               }
               __syncwarp();
@@ -439,62 +441,60 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       warp_wait(&o_full[(i - 1) & 1], (uint32_t)((i - 1) >> 1) & 1, abort_flag);
       const bool ok = *abort_flag == 0;
       tc_fence_after_sync();
-      float o[R];
-      tmem_ld<R>(t_o, reinterpret_cast<uint32_t*>(o));
+      float o[RG];
+      tmem_ld16(t_o, reinterpret_cast<uint32_t*>(o));
       {
-        float v[R];
+        float v[RG];
 #pragma unroll
-        for (int k = 0; k < R / 2; ++k) f2_unpack(l2[k], v[2 * k], v[2 * k + 1]);
-        // halves of the rows change lanes while the sums are formed: lane x ends with row x (R = 32) or x / 2 (R = 16)
-        int width = R;
+        for (int k = 0; k < RG / 2; ++k) f2_unpack(l2[k], v[2 * k], v[2 * k + 1]);
+        // halves of the rows change lanes while the sums are formed: lanes 2 x and 2 x + 1 end with row x
+        int width = RG;
 #pragma unroll
-        for (int d = 16; d > 0; d >>= 1) {
-          if (width > 1) {
-            width >>= 1;
+        for (int d = 16; d > 1; d >>= 1) {
+          width >>= 1;
 #pragma unroll
-            for (int k = 0; k < R / 2; ++k)
-              if (k < width) {
-                const float send = lane & d ? v[k] : v[k + width], keep = lane & d ? v[k + width] : v[k];
-                v[k] = keep + __shfl_xor_sync(0xffffffffu, send, d);
-              }
-          } else {
-            v[0] += __shfl_xor_sync(0xffffffffu, v[0], d);
-          }
+          for (int k = 0; k < RG / 2; ++k)
+            if (k < width) {
+              const float send = lane & d ? v[k] : v[k + width], keep = lane & d ? v[k + width] : v[k];
+              v[k] = keep + __shfl_xor_sync(0xffffffffu, send, d);
+            }
         }
-        if (R == 32 || (lane & 1) == 0) max_sh[sw * R + (R == 32 ? lane : lane >> 1)] = v[0];
+        v[0] += __shfl_xor_sync(0xffffffffu, v[0], 1);
+        if ((lane & 1) == 0) max_sh[wq * RG + (lane >> 1)] = v[0];
       }
-      softmax_sync();
-      const int row = lane;  // of lanes < R
-      const float total = lane < R ? (max_sh[lane] + max_sh[R + lane]) + (max_sh[2 * R + lane] + max_sh[3 * R + lane]) : 0.f;
+      group_sync(g);
+      const int row = g * RG + lane;  // of lanes < RG
+      const float total = lane < RG ? (max_sh[lane] + max_sh[RG + lane]) + (max_sh[2 * RG + lane] + max_sh[3 * RG + lane]) : 0.f;
       tmem_wait_ld();
       if (nan_rows) {
 #pragma unroll
-        for (int r = 0; r < R; ++r)
+        for (int r = 0; r < RG; ++r)
           if (nan_rows >> r & 1u) o[r] = __uint_as_float(0x7fffffffu);
       }
+      const int rows = unit.rows - g * RG;  // of this group, when positive
       if (walk.whole()) {
-        const bool owned = lane < R && row < unit.rows;
+        const bool owned = lane < RG && lane < rows;
         const int flat = unit.first + (owned ? row : 0), tok = by_group(p, flat), head = h * p.group + flat - tok * p.group;
         if (owned && ok) {
-          if (p.lse && sw == 0)
+          if (p.lse && wq == 0)
             p.lse[(int64_t)(ent.row0 + tok) * p.hq + head] = total != 0.f ? (m - kPaShift + log2f(total)) * 0.6931471805599453f : -INFINITY;
         }
-        if (lane < R) {
+        if (lane < RG) {
           inv_sh[lane] = total != 0.f ? 1.0f / total : 0.f;  // nothing seen: zero
           at_sh[lane] = (int64_t)(ent.row0 + tok) * p.o_st + (int64_t)head * p.o_sh;
         }
         __syncwarp();
 #pragma unroll
-        for (int r = 0; r < R; ++r)
-          if (ok && r < unit.rows) p.out[at_sh[r] + key] = __float2bfloat16_rn(o[r] * inv_sh[r]);
+        for (int r = 0; r < RG; ++r)
+          if (ok && r < rows) p.out[at_sh[r] + key] = __float2bfloat16_rn(o[r] * inv_sh[r]);
         __syncwarp();
       } else {
         const int64_t slot = 2 * (int64_t)blockIdx.x + (first == 0 ? 1 : 0);
-        float* part = p.parts + slot * R * kHeadDim;
+        float* part = p.parts + (slot * R + g * RG) * kHeadDim;
 #pragma unroll
-        for (int r = 0; r < R; ++r)
-          if (r < unit.rows) part[r * kHeadDim + key] = o[r];
-        if (sw == 0 && lane < R) p.stats[slot * R + row] = make_float2(m, total);
+        for (int r = 0; r < RG; ++r)
+          if (r < rows) part[r * kHeadDim + key] = o[r];
+        if (wq == 0 && lane < RG) p.stats[slot * R + row] = make_float2(m, total);
         if (first == 0 && sw == 0 && lane == 0) p.headers[blockIdx.x] = {1, walk.b, h, walk.j, walk.last_block(st.per_block), {0, 0, 0}};
       }
       ++units;
