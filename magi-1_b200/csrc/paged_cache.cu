@@ -13,6 +13,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 
+#include <algorithm>
+
 #include "paged.cuh"
 
 namespace magi {
@@ -400,45 +402,52 @@ __device__ __forceinline__ uint2 pack8_e4m3(const float* f) {
   return make_uint2(w[0], w[1]);
 }
 
-// One block per (page that an entry touches, kv head, entry, K or V): 256 threads, thread = (row group, 8 channels); the
-// page's new tokens stay in registers between the search for the largest value and the conversion, so HBM sees one read and
-// one half-size write.  Tokens that the page holds already are read only when its scale grows.
-__global__ void __launch_bounds__(256) paged_append_kernel(const PagedView c, const AppendParams p, int* status) {
-  const int entry = blockIdx.z >> 1, kv = blockIdx.z & 1, head = blockIdx.y;
-  const int start = p.starts[entry];
+// One block per (page that an entry touches, kv head, entry, K or V), heads next to each other, as their rows lie in memory:
+// 256 threads, thread = (row group, 8 channels); the page's new tokens stay in registers between the search for the largest
+// value and the conversion, so HBM sees one read and one half-size write.  Tokens that the page holds already are read only
+// when its scale grows.  What a block has to look up is asked for as early as its address is known - entry; length, page and
+// new tokens; references and scale - because for one token these three trips to memory are the whole time.
+// kSlots: new tokens of a page that a thread takes, 16 apart (1 when a call has at most 16 per entry: half the registers,
+// so that all blocks of a batch are resident at once).
+template <int kSlots>
+__global__ void __launch_bounds__(256) paged_append_kernel(const PagedView c, const AppendParams p, int page_shift, int* status) {
+  const int entry = blockIdx.y >> 1;
+  const bool kv = blockIdx.y & 1;
+  const int nth = blockIdx.x / c.n_kv_heads, head = blockIdx.x - nth * c.n_kv_heads;
+  const int start = p.starts[entry], seq = p.seqs[entry];
   const int row0 = p.cu ? p.cu[entry] : entry;
   const int count = p.cu ? p.cu[entry + 1] - row0 : 1;
   if (start < 0 || count == 0) return;
-  const int P = c.page_tokens;
-  const int first = start / P, slot = first + blockIdx.x;
-  if (slot > (start + (int64_t)count - 1) / P && blockIdx.x > 0) return;
-  const int seq = p.seqs[entry];
-  const int len = seq >= 0 && seq < c.max_seqs ? c.lens[seq] : -1;
-  bool bad = count < 0 || count > p.max_new || row0 < 0 || (int64_t)row0 + count > p.total || (int64_t)start + count > len ||
-             len > (int64_t)c.per_row * P;
-  int page = -1;
-  if (!bad) {
-    page = c.table[(int64_t)seq * c.per_row + slot];
-    bad = page < 0 || page >= c.n_pages || c.refs[page] != 1;
-  }
-  if (bad) {
-    if (threadIdx.x == 0) *status = MAGI_E_RANGE;
-    return;
-  }
-  const int base = slot * P;                          // position of the page's first token
+  const int P = c.page_tokens, slot = (start >> page_shift) + nth;
+  if (nth > 0 && slot > (start + (int64_t)count - 1) >> page_shift) return;
+  bool bad = count < 0 || count > p.max_new || row0 < 0 || (int64_t)row0 + count > p.total || seq < 0 || seq >= c.max_seqs ||
+             slot >= c.per_row;
+  const int len = bad ? -1 : c.lens[seq];
+  const int page = bad ? -1 : c.table[(int64_t)seq * c.per_row + slot];
+  const int base = slot << page_shift;                // position of the page's first token
   const int lo = max(start, base) - base;             // new tokens: rows [lo, hi) of the page
-  const int hi = min(start + count, base + P) - base;
-  const int held = min(len - base, P);                // tokens of the sequence in the page, new ones included
-  const bool others = lo > 0 || hi < held;
-  const __nv_bfloat16* x = p.x[kv] + ((int64_t)row0 + base - start) * p.st[kv] + (int64_t)head * p.sh[kv];  // row r: x + r * st
+  const int hi = bad ? lo : (int)min((int64_t)start + count - base, (int64_t)P);
+  const int64_t st = kv ? p.st[1] : p.st[0];
+  // row r of the page: x + r * st
+  const __nv_bfloat16* x = (kv ? p.x[1] : p.x[0]) + ((int64_t)row0 + base - start) * st + (int64_t)head * (kv ? p.sh[1] : p.sh[0]);
   const int col = (threadIdx.x & 15) * 8, r0 = threadIdx.x >> 4;
-  uint4 v[8];
+  const int first = kSlots == 1 ? lo : 0;
+  uint4 v[kSlots];
+#pragma unroll
+  for (int i = 0; i < kSlots; ++i) {
+    const int r = first + r0 + i * 16;
+    v[i] = make_uint4(0, 0, 0, 0);
+    if (r >= lo && r < hi) v[i] = __ldg(reinterpret_cast<const uint4*>(x + (int64_t)r * st + col));
+  }
+  bad = bad || (int64_t)start + count > len || len > (int64_t)c.per_row << page_shift || page < 0 || page >= c.n_pages;
+  const int64_t block = ((int64_t)p.layer * c.n_pages + (bad ? 0 : page)) * c.n_kv_heads + head;
+  float* scale = (kv ? c.v_scale : c.k_scale) + block;
+  uint8_t* codes = (kv ? c.v8 : c.k8) + block * P * kHeadDim;
+  const int refs = bad ? 0 : c.refs[page];
+  const float stored = *scale;
   uint32_t top = 0;  // largest finite magnitude, as bits
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int r = r0 + i * 16;
-    v[i] = make_uint4(0, 0, 0, 0);
-    if (r >= lo && r < hi) v[i] = __ldg(reinterpret_cast<const uint4*>(x + (int64_t)r * p.st[kv] + col));
+  for (int i = 0; i < kSlots; ++i) {
     const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -450,10 +459,13 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const PagedView c, co
   __shared__ uint32_t s_top[8];
   top = __reduce_max_sync(0xffffffffu, top);
   if ((threadIdx.x & 31) == 0) s_top[threadIdx.x >> 5] = top;
-  const int64_t block = ((int64_t)p.layer * c.n_pages + page) * c.n_kv_heads + head;
-  float* scale = (kv ? c.v_scale : c.k_scale) + block;
-  uint8_t* codes = (kv ? c.v8 : c.k8) + block * P * kHeadDim;
-  const float before = others ? *scale : 0.f;
+  if (refs != 1) {  // none, or others that share it
+    if (threadIdx.x == 0) *status = MAGI_E_RANGE;
+    return;
+  }
+  const int held = min(len - base, P);                // tokens of the sequence in the page, new ones included
+  const bool others = lo > 0 || hi < held;
+  const float before = others ? stored : 0.f;
   __syncthreads();  // every thread has read the scale before one of them replaces it
 #pragma unroll
   for (int i = 0; i < 8; ++i) top = max(top, s_top[i]);
@@ -464,8 +476,8 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const PagedView c, co
   const float inv = __frcp_rn(after);
   if (threadIdx.x == 0 && after != before) *scale = after;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int r = r0 + i * 16;
+  for (int i = 0; i < kSlots; ++i) {
+    const int r = first + r0 + i * 16;
     if (r < lo || r >= hi) continue;
     const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
     float f[8];
@@ -479,17 +491,26 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const PagedView c, co
   if (others && after != before) {
     const float ratio = before * inv;
 #pragma unroll 1
-    for (int r = r0; r < held; r += 16) {
-      if (r >= lo && r < hi) continue;
-      const uint2 raw = *reinterpret_cast<const uint2*>(codes + r * kHeadDim + col);
-      const uint8_t* b = reinterpret_cast<const uint8_t*>(&raw);
-      float f[8];
+    for (int rb = r0; rb < held; rb += 64) {
+      uint2 raw[4];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const __half_raw hr = __nv_cvt_fp8_to_halfraw(b[k], __NV_E4M3);
-        f[k] = __half2float(*reinterpret_cast<const __half*>(&hr)) * ratio;
+      for (int i = 0; i < 4; ++i) {
+        const int r = rb + i * 16;
+        if (r < held && (r < lo || r >= hi)) raw[i] = *reinterpret_cast<const uint2*>(codes + r * kHeadDim + col);
       }
-      *reinterpret_cast<uint2*>(codes + r * kHeadDim + col) = pack8_e4m3(f);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = rb + i * 16;
+        if (r >= held || (r >= lo && r < hi)) continue;
+        const uint8_t* b = reinterpret_cast<const uint8_t*>(&raw[i]);
+        float f[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const __half_raw hr = __nv_cvt_fp8_to_halfraw(b[k], __NV_E4M3);
+          f[k] = __half2float(*reinterpret_cast<const __half*>(&hr)) * ratio;
+        }
+        *reinterpret_cast<uint2*>(codes + r * kHeadDim + col) = pack8_e4m3(f);
+      }
     }
   }
 }
@@ -566,9 +587,15 @@ extern "C" int magi_token_cache_append(magi_ctx* ctx, const magi_token_cache* ca
     return set_err(ctx, MAGI_E_ALIGN, "token cache append: k and v must be 16-byte aligned with strides multiples of 8 elements");
   AppendParams p = {{static_cast<const __nv_bfloat16*>(k), static_cast<const __nv_bfloat16*>(v)}, {k_stride_t, v_stride_t},
                     {k_stride_h, v_stride_h}, seqs, starts, cu_new, n, max_new, total_new, layer};
-  const int slots = (int)(((int64_t)max_new + view.page_tokens - 2) / view.page_tokens) + 1;  // pages that max_new tokens can touch
+  // pages that max_new tokens can touch, no more than a sequence can hold
+  int64_t slots = ((int64_t)max_new + view.page_tokens - 2) / view.page_tokens + 1;
+  slots = std::min<int64_t>(slots, std::min(view.per_row, view.n_pages));
+  const int shift = __builtin_ctz(view.page_tokens);
+  const dim3 grid((unsigned)(slots * view.n_kv_heads), 2 * n);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   DeviceScope dev(ctx);
-  paged_append_kernel<<<dim3(slots, view.n_kv_heads, 2 * n), 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(view, p, status_word(ctx));
+  if (max_new <= 16) paged_append_kernel<1><<<grid, 256, 0, st>>>(view, p, shift, status_word(ctx));
+  else paged_append_kernel<8><<<grid, 256, 0, st>>>(view, p, shift, status_word(ctx));
   return launched(ctx, "token cache append");
 }
 

@@ -1,7 +1,7 @@
 // Rotary embedding by position, both channel layouts, on the first rot_dim channels of a head, forward and transposed:
 //     (a, b) -> mscale * (a cos - b sin, b cos + a sin),  angle = positions[t] * inv_freq[i]
 // Memory-bound: each element is read once and written once in 16-byte pieces.  A block takes a group of tokens, forms the
-// group's cosines and sines once in shared memory (64-bit product, reduced to a fraction of a turn before it becomes fp32:
+// group's cosines and sines once in shared memory, while its first channels are on their way (64-bit product, reduced to a fraction of a turn before it becomes fp32:
 // at position 10^6 a 32-bit product alone would be 0.03 radians off) and applies them to every head.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -12,6 +12,7 @@ namespace magi {
 
 constexpr int kRotThreads = 256;
 constexpr int kRotAngles = 2048;  // angles a block holds: 16 KB
+constexpr int kRotBatch = 4;      // 16-byte pieces that a thread has in flight
 
 struct RotaryKernelParams {
   const void* x;
@@ -56,59 +57,78 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotaryKernelP
   __shared__ float2 cs[kRotAngles];
   const int t0 = blockIdx.x * p.group;
   const int nt = min(p.group, p.T - t0);
+  constexpr int kStep = kInterleaved && V == 1 ? 2 : V;  // channels that a rotated unit covers in its first part
+  constexpr bool kPair = V == 1 || !kInterleaved;        // a rotated unit has two pieces
+  constexpr int kBatch = kPair ? kRotBatch / 2 : kRotBatch;
+  const int rot_units = kInterleaved ? 2 * p.half / kStep : p.half / kStep;
+  const int units = rot_units + (p.dim - 2 * p.half) / V;
+  const int h0 = blockIdx.y * p.heads_per_block, nh = min(p.heads_per_block, p.H - h0);
+  // this thread's unit (token t, head h, piece k), and the way to its next one, as the digits of kRotThreads
+  int h = threadIdx.x / units, k = threadIdx.x - h * units, t = h / nh;
+  h -= t * nh;
+  int dh = kRotThreads / units;
+  const int dk = kRotThreads - dh * units, dt = dh / nh;
+  dh -= dt * nh;
+  Piece<E, V> lo[kBatch], hi[kBatch];
+  int at_t[kBatch], at_h[kBatch], at_k[kBatch];
+  auto load = [&]() {
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      at_t[b] = t, at_h[b] = h, at_k[b] = k;
+      if (t < nt) {
+        const E* x = static_cast<const E*>(p.x) + (int64_t)(t0 + t) * p.x_st + (int64_t)(h0 + h) * p.x_sh;
+        const bool turned = k < rot_units;
+        lo[b] = *reinterpret_cast<const Piece<E, V>*>(x + (turned ? k * kStep : 2 * p.half + (k - rot_units) * V));
+        if (kPair && turned) hi[b] = *reinterpret_cast<const Piece<E, V>*>(x + (kInterleaved ? 2 * k + 1 : p.half + k * V));
+      }
+      k += dk, h += dh, t += dt;
+      if (k >= units) k -= units, ++h;
+      if (h >= nh) h -= nh, ++t;
+    }
+  };
+  load();  // in flight while the angles are formed
   for (int i = threadIdx.x; i < nt * p.half; i += kRotThreads) {
-    const int t = i / p.half, c = i - t * p.half;
-    const double pos = p.pos64 ? (double)__ldg(reinterpret_cast<const long long*>(p.positions) + t0 + t)
-                               : (double)__ldg(reinterpret_cast<const int*>(p.positions) + t0 + t);
+    const int a = i / p.half, c = i - a * p.half;
+    const double pos = p.pos64 ? (double)__ldg(reinterpret_cast<const long long*>(p.positions) + t0 + a)
+                               : (double)__ldg(reinterpret_cast<const int*>(p.positions) + t0 + a);
     const double turns = pos * (__ldg(p.inv_freq + c) * 0.15915494309189535);  // 1 / (2 pi)
     float s, co;
     sincospif(2.0f * (float)(turns - rint(turns)), &s, &co);
     cs[i] = make_float2(co * p.mscale, (p.inverse ? -s : s) * p.mscale);
   }
   __syncthreads();
-  constexpr int kStep = kInterleaved && V == 1 ? 2 : V;  // channels that a rotated unit covers in its first part
-  const int rot_units = kInterleaved ? 2 * p.half / kStep : p.half / kStep;
-  const int units = rot_units + (p.dim - 2 * p.half) / V;
-  const int h0 = blockIdx.y * p.heads_per_block, nh = min(p.heads_per_block, p.H - h0);
-  const int total = nt * nh * units;
-  for (int u = threadIdx.x; u < total; u += kRotThreads) {
-    const int th = u / units, k = u - th * units;
-    const int t = th / nh, h = h0 + th - t * nh;
-    const E* x = static_cast<const E*>(p.x) + (int64_t)(t0 + t) * p.x_st + (int64_t)h * p.x_sh;
-    E* o = static_cast<E*>(p.out) + (int64_t)(t0 + t) * p.o_st + (int64_t)h * p.o_sh;
-    const float2* a = cs + t * p.half;
-    if (k >= rot_units) {
-      const int c = 2 * p.half + (k - rot_units) * V;
-      *reinterpret_cast<Piece<E, V>*>(o + c) = *reinterpret_cast<const Piece<E, V>*>(x + c);
-    } else if constexpr (!kInterleaved) {
-      const int c = k * V;
-      Piece<E, V> lo = *reinterpret_cast<const Piece<E, V>*>(x + c), hi = *reinterpret_cast<const Piece<E, V>*>(x + p.half + c);
+  while (true) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float2 r = a[c + i];
-        const float l = to_f(lo.v[i]), g = to_f(hi.v[i]);
-        lo.v[i] = from_f<E>(l * r.x - g * r.y);
-        hi.v[i] = from_f<E>(g * r.x + l * r.y);
-      }
-      *reinterpret_cast<Piece<E, V>*>(o + c) = lo;
-      *reinterpret_cast<Piece<E, V>*>(o + p.half + c) = hi;
-    } else if constexpr (V == 1) {
-      const float2 r = a[k];
-      const float l = to_f(x[2 * k]), g = to_f(x[2 * k + 1]);
-      o[2 * k] = from_f<E>(l * r.x - g * r.y);
-      o[2 * k + 1] = from_f<E>(g * r.x + l * r.y);
-    } else {
-      const int c = k * V;
-      Piece<E, V> w = *reinterpret_cast<const Piece<E, V>*>(x + c);
+    for (int b = 0; b < kBatch; ++b) {
+      if (at_t[b] >= nt) continue;
+      E* o = static_cast<E*>(p.out) + (int64_t)(t0 + at_t[b]) * p.o_st + (int64_t)(h0 + at_h[b]) * p.o_sh;
+      const float2* a = cs + at_t[b] * p.half;
+      const int u = at_k[b];
+      if (u >= rot_units) {
+        *reinterpret_cast<Piece<E, V>*>(o + 2 * p.half + (u - rot_units) * V) = lo[b];
+      } else if constexpr (kPair) {
 #pragma unroll
-      for (int i = 0; i < V; i += 2) {
-        const float2 r = a[(c + i) / 2];
-        const float l = to_f(w.v[i]), g = to_f(w.v[i + 1]);
-        w.v[i] = from_f<E>(l * r.x - g * r.y);
-        w.v[i + 1] = from_f<E>(g * r.x + l * r.y);
+        for (int i = 0; i < V; ++i) {
+          const float2 r = a[u * V + i];
+          const float l = to_f(lo[b].v[i]), g = to_f(hi[b].v[i]);
+          lo[b].v[i] = from_f<E>(l * r.x - g * r.y);
+          hi[b].v[i] = from_f<E>(g * r.x + l * r.y);
+        }
+        *reinterpret_cast<Piece<E, V>*>(o + u * kStep) = lo[b];
+        *reinterpret_cast<Piece<E, V>*>(o + (kInterleaved ? 2 * u + 1 : p.half + u * V)) = hi[b];
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; i += 2) {
+          const float2 r = a[(u * V + i) / 2];
+          const float l = to_f(lo[b].v[i]), g = to_f(lo[b].v[i + 1]);
+          lo[b].v[i] = from_f<E>(l * r.x - g * r.y);
+          lo[b].v[i + 1] = from_f<E>(g * r.x + l * r.y);
+        }
+        *reinterpret_cast<Piece<E, V>*>(o + u * V) = lo[b];
       }
-      *reinterpret_cast<Piece<E, V>*>(o + c) = w;
     }
+    if (t >= nt) return;
+    load();
   }
 }
 
