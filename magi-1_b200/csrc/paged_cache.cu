@@ -410,7 +410,7 @@ __device__ __forceinline__ uint2 pack8_e4m3(const float* f) {
 // kSlots: new tokens of a page that a thread takes, 16 apart (1 when a call has at most 16 per entry: half the registers,
 // so that all blocks of a batch are resident at once).
 template <int kSlots>
-__global__ void __launch_bounds__(256) paged_append_kernel(const PagedView c, const AppendParams p, int page_shift, int* status) {
+__global__ void __launch_bounds__(256, 5) paged_append_kernel(const PagedView c, const AppendParams p, int page_shift, int* status) {
   const int entry = blockIdx.y >> 1;
   const bool kv = blockIdx.y & 1;
   const int nth = blockIdx.x / c.n_kv_heads, head = blockIdx.x - nth * c.n_kv_heads;
