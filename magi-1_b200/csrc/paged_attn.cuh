@@ -59,10 +59,11 @@ inline void set_group(PagedAttnKernelParams* p, int group) {
 
 // What a block leaves behind about its last unit, when others continue it.
 struct PaHeader {
-  int open;        // 1: the unit starts in this block and ends in block `last`
-  int b, h, j;     // entry, kv head, row tile
+  int open;         // 1: the unit starts in this block and ends in block `last`
   int last;
-  int pad[3];
+  int row0, h;      // of its entry, its kv head
+  int first, rows;  // its flattened rows
+  int pad[2];
 };
 
 // One entry of the call as the kernels see it; rows and lengths that make no sense count as none.

@@ -495,7 +495,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
         for (int r = 0; r < RG; ++r)
           if (r < rows) part[r * kHeadDim + key] = o[r];
         if (wq == 0 && lane < RG) p.stats[slot * R + row] = make_float2(m, total);
-        if (first == 0 && sw == 0 && lane == 0) p.headers[blockIdx.x] = {1, walk.b, h, walk.j, walk.last_block(st.per_block), {0, 0, 0}};
+        if (first == 0 && sw == 0 && lane == 0) p.headers[blockIdx.x] = {1, walk.last_block(st.per_block), ent.row0, h, unit.first, unit.rows, {0, 0}};
       }
       ++units;
     }
@@ -519,15 +519,11 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const PaHeader hd = p.headers[blockIdx.x];
   if (!hd.open) return;
-  bool bad;
-  const PaEntry e = load_entry(p, hd.b, &bad);
-  PaUnit u;
-  unit_tiles<R>(p, e, hd.j, &u);
   __shared__ float s_sum[8];
   __shared__ float4 s_acc[8][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r = kWide ? blockIdx.y : blockIdx.y * 8 + warp;
-  if (r >= u.rows) return;
+  if (r >= hd.rows) return;
   const int n_parts = hd.last - blockIdx.x + 1;
   auto slot = [&](int k) { return (k == 0 ? 2 * (int64_t)blockIdx.x + 1 : 2 * (int64_t)(blockIdx.x + k)) * R + r; };
   float top = -INFINITY;  // every warp looks at all maxima of its row
@@ -566,11 +562,11 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
     }
   }
   const float inv = sum != 0.f ? 1.0f / sum : 0.f;
-  const int flat = u.first + r, tok = by_group(p, flat), head = hd.h * p.group + flat - tok * p.group;
-  *reinterpret_cast<uint2*>(p.out + (int64_t)(e.row0 + tok) * p.o_st + (int64_t)head * p.o_sh + lane * 4) =
+  const int flat = hd.first + r, tok = by_group(p, flat), head = hd.h * p.group + flat - tok * p.group;
+  *reinterpret_cast<uint2*>(p.out + (int64_t)(hd.row0 + tok) * p.o_st + (int64_t)head * p.o_sh + lane * 4) =
       make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
   if (p.lse && lane == 0)
-    p.lse[(int64_t)(e.row0 + tok) * p.hq + head] = sum != 0.f ? (top - kPaShift + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+    p.lse[(int64_t)(hd.row0 + tok) * p.hq + head] = sum != 0.f ? (top - kPaShift + log2f(sum)) * 0.6931471805599453f : -INFINITY;
 }
 
 // ---------------------------------------------------------------------------------------------- host side

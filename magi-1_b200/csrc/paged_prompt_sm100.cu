@@ -452,7 +452,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
           p.lse[(int64_t)(ent.row0 + tok) * p.hq + head] = total != 0.f ? (m - kPaShift + log2f(total)) * 0.6931471805599453f : -INFINITY;
       }
       if (!whole && first == 0 && threadIdx.x == 128)
-        p.headers[blockIdx.x] = {1, walk.b, walk.h, walk.j, walk.last_block(st.per_block), {0, 0, 0}};
+        p.headers[blockIdx.x] = {1, walk.last_block(st.per_block), ent.row0, walk.h, unit.first, unit.rows, {0, 0}};
       __syncwarp();
     }
   }
