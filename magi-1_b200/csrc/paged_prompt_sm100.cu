@@ -261,37 +261,51 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
           }
         };
         // At the borders: columns that no row of this warp sees are left out, those that all rows see are like any other.
-        const int all_last = __reduce_min_sync(0xffffffffu, last), all_begin = __reduce_max_sync(0xffffffffu, begin);
-        const int any_last = __reduce_max_sync(0xffffffffu, last), any_begin = __reduce_min_sync(0xffffffffu, begin);
+        int all_last = 0, all_begin = 0, any_last = 0, any_begin = 0;
+        if (border) {
+          all_last = __reduce_min_sync(0xffffffffu, last), all_begin = __reduce_max_sync(0xffffffffu, begin);
+          any_last = __reduce_max_sync(0xffffffffu, last), any_begin = __reduce_min_sync(0xffffffffu, begin);
+        }
         auto hidden = [&](int at) { return at > any_last || at + 31 < any_begin; };
         auto mixed = [&](int at) { return at + 31 > all_last || at < all_begin; };
-        float t0 = -INFINITY, t1 = -INFINITY;
-        auto find_top = [&](int at) {
-          float s[32], kc[kPer], bias[kPer], inv[kPer];
-          tmem_ld32(t_s + at, reinterpret_cast<uint32_t*>(s));
-          factors(at, kc, bias, inv);
-          tmem_wait_ld();
-#pragma unroll
-          for (int c = 0; c < 32; ++c) s[c] = fmaf(s[c], kc[c / kGroup], bias[c / kGroup]);
+        float top = -INFINITY;
+        // The largest exponent of 32 keys.  It belongs to the largest score of a page, as kc is not negative.
+        auto find_top = [&](int at, float (&s)[32]) {
           if (border && mixed(at)) {
 #pragma unroll
             for (int c = 0; c < 32; ++c) s[c] = at + c <= last && at + c >= begin ? s[c] : -INFINITY;
           }
+          float kc[kPer], bias[kPer], inv[kPer];
+          factors(at, kc, bias, inv);
 #pragma unroll
-          for (int c = 0; c < 32; c += 4) {
-            t0 = max3(t0, s[c], s[c + 1]);
-            t1 = max3(t1, s[c + 2], s[c + 3]);
+          for (int g = 0; g < kPer; ++g) {
+            float t0 = fmaxf(s[g * kGroup], s[g * kGroup + 1]), t1 = fmaxf(s[g * kGroup + 2], s[g * kGroup + 3]);
+#pragma unroll
+            for (int c = g * kGroup + 4; c < (g + 1) * kGroup; c += 4) {
+              t0 = max3(t0, s[c], s[c + 1]);
+              t1 = max3(t1, s[c + 2], s[c + 3]);
+            }
+            t0 = fmaxf(t0, t1);
+            top = fmaxf(top, t0 == -INFINITY ? t0 : fmaf(t0, kc[g], bias[g]));
           }
         };
         if (!border) {
-          find_top(half * 64);
-          find_top(half * 64 + 32);
+          float s0[32], s1[32];
+          tmem_ld32(t_s + half * 64, reinterpret_cast<uint32_t*>(s0));
+          tmem_ld32(t_s + half * 64 + 32, reinterpret_cast<uint32_t*>(s1));
+          tmem_wait_ld();
+          find_top(half * 64, s0);
+          find_top(half * 64 + 32, s1);
         } else {
 #pragma unroll 1
           for (int at = half * 64; at < half * 64 + 64; at += 32)
-            if (!hidden(at)) find_top(at);
+            if (!hidden(at)) {
+              float s[32];
+              tmem_ld32(t_s + at, reinterpret_cast<uint32_t*>(s));
+              tmem_wait_ld();
+              find_top(at, s);
+            }
         }
-        float top = fmaxf(t0, t1);
         top_mine[(seen & 1) * 512] = top;
         pair_sync(x);
         top = fmaxf(top, top_other[(seen & 1) * 512]);
