@@ -66,7 +66,8 @@ def _one_place_each(t: torch.Tensor, name: str) -> None:
 class TokenPagedKVCache:
     """Pages of page_tokens tokens, e4m3 codes with a power-of-two scale per (page, kv head), K and V separate.
 
-    Device state, all of it plain tensors that may be read (and saved and put back, e.g. to rewind) at any time:
+    Device state, all of it plain tensors that may be read at any time (and saved and put back with copy_, all three books
+    together, e.g. to rewind):
       k8, v8 [n_layers, n_pages, n_kv_heads, page_tokens, 128] float8_e4m3fn; k_scale, v_scale [n_layers, n_pages, n_kv_heads]
       page_table [max_seqs, max_pages_per_seq] int32 (-1 = none); seq_lens [max_seqs] int32; page_refs [n_pages] int32
     A page id names the same page in every layer.  The index arguments of the methods are int32 tensors on the cache's
@@ -208,6 +209,8 @@ def paged_attn(q: torch.Tensor, cache: TokenPagedKVCache, layer: int, seqs: torc
     layer, window, max_q = int(layer), int(window), int(max_q)
     if not 0 <= window <= _INT32_MAX or not 0 <= max_q <= _INT32_MAX:
         raise ValueError("window and max_q must be non-negative 32-bit numbers")
+    if softmax_scale is not None and not 0.0 < softmax_scale < math.inf:
+        raise ValueError("softmax_scale must be a positive number")
     raw = _on(stream, dev)
     rows, heads, _ = shape = q.shape
     stride_t, stride_h, _ = q.stride()

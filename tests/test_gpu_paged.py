@@ -169,6 +169,59 @@ def test_nan_and_infinite_queries_stay_in_their_rows():
     assert torch.equal(out[~bad], clean[~bad])
 
 
+@pytest.mark.parametrize("n_q,window", [(2, 0), (2, 20), (5, 0), (5, 9), (40, 0), (40, 30)])
+def test_nan_values_reach_only_the_rows_that_see_them(n_q, window):
+    """In every form (12, 30 and 240 rows of the kv head), with NaN codes on both sides of what the rows see."""
+    n = 300
+    c = make_cache([n], 32, 1, seed=n_q)
+    ids = c.page_table[0].long()
+    spots = [(n - 1, 3), (n - 2, 64), (n - 1, 127), (n - n_q - 15, 70), (n - n_q, 31), (n - 130, 9)]  # (position, channel)
+    for at, ch in spots:
+        c.v8.view(torch.uint8)[0, int(ids[at // 32]), 0, at % 32, ch] = 0xff if ch & 1 else 0x7f
+    o = check_attn(c, strided_bf16(n_q, 6, 17), [0], [0, n_q], window=window)
+    for at, ch in spots:
+        for t in range(n_q):
+            pos = n - n_q + t
+            assert np.isnan(o[t, :, ch]).all() == (at <= pos and (window == 0 or at > pos - window)), (at, ch, t)
+
+
+# More units than blocks, so that every block begins and ends several; short ones, whose tiles are all at a border.
+@pytest.mark.parametrize("n,hq,hkv,q_hi,len_hi,window", [(900, 8, 2, 1, 300, 0), (900, 8, 2, 1, 300, 40), (700, 12, 2, 5, 400, 0), (700, 12, 2, 5, 400, 130),
+                                                         (260, 6, 1, 300, 420, 0), (260, 6, 1, 300, 420, 150), (150, 21, 3, 70, 200, 3)])
+def test_many_short_units(n, hq, hkv, q_hi, len_hi, window):
+    rng = np.random.RandomState(n + window)
+    lens = rng.randint(0, len_hi + 1, n).tolist()
+    n_q = [1] * n if q_hi == 1 else rng.randint(0, q_hi + 1, n).tolist()
+    c = make_cache(lens, 64 if window else 16, hkv, seed=n)
+    cu = np.concatenate([[0], np.cumsum(n_q)]).tolist()
+    check_attn(c, strided_bf16(cu[-1], hq, 19), rng.permutation(n).tolist(), cu, window=window)
+
+
+@pytest.mark.parametrize("hq,hkv,n_q", [(21, 3, 2), (21, 3, 4), (21, 3, 60), (5, 1, 6), (13, 1, 11), (31, 1, 1), (31, 1, 9), (33, 1, 1), (257, 1, 3)])
+def test_groups_that_are_no_power_of_two(hq, hkv, n_q):
+    c = make_cache([n_q + 150, n_q], 32, hkv, seed=hq)
+    check_attn(c, strided_bf16(2 * n_q, hq, 23), [0, 1], [0, n_q, 2 * n_q])
+
+
+def test_scores_that_grow_from_tile_to_tile():
+    """Every tile asks for a new reference, by less and by more than what a weight has room for."""
+    for step in (0.5, 2.0, 3.9, 9.0, 40.0):
+        n = 1500
+        c = make_cache([n], 64, 1, seed=31)
+        ids = c.page_table[0].long()
+        c.k8.view(torch.uint8).zero_()
+        c.k_scale.fill_(2.0 ** -20)
+        for page, i in enumerate(ids[:-(-n // 64)].tolist()):
+            c.k8.view(torch.uint8)[0, i, 0, :, 0] = 0x38          # 1.0 in channel 0, times the page's scale
+            c.k8.view(torch.uint8)[0, i, 0, :, 1] = (torch.arange(64, device="cuda") % 8 + 0x30).to(torch.uint8)
+            c.k_scale[0, i, 0] = 2.0 ** (page // 2 - 6)           # doubles from tile to tile
+        q = torch.zeros(40, 6, 128, dtype=torch.bfloat16, device="cuda")
+        q[:, :, 0] = step
+        q[:, :, 1] = torch.linspace(-1, 1, 40, device="cuda").to(torch.bfloat16)[:, None]
+        for m in (1, 5, 40):
+            check_attn(c, q[:m], [0], [0, m])
+
+
 def test_queries_of_any_size():
     c = make_cache([150], 64, 1, seed=9)
     q = strided_bf16(6, 6, 14) * torch.tensor([1e-30, 0.0, 1e-3, 30.0, 1.0, 1e-38], device="cuda")[:, None, None].to(torch.bfloat16)
@@ -570,3 +623,11 @@ def test_a_long_tail_behind_one_large_weight():
         # every small weight is the same number and rounds the same way, by at most 2^-3 of it (e5m2): the bound of the result
         assert abs(float(out.double().mean()) - want) <= (2.0 ** -8 + 2.0 ** -3) * want
         assert abs(float(lse[0, 0]) - math.log(n - 1 + big)) <= 1e-4
+
+
+def test_a_scale_that_is_no_positive_number_is_refused():
+    import magi_b200 as mb
+    c = make_cache([10], 16, 2, seed=1)
+    for scale in (0.0, -1.0, math.nan, math.inf):
+        with pytest.raises(ValueError):
+            mb.paged_attn(strided_bf16(1, 4, 1), c, 0, i32([0]), softmax_scale=scale)
