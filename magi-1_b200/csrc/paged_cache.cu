@@ -445,17 +445,27 @@ __global__ void __launch_bounds__(256, 5) paged_append_kernel(const PagedView c,
   uint8_t* codes = (kv ? c.v8 : c.k8) + block * P * kHeadDim;
   const int refs = bad ? 0 : c.refs[page];
   const float stored = *scale;
-  uint32_t top = 0;  // largest finite magnitude, as bits
+  // largest finite magnitude, as bits: two at a time, and one by one only where some are not finite
+  uint32_t tops = 0;
 #pragma unroll
-  for (int i = 0; i < kSlots; ++i) {
-    const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+  for (int i = 0; i < kSlots; ++i)
+    tops = __vmaxu2(__vmaxu2(__vmaxu2(tops, v[i].x & 0x7fff7fffu), v[i].y & 0x7fff7fffu),
+                    __vmaxu2(v[i].z & 0x7fff7fffu, v[i].w & 0x7fff7fffu));
+  uint32_t top = max(tops & 0xffffu, tops >> 16);
+  if (top >= 0x7f80u) {
+    top = 0;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const uint32_t a = w[k] & 0x7fffu, b = w[k] >> 16 & 0x7fffu;
-      if (a < 0x7f80u) top = max(top, a);
-      if (b < 0x7f80u) top = max(top, b);
+    for (int i = 0; i < kSlots; ++i) {
+      const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t a = w[k] & 0x7fffu, b = w[k] >> 16 & 0x7fffu;
+        if (a < 0x7f80u) top = max(top, a);
+        if (b < 0x7f80u) top = max(top, b);
+      }
     }
   }
+  __syncwarp();
   __shared__ uint32_t s_top[8];
   top = __reduce_max_sync(0xffffffffu, top);
   if ((threadIdx.x & 31) == 0) s_top[threadIdx.x >> 5] = top;
