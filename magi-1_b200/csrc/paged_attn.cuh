@@ -16,8 +16,8 @@ constexpr int kPaTileBytes = kPaTile * kHeadDim;
 constexpr int kPromptRows = 256;               // query rows of a block in the prompt form
 constexpr int kPaNear = 64;                    // entries whose lengths a block keeps in shared memory
 // P = 2^(w - reference + 5).  The reference of a row is the exact maximum when it is set and stays while no weight exceeds
-// e4m3's 448 = 2^8.8, that is until the maximum has grown 14-fold: nearly every tile then needs one vote of the group in
-// place of its maxima, and the tensor core goes on summing in TMEM.  The residual term is e5m2, whose smallest step is 2^-16:
+// e4m3's 448 = 2^8.8, that is until the maximum has grown 14-fold: in nearly every tile the tensor core goes on summing in
+// TMEM, and the few-row form needs one vote of the group in place of the maxima.  The residual term is e5m2, whose smallest step is 2^-16:
 // a weight is dropped only below 2^-22 of the reference, so a long tail of small weights behind one large one keeps its mass.
 constexpr float kPaShift = 5.0f, kPaLimit = 8.8f;
 

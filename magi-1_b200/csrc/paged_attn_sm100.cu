@@ -5,15 +5,15 @@
 // The scores are formed TRANSPOSED, S^T [128 keys x R rows] = K8 Q^T and O^T [128 channels x R rows] = V8^T P^T, so that
 // the long side of every product is the cache: the e4m3 tiles go from HBM through TMA and shared memory to tcgen05.mma
 // (kind::f8f6f4, M = 128) exactly as they are stored, nothing is ever converted to a wider type, and a tile costs the same
-// few instructions whether a sequence has one new token (R = 16 covers 16 query heads of a kv head) or many.  K8 is the
-// K-major A operand of the first product, V8 - stored [key][channel] - the MN-major A operand of the second.
+// few instructions whether a sequence has one new token (R = 16 covers 16 query heads of a kv head) or several (R = 32).  K8
+// is the K-major A operand of the first product, V8 - stored [key][channel] - the MN-major A operand of the second.
 //
-// Precision: Q and P are carried as two e4m3 terms each (value + rounding residual; two instructions that accumulate into
-// the same columns).  bf16 has 8 significant bits and two e4m3 terms hold 8, so Q loses nothing except what lies 2^-17
-// below its row's largest entry; P is rounded to 2^-8 of each weight, like the bf16 result.  Sums, maxima and the output
-// accumulator are fp32 in registers.  The V scale is folded into the exponent, w = s log2e + log2(sv), and the running
-// maximum is taken over w: then every P is at most 1 however different the pages' scales are, O needs no scale per page
-// and the denominator adds P / sv.
+// Precision: Q and P are carried as two terms each (value + rounding residual; two instructions that accumulate into the
+// same columns).  bf16 has 8 significant bits and two e4m3 terms hold 8, so Q loses nothing except what lies 2^-17 below
+// its row's largest entry; P is e4m3 and an e5m2 residual, off by at most 2^-4 of 2^-3 of a weight (e5m2 for its range: see
+// kPaShift).  Sums and maxima are fp32 in registers, the output accumulator fp32 in TMEM.  The V scale is folded into the
+// exponent, w = s log2e + log2(sv), and a row's reference is taken over w: then P stays within e4m3 however different the
+// pages' scales are, O needs no scale per page and the denominator adds P / sv.
 //
 // Work: the 128-key tiles of all (sequence, kv head, row tile) units in a row are dealt out to the blocks in equal
 // contiguous parts, so a long sequence is split over many blocks and ragged batches balance; the lengths are read on the
@@ -21,9 +21,15 @@
 // and accumulator in the workspace, and a second kernel joins them in the order of the keys (no atomics: the same bits
 // every time).
 //
+// What bounds it: HBM, once the batch fills the machine (8 sequences of 10^5 tokens, 1.9 GB: 292 us, the copy rate; 64 of
+// 300 to 8191: 98 us, of which 7 pass until the first tile is in and 3 in the join), else the latencies of one tile: plan 2 us,
+// first tile 2, softmax and output 2, join 2.  Two blocks per SM with five stages of 16 KB: one's softmax hides behind the
+// other's loads (three with three stages: 121 us for the batch, against 108 then).
+//
 //   warp 0     TMA: pages of K and V into a ring of 16 KB tiles, their scales by cp.async beside them
 //   warp 1     UMMA issuer (one thread)
-//   warps 2+   G groups of four: thread = key of S^T, then channel of O^T; a group takes RG of the R rows
+//   warps 2+   R / 16 groups of four: thread = key of S^T, then channel of O^T; a group takes 16 of the R rows (32 rows in one
+//              group: 21 us against 16.5 for 16 sequences of 2 to 5 tokens with a window of 4099)
 // Every wait is bounded (MAGI_E_TIMEOUT).
 #include "paged_attn.cuh"
 
@@ -37,7 +43,8 @@ struct PaShared {
   static constexpr int kStages = R == 16 ? 5 : 4;
   static constexpr int kBlocksPerSm = 2;
   static constexpr int kSlots = 8;                             // tiles whose page scales are kept
-  static constexpr int kCost = 4;                              // beginning and ending a unit, in tiles
+  // beginning and ending a unit, in tiles (64 sequences of 300 to 8191: 121 us at 1, 112 at 2, 108 at 4, 110 at 6)
+  static constexpr int kCost = 4;
   static constexpr int kGroups = R / 16;                       // of four softmax warps, 16 rows each
   static constexpr int kThreads = 64 + 128 * kGroups;
   static constexpr int kRing = 0;

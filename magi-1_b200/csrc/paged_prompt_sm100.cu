@@ -2,14 +2,21 @@
 //
 // Same products, precision and work split as the few-row form (paged_attn_sm100.cu), with the rows across: S [128 rows x 128
 // keys] = Q K8^T and O [128 rows x 128 channels] = P V8, a thread owning a row.  Maximum, reference and sum of a row then live
-// in its thread, no vote or barrier is needed between tiles, and the fixed cost of a tile (barriers, tensor memory latency) is
-// spread over 128 elements of each thread instead of 32.
+// in its thread, and the fixed cost of a tile (barriers, tensor memory latency) is spread over 64 elements of each thread.
 //
 // A block works on 256 rows (query tokens times the heads of a kv head, flattened), two tiles of 128 that take turns on the
 // tensor core.  K and V tiles are read once for all 256 rows.  Two warpgroups share a row tile, 64 keys each (and 64 channels of
 // the result): with one, the latencies of its conversions lay open, 7000 cycles a tile.  They exchange the row maxima through
 // shared memory, one barrier a tile.  P goes back over S in TMEM (32 keys: 8 columns of e4m3, 8 of the e5m2 residual) and is the
 // A operand of the second product from there.
+//
+// What bounds it: issue slots (58 % busy; 13.4 instructions per weight, 6.1 of them the product, the exponential, the sum and
+// the two conversions) and the latency of tensor memory between them; the tensor pipe is busy 35 %.  428 GFLOP over ragged
+// prompts 629 us, 476 GFLOP over one of 9001 tokens 649 us (734 TFLOP/s, at the power limit).  A tile's weights against the
+// reference as it stands, checked afterwards, would save the pass for the maximum, but one of 128 rows asks for a new reference
+// in most tiles: 926 us.  A unit costs about five tiles to begin and end (ragged prompts: 739 us counted as 3 tiles and with the
+// queries split 16 rows at a time, 674 at 4, 669 at 5, 677 at 6).
+//
 //   warp 0 TMA, warp 1 UMMA issuer, warps 2, 3 idle, warps 4-19 softmax (warpgroup 2 x + half: row tile x, keys 64 half ..)
 //   TMEM columns: S of row tile 0, 1 at 0, 128; O at 256, 384
 #include <type_traits>
@@ -23,7 +30,7 @@ int launch_prompt_join(magi_ctx* ctx, const PagedAttnKernelParams& k, cudaStream
 struct PromptShared {
   static constexpr int kStages = 8;
   static constexpr int kSlots = 8;                             // tiles whose page scales are kept
-  static constexpr int kCost = 5;                              // beginning and ending a unit, in tiles
+  static constexpr int kCost = 5;                              // beginning and ending a unit, in tiles (see above)
   static constexpr int kThreads = 640;
   static constexpr int kRing = 0;
   static constexpr int kQ = kRing + kStages * kPaTileBytes;    // [2 terms][2 warpgroups][128 rows][128 bytes]
