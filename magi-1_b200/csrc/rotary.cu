@@ -1,10 +1,11 @@
 // Rotary embedding by position, both channel layouts, on the first rot_dim channels of a head, forward and transposed:
 //     (a, b) -> mscale * (a cos - b sin, b cos + a sin),  angle = positions[t] * inv_freq[i]
 // Memory-bound: each element is read once and written once in 16-byte pieces.  A block takes a group of tokens, forms the
-// group's cosines and sines once in shared memory, while its first channels are on their way (64-bit product, reduced to a fraction of a turn before it becomes fp32:
-// at position 10^6 a 32-bit product alone would be 0.03 radians off) and applies them to every head.  What takes time beside
-// the memory is instructions: threads walk over their pieces by adding steps, without a division, and 16-bit results are
-// rounded two at a time.  21600 x 24 x 128: bf16 49 us (5.4 TB/s), fp32 86 us (6.2 TB/s).
+// group's cosines and sines once in shared memory while its first channels are on their way (64-bit product, reduced to a
+// fraction of a turn before it becomes fp32: at position 10^6 a 32-bit product alone would be 0.03 radians off) and applies
+// them to every head.  What takes time beside the memory is instructions: threads walk over their pieces by adding steps,
+// without a division, and 16-bit results are rounded two at a time.  21600 x 24 x 128: bf16 49 us (5.4 TB/s), fp32 86 us
+// (6.2 TB/s).
 #include <algorithm>
 #include <type_traits>
 

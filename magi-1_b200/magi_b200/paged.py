@@ -53,6 +53,10 @@ def _rows(t, name: str, device, heads: Optional[int] = None) -> torch.Tensor:
     return t
 
 
+def _layer(layer, cache) -> int:
+    return min(max(int(layer), -1), cache.n_layers)  # the library refuses both ends; nothing wraps on its way there
+
+
 def _one_place_each(t: torch.Tensor, name: str) -> None:
     """Refuse a result tensor in which two elements share memory (a broadcast view)."""
     span = 1
@@ -71,10 +75,10 @@ class TokenPagedKVCache:
       k8, v8 [n_layers, n_pages, n_kv_heads, page_tokens, 128] float8_e4m3fn; k_scale, v_scale [n_layers, n_pages, n_kv_heads]
       page_table [max_seqs, max_pages_per_seq] int32 (-1 = none); seq_lens [max_seqs] int32; page_refs [n_pages] int32
     A page id names the same page in every layer.  The index arguments of the methods are int32 tensors on the cache's
-    device, at most 1024 entries, no sequence twice (attention excepted).  A book-keeping call that cannot be served - an
-    index out of range, a sequence named twice or longer than its table row, too few free pages - changes nothing and
-    shows in Context.status(): E_RANGE or E_NOMEM.  Calls on one cache must be stream-ordered, except that append and
-    paged_attn of different layers may overlap."""
+    device, at most 1024 entries, no sequence twice (attention excepted); they and the books stay as they are while a call
+    that reads them runs.  A book-keeping call that cannot be served - an index out of range, a sequence named twice or longer
+    than its table row, too few free pages - changes nothing and shows in Context.status(): E_RANGE or E_NOMEM.  Calls on one
+    cache must be stream-ordered, except that append and paged_attn of different layers may overlap."""
 
     def __init__(self, n_layers: int, n_pages: int, page_tokens: int, n_kv_heads: int, max_seqs: int, max_pages_per_seq: int,
                  device=None):
@@ -148,9 +152,12 @@ class TokenPagedKVCache:
             cu_new = _index(cu_new, "cu_new", self.device, seqs.shape[0] + 1)
         elif k.shape[0] != seqs.shape[0] or max_new != 1:
             raise ValueError("without cu_new every entry has one token")
+        max_new = int(max_new)
+        if not 0 <= max_new <= _INT32_MAX:
+            raise ValueError("max_new must be a non-negative 32-bit number")
         raw = _on(stream, self.device)
-        check(lib.magi_token_cache_append(self.ctx.handle, self._view_ref, int(layer), seqs.data_ptr(), starts.data_ptr(),
-                                          cu_new.data_ptr() if cu_new is not None else None, seqs.shape[0], int(max_new), k.shape[0],
+        check(lib.magi_token_cache_append(self.ctx.handle, self._view_ref, _layer(layer, self), seqs.data_ptr(), starts.data_ptr(),
+                                          cu_new.data_ptr() if cu_new is not None else None, seqs.shape[0], max_new, k.shape[0],
                                           k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), raw),
               self.ctx.handle)
         KERNEL_LAUNCHES[0] += 1
@@ -206,7 +213,7 @@ def paged_attn(q: torch.Tensor, cache: TokenPagedKVCache, layer: int, seqs: torc
         raise ValueError("without cu_q every entry has one query row")
     if q.shape[1] % cache.n_kv_heads:
         raise ValueError("the query heads must be a multiple of the cache's kv heads")
-    layer, window, max_q = int(layer), int(window), int(max_q)
+    layer, window, max_q = _layer(layer, cache), int(window), int(max_q)
     if not 0 <= window <= _INT32_MAX or not 0 <= max_q <= _INT32_MAX:
         raise ValueError("window and max_q must be non-negative 32-bit numbers")
     if softmax_scale is not None and not 0.0 < softmax_scale < math.inf:

@@ -631,3 +631,16 @@ def test_a_scale_that_is_no_positive_number_is_refused():
     for scale in (0.0, -1.0, math.nan, math.inf):
         with pytest.raises(ValueError):
             mb.paged_attn(strided_bf16(1, 4, 1), c, 0, i32([0]), softmax_scale=scale)
+
+
+def test_numbers_beyond_32_bits_do_not_wrap():
+    import magi_b200 as mb
+    c = make_cache([10], 16, 2, seed=1)
+    q, k = strided_bf16(1, 4, 1), strided_bf16(1, 2, 2)
+    for bad in (lambda: mb.paged_attn(q, c, 2 ** 32, i32([0])), lambda: c.append(-2 ** 32, i32([0]), i32([9]), k, k)):
+        with pytest.raises(mb.MagiError):
+            bad()
+    with pytest.raises(ValueError):
+        c.append(0, i32([0]), i32([9]), k, k, i32([0, 1]), max_new=2 ** 32 + 1)
+    with pytest.raises(ValueError):
+        mb.paged_attn(q, c, 0, i32([0]), i32([0, 1]), max_q=2 ** 32 + 1)
