@@ -14,7 +14,8 @@ using namespace ptx;
 constexpr int kPaTile = 128;                   // keys of a tile
 constexpr int kPaTileBytes = kPaTile * kHeadDim;
 constexpr int kPromptRows = 256;               // query rows of a block in the prompt form
-constexpr int kPaNear = 64;                    // entries whose lengths a block keeps in shared memory
+constexpr int kPaNear = 128;                   // entries with rows that a block's part can reach, kept in shared memory
+constexpr int kPaSpread = 48;                  // see plan_tiles
 // P = 2^(w - reference + 5).  The reference of a row is the exact maximum when it is set and stays while no weight exceeds
 // e4m3's 448 = 2^8.8, that is until the maximum has grown 14-fold: in nearly every tile the tensor core goes on summing in
 // TMEM, and the few-row form needs one vote of the group in place of the maxima.  The residual term is e5m2, whose smallest step is 2^-16:
@@ -130,7 +131,8 @@ __device__ __forceinline__ int row_tiles(const PagedAttnKernelParams& p, const P
 struct PaStart {
   int64_t t0, t1;       // tiles [t0, t1)
   int64_t per_block;
-  int b, h, j, off;     // unit and tile within it
+  int h, j, off;        // unit of the first entry in `near`, and where in its weight
+  int extra;            // weight of an entry beside its units'
 };
 
 __device__ __forceinline__ void tma_load_2d(void* smem_dst, const CUtensorMap* m, uint64_t* bar, int c0, int c1) {
@@ -189,14 +191,18 @@ __device__ __forceinline__ void warp_arrive(uint64_t* bar) {
 }
 
 // Which tiles are this block's: the tiles of all units in a row, dealt out in contiguous parts of equal weight.  A unit weighs
-// its tiles and kCost more for what it takes to begin and end one, as if it had so many empty tiles in front.  Whole block; scratch
-// needs kPlanScratch bytes.  The caller puts a barrier behind it.
-constexpr int kPlanScratch = (8 + (int)sizeof(PaEntry)) * kPgMaxEntries;
+// its tiles and kCost more for what it takes to begin and end one, as if it had so many empty tiles in front.  An entry weighs
+// 1 / kPaSpread of a block's part more (nothing in small calls): with at most 1024 entries on B blocks a part then reaches no
+// more than kPaSpread + 1024 / B + 2 entries that have rows, which fit in shared memory from 14 blocks on.  So every warp of the
+// block walks over one and the same list, read once: lengths that change while the call runs spoil the result, no more.
+// Whole block; scratch needs kPlanScratch bytes.  The caller puts a barrier behind it.
+constexpr int kPlanScratch = (8 + 4 + (int)sizeof(PaEntry)) * kPgMaxEntries;
 template <int R, int kThreads, int kCost>
 __device__ __forceinline__ void plan_tiles(const PagedAttnKernelParams& p, uint8_t* scratch, PaStart* start, PaEntry* near) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hkv = p.c.n_kv_heads;
   int64_t* sums = reinterpret_cast<int64_t*>(scratch);  // [n] tiles of an entry, then their prefix sums
   PaEntry* entries = reinterpret_cast<PaEntry*>(scratch + 8 * kPgMaxEntries);
+  int* counts = reinterpret_cast<int*>(entries + kPgMaxEntries);  // [n] entries with rows up to here
   const bool single = (int64_t)p.max_q * p.group <= R;                   // one row tile per entry
   bool any_bad = false;
   for (int b = threadIdx.x; b < p.n; b += kThreads) {
@@ -222,59 +228,76 @@ __device__ __forceinline__ void plan_tiles(const PagedAttnKernelParams& p, uint8
   }
   if (warp == 0) {
     int64_t carry = 0;
+    int count = 0;
     for (int b0 = 0; b0 < p.n; b0 += 32) {
       int64_t x = b0 + lane < p.n ? sums[b0 + lane] : 0;
+      const uint32_t rows = __ballot_sync(0xffffffffu, x > 0);
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
         const int64_t y = __shfl_up_sync(0xffffffffu, x, d);
         if (lane >= d) x += y;
       }
-      if (b0 + lane < p.n) sums[b0 + lane] = carry + x;
+      if (b0 + lane < p.n) {
+        sums[b0 + lane] = carry + x;
+        counts[b0 + lane] = count + __popc(rows & (0xffffffffu >> (31 - lane)));
+      }
       carry += __shfl_sync(0xffffffffu, x, 31);
+      count += __popc(rows);
     }
     __syncwarp();
-    const int64_t total = carry;
+    const int64_t extra = min(carry / ((int64_t)gridDim.x * kPaSpread), (int64_t)1 << 30);
+    auto weight_to = [&](int b) { return sums[b] + extra * counts[b]; };  // of entries 0 .. b
+    const int64_t total = carry + extra * count;
     const int64_t per_block = (total + gridDim.x - 1) / gridDim.x;
     const int64_t t0 = min((int64_t)blockIdx.x * per_block, total), t1 = min(t0 + per_block, total);
     if (t0 < t1) {
       int b = 0;  // first entry whose sum exceeds t0
       for (int b0 = 0; b0 < p.n; b0 += 32) {
-        const bool over = b0 + lane < p.n && sums[b0 + lane] > t0;
+        const bool over = b0 + lane < p.n && weight_to(b0 + lane) > t0;
         const uint32_t m = __ballot_sync(0xffffffffu, over);
         if (m) {
           b = b0 + __ffs(m) - 1;
           break;
         }
       }
-      const int64_t before = b > 0 ? sums[b - 1] : 0;
-      const int64_t per_head = (sums[b] - before) / hkv;
-      const int h = (int)((t0 - before) / per_head);
-      int64_t rem = (t0 - before) - h * per_head;
-      int j = 0;
-      if (!single) {
-        const PaEntry e = entries[b];
-        const int n_j = row_tiles<R>(p, e);
-        for (int j0 = 0; j0 < n_j; j0 += 32) {
-          const int64_t mine = j0 + lane < n_j ? unit_tiles<R>(p, e, j0 + lane, nullptr) + kCost : 0;
-          int64_t x = mine;
+      const int64_t per_head = (sums[b] - (b > 0 ? sums[b - 1] : 0)) / hkv;
+      int64_t rem = t0 - (b > 0 ? weight_to(b - 1) : 0);
+      int h = 0, j = 0;
+      if (rem >= extra) {  // else in front of the entry's first unit
+        rem -= extra;
+        h = (int)(rem / per_head);
+        rem -= h * per_head;
+        if (!single) {
+          const PaEntry e = entries[b];
+          const int n_j = row_tiles<R>(p, e);
+          for (int j0 = 0; j0 < n_j; j0 += 32) {
+            const int64_t mine = j0 + lane < n_j ? unit_tiles<R>(p, e, j0 + lane, nullptr) + kCost : 0;
+            int64_t x = mine;
 #pragma unroll
-          for (int d = 1; d < 32; d <<= 1) {
-            const int64_t y = __shfl_up_sync(0xffffffffu, x, d);
-            if (lane >= d) x += y;
+            for (int d = 1; d < 32; d <<= 1) {
+              const int64_t y = __shfl_up_sync(0xffffffffu, x, d);
+              if (lane >= d) x += y;
+            }
+            const uint32_t m = __ballot_sync(0xffffffffu, x > rem);
+            if (m) {
+              const int f = __ffs(m) - 1;
+              rem -= __shfl_sync(0xffffffffu, x - mine, f);
+              j = j0 + f;
+              break;
+            }
+            rem -= __shfl_sync(0xffffffffu, x, 31);
           }
-          const uint32_t m = __ballot_sync(0xffffffffu, x > rem);
-          if (m) {
-            const int f = __ffs(m) - 1;
-            rem -= __shfl_sync(0xffffffffu, x - mine, f);
-            j = j0 + f;
-            break;
-          }
-          rem -= __shfl_sync(0xffffffffu, x, 31);
         }
+        if (h == 0 && j == 0) rem += extra;
       }
-      for (int i = lane; i < kPaNear; i += 32)
-        if (b + i < p.n) near[i] = entries[b + i];
-      if (lane == 0) *start = {t0, t1, per_block, b, h, j, (int)rem};
+      for (int b0 = b, found = 0; b0 < p.n && found < kPaNear; b0 += 32) {
+        const bool has = b0 + lane < p.n && entries[b0 + lane].n_q > 0;
+        const uint32_t m = __ballot_sync(0xffffffffu, has);
+        const int at = found + __popc(m & ((1u << lane) - 1));
+        if (has && at < kPaNear) near[at] = entries[b0 + lane];
+        found += __popc(m);
+      }
+      if (lane == 0) *start = {t0, t1, per_block, h, j, (int)rem, (int)extra};
     } else if (lane == 0) {
       *start = {t0, t0, per_block, 0, 0, 0, 0};
     }
@@ -288,31 +311,28 @@ struct PaWalk {
   const PagedAttnKernelParams& p;
   const PaEntry* near;
   int64_t t, t1;        // weight: the segment's start, the block's end
-  int b, h, j, at;      // unit, and where in its weight the segment starts
-  int b0, n_j, weight;  // weight of the segment
+  int e, h, j, at;      // unit (its entry as a place in `near`), and where in its weight the segment starts
+  int extra, n_j, cost, weight;  // of the unit: weight in front of its tiles; weight of the segment
   int first, n_seg;     // its tiles [first, first + n_seg) of the unit's
   PaEntry ent;
   PaUnit unit;
 
   __device__ __forceinline__ PaWalk(const PagedAttnKernelParams& params, const PaStart& st, const PaEntry* entries)
-      : p(params), near(entries), t(st.t0), t1(st.t1), b(st.b), h(st.h), j(st.j), at(st.off), b0(st.b) {
+      : p(params), near(entries), t(st.t0), t1(st.t1), e(0), h(st.h), j(st.j), at(st.off), extra(st.extra) {
     if (t < t1) fetch();
   }
   __device__ __forceinline__ void fetch() {
-    if (b - b0 < kPaNear) ent = near[b - b0];
-    else {
-      bool bad;
-      ent = load_entry(p, b, &bad);
-    }
+    ent = near[e];
     n_j = row_tiles<R>(p, ent);
   }
   // The current segment; false behind the last one.
   __device__ __forceinline__ bool segment() {
     while (t < t1) {
       unit_tiles<R>(p, ent, j, &unit);
-      weight = (int)min((int64_t)(unit.tiles + kCost - at), t1 - t);
-      first = max(at - kCost, 0);
-      n_seg = max(at + weight - kCost, 0) - first;
+      cost = (h | j) == 0 ? kCost + extra : kCost;
+      weight = (int)min((int64_t)(unit.tiles + cost - at), t1 - t);
+      first = max(at - cost, 0);
+      n_seg = max(at + weight - cost, 0) - first;
       if (n_seg > 0) return true;
       advance();  // none of the unit's tiles are in this block
     }
@@ -320,7 +340,7 @@ struct PaWalk {
   }
   __device__ __forceinline__ bool whole() const { return first == 0 && n_seg == unit.tiles; }
   // The block that the unit's last tile is in.
-  __device__ __forceinline__ int last_block(int64_t per_block) const { return (int)((t - at + unit.tiles + kCost - 1) / per_block); }
+  __device__ __forceinline__ int last_block(int64_t per_block) const { return (int)((t - at + unit.tiles + cost - 1) / per_block); }
   __device__ __forceinline__ void advance() {
     t += weight;
     if (t >= t1) return;
@@ -329,10 +349,8 @@ struct PaWalk {
     j = 0;
     if (++h < p.c.n_kv_heads) return;
     h = 0;
-    do {
-      if (++b >= p.n) return;
-      fetch();
-    } while (n_j == 0);
+    if (++e < kPaNear) fetch();
+    else t = t1;  // not reached: see plan_tiles
   }
 };
 

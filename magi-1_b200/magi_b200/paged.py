@@ -232,9 +232,10 @@ def paged_attn(q: torch.Tensor, cache: TokenPagedKVCache, layer: int, seqs: torc
         out_t, out_h, _ = out.stride()
     lse = _empty_on(stream, (rows, heads), torch.float32, dev) if return_lse else None
     handle = cache.ctx.handle
-    nbytes = cache._attn_bytes.get((max_q, heads))
+    key = min(max_q, 33), heads  # more than 32 rows: one form
+    nbytes = cache._attn_bytes.get(key)
     if nbytes is None:
-        nbytes = cache._attn_bytes[max_q, heads] = lib.magi_paged_attn_workspace_bytes(handle, max_q, heads, cache.n_kv_heads)
+        nbytes = cache._attn_bytes[key] = lib.magi_paged_attn_workspace_bytes(handle, max_q, heads, cache.n_kv_heads)
     ws = _empty_on(stream, nbytes, torch.uint8, dev)
     p = PagedAttnParams(
         struct_size=_ATTN_BYTES, layer=layer, q=q.data_ptr(), q_stride_t=stride_t, q_stride_h=stride_h, out=out.data_ptr(),

@@ -197,6 +197,19 @@ def test_many_short_units(n, hq, hkv, q_hi, len_hi, window):
     check_attn(c, strided_bf16(cu[-1], hq, 19), rng.permutation(n).tolist(), cu, window=window)
 
 
+@pytest.mark.parametrize("n_q,hq", [(1, 6), (4, 6), (8, 6)])
+def test_one_long_sequence_among_many_short_ones(n_q, hq):
+    """A block's part then reaches hundreds of short entries, some of them without rows."""
+    rng = np.random.RandomState(n_q)
+    n = 1024
+    lens = rng.randint(n_q, 20, n).tolist()
+    rows = np.where(rng.rand(n) < 0.4, 0, n_q).tolist()
+    lens[300], rows[300] = 200000, n_q
+    c = make_cache(lens, 128, 1, seed=n_q)
+    cu = np.concatenate([[0], np.cumsum(rows)]).tolist()
+    check_attn(c, strided_bf16(cu[-1], hq, 29), list(range(n)), cu)
+
+
 @pytest.mark.parametrize("hq,hkv,n_q", [(21, 3, 2), (21, 3, 4), (21, 3, 60), (5, 1, 6), (13, 1, 11), (31, 1, 1), (31, 1, 9), (33, 1, 1), (257, 1, 3)])
 def test_groups_that_are_no_power_of_two(hq, hkv, n_q):
     c = make_cache([n_q + 150, n_q], 32, hkv, seed=hq)
