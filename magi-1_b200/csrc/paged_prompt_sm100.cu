@@ -10,11 +10,11 @@
 // shared memory, one barrier a tile.  P goes back over S in TMEM (32 keys: 8 columns of e4m3, 8 of the e5m2 residual) and is the
 // A operand of the second product from there.
 //
-// What bounds it: issue slots (58 % busy; 13.4 instructions per weight, 6.1 of them the product, the exponential, the sum and
-// the two conversions) and the latency of tensor memory between them; the tensor pipe is busy 35 %.  428 GFLOP over ragged
-// prompts 629 us, 476 GFLOP over one of 9001 tokens 649 us (734 TFLOP/s, at the power limit).  A tile's weights against the
-// reference as it stands, checked afterwards, would save the pass for the maximum, but one of 128 rows asks for a new reference
-// in most tiles: 926 us.  A unit costs about five tiles to begin and end (ragged prompts: 739 us counted as 3 tiles and with the
+// What bounds it: power on even work (476 GFLOP over one prompt of 9001 tokens: 615 us, 775 TFLOP/s, 990 W at 1.85 GHz), else
+// issue slots (58 % busy, about 13 instructions per weight) and the latency of tensor memory between them; the tensor pipe is
+// busy 35 %.  428 GFLOP over ragged prompts: 600 us (629 with products and sums one at a time instead of in pairs).  A tile's
+// weights against the reference as it stands, checked afterwards, would save the pass for the maximum, but one of 128 rows asks
+// for a new reference in most tiles: 926 us against 669 then.  A unit costs about five tiles to begin and end (ragged prompts: 739 us counted as 3 tiles and with the
 // queries split 16 rows at a time, 674 at 4, 669 at 5, 677 at 6).
 //
 //   warp 0 TMA, warp 1 UMMA issuer, warps 2, 3 idle, warps 4-19 softmax (warpgroup 2 x + half: row tile x, keys 64 half ..)
@@ -339,13 +339,16 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         const float plus = m == -INFINITY ? 0.f : kPaShift - m;
         auto weigh_keys = [&](int at) {
           uint32_t w[16];
-          float s[32], kc[kPer], bias[kPer], inv[kPer], sum[2 * kPer];
+          float s[32], kc[kPer], bias[kPer], inv[kPer];
+          uint64_t sum[kPer], kc2[kPer], bias2[kPer];
           tmem_ld32(t_s + at, reinterpret_cast<uint32_t*>(s));
           factors(at, kc, bias, inv);
 #pragma unroll
           for (int g = 0; g < kPer; ++g) {
             bias[g] += plus;
-            sum[2 * g] = sum[2 * g + 1] = 0.f;
+            sum[g] = 0;
+            kc2[g] = f2_pack(kc[g], kc[g]);
+            bias2[g] = f2_pack(bias[g], bias[g]);
           }
           tmem_wait_ld();
           auto weigh = [&](auto masked) {  // exponentials and conversions run in different pipes: four keys of each in turn
@@ -353,20 +356,25 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             for (int c = 0; c < 32; c += 4) {
               const int g = c / kGroup;
               float p[4];
+              f2_unpack(f2_fma(f2_pack(s[c], s[c + 1]), kc2[g], bias2[g]), p[0], p[1]);
+              f2_unpack(f2_fma(f2_pack(s[c + 2], s[c + 3]), kc2[g], bias2[g]), p[2], p[3]);
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                p[e] = ex2(fmaf(s[c + e], kc[g], bias[g]));
+                p[e] = ex2(p[e]);
                 if constexpr (decltype(masked)::value) p[e] = at + c + e <= last && at + c + e >= begin ? p[e] : 0.f;
               }
-              sum[2 * g] += p[0] + p[1];
-              sum[2 * g + 1] += p[2] + p[3];
+              sum[g] = f2_add(sum[g], f2_add(f2_pack(p[0], p[1]), f2_pack(p[2], p[3])));
               split_weights(p[0], p[1], p[2], p[3], &w[c / 4], &w[8 + c / 4]);
             }
           };
           if (border && mixed(at)) weigh(std::true_type());
           else weigh(std::false_type());
 #pragma unroll
-          for (int g = 0; g < kPer; ++g) l = fmaf(sum[2 * g] + sum[2 * g + 1], inv[g], l);
+          for (int g = 0; g < kPer; ++g) {
+            float a, b;
+            f2_unpack(sum[g], a, b);
+            l = fmaf(a + b, inv[g], l);
+          }
           tmem_st16(t_s + at, w);
         };
         if (!border) {
