@@ -210,6 +210,24 @@ def test_one_long_sequence_among_many_short_ones(n_q, hq):
     check_attn(c, strided_bf16(cu[-1], hq, 29), list(range(n)), cu)
 
 
+@pytest.mark.parametrize("n_q", [1, 4, 8])
+def test_much_work_and_many_short_entries(n_q):
+    """100 entries of one long sequence, the same rows, between 924 short ones: a block's part is then worth hundreds of those."""
+    import magi_b200 as mb
+    rng = np.random.RandomState(n_q)
+    lens = [131072 - 5] + rng.randint(n_q, 20, 924).tolist()
+    c = make_cache(lens, 128, 1, seed=n_q)
+    q = strided_bf16(925 * n_q, 6, 31)
+    order = np.concatenate([np.zeros(100, np.int64), np.arange(1, 925)])
+    rng.shuffle(order)
+    order[:500] = np.sort(order[:500])  # long ones in a row, and long ones apart
+    rows = (order[:, None] * n_q + np.arange(n_q)).reshape(-1)
+    got, _ = mb.paged_attn(q[torch.from_numpy(rows).cuda()], c, 0, i32(order.tolist()), i32((np.arange(1025) * n_q).tolist()), max_q=n_q)
+    ref, _, tol, _ = R.attention(R.Books(c), 0, q.double().cpu().numpy(), list(range(925)), (np.arange(926) * n_q).tolist(), 1)
+    assert status() == 0
+    assert (np.abs(got.double().cpu().numpy() - ref[rows]) <= tol[rows]).all()
+
+
 @pytest.mark.parametrize("hq,hkv,n_q", [(21, 3, 2), (21, 3, 4), (21, 3, 60), (5, 1, 6), (13, 1, 11), (31, 1, 1), (31, 1, 9), (33, 1, 1), (257, 1, 3)])
 def test_groups_that_are_no_power_of_two(hq, hkv, n_q):
     c = make_cache([n_q + 150, n_q], 32, hkv, seed=hq)
