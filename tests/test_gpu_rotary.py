@@ -121,3 +121,17 @@ def test_refusals():
         with pytest.raises(ValueError):
             bad()
     assert mb.rotary(x[:0], pos[:0], freq).shape == (0, 2, 128)
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("T,H,D,rot", [(3, 57, 72, 24), (501, 7, 40, 40), (37, 113, 96, 64), (2003, 3, 10, 6), (5000, 1, 2, 2), (1, 300, 136, 128),
+                                       (90, 11, 264, 16), (300, 5, 3, 2), (11, 2, 4096, 4096), (700, 1, 17, 0)])
+def test_walks_over_odd_shapes(layout, T, H, D, rot):
+    """Several batches per thread, steps that carry from pieces to heads to tokens, and x itself as the result."""
+    import magi_b200 as mb
+    pos = torch.arange(T, device="cuda", dtype=torch.int32) * 3
+    freq = mb.rotary_frequencies(rot)[0] if rot else torch.empty(0, dtype=torch.float64, device="cuda")
+    for dtype in HALF_STEP:
+        x = torch.randn(T, H, D, generator=torch.Generator().manual_seed(D)).to(dtype).cuda()
+        want = check(x, pos, freq, layout, 0.9)
+        assert mb.rotary(x, pos, freq, layout=layout, mscale=0.9, out=x) is x and torch.equal(x, want)
