@@ -363,6 +363,20 @@ def test_append_of_unusual_values():
     assert float(c.k_scale[0, int(c.page_table[0, 1]), 0]) == 2.0 ** 60 and float(c.v_scale[0, int(c.page_table[0, 0]), 0]) == 2.0 ** -60
 
 
+@pytest.mark.parametrize("n,at", [(1, 0), (1, 15), (9, 11), (16, 5), (17, 5)])
+def test_a_few_tokens_of_unusual_values(n, at):
+    """Calls of at most 16 tokens and just above, behind tokens that are there already."""
+    c = make_cache([at + n], 16, 2, seed=3, poison=False)
+    books = R.Books(c)
+    x = torch.randn(n, 2, 128, generator=torch.Generator().manual_seed(n + at)) * 1e4
+    x[0, 0, :4] = torch.tensor([math.nan, math.inf, -math.inf, 3.0])
+    x[-1, 1] = math.nan   # nothing finite in this row
+    k, v = x.to(torch.bfloat16).cuda(), (x * 1e-6).to(torch.bfloat16).cuda()
+    c.append(0, i32([0]), i32([at]), k, v, i32([0, n]), max_new=n)
+    books.append(0, 0, at, k.double().cpu().numpy(), v.double().cpu().numpy())
+    assert status() == 0 and books.same(c) is None, books.same(c)
+
+
 def test_rewriting_tokens_in_the_middle_keeps_their_neighbours():
     c = make_cache([50], 32, 1, seed=5, poison=False)
     books = R.Books(c)
