@@ -244,8 +244,11 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
 #pragma unroll 1
       for (int k = 0; k < n_seg; ++k, ++i, ++seen) {
         const int k0 = (unit.tile0 + first + k) * kPaTile;
-        warp_wait(&sc_full[i % L::kSlots], (uint32_t)(i / L::kSlots) & 1, abort_flag);
+        // The scores first: row tile 1 leaves short units out without waiting for their tiles, so that its slot of the scales may be
+        // more than one fill behind, which the parity does not show.  Scores of tile i are issued behind row tile 0's weights of the
+        // tile before, and row tile 0 waits for the scales of every tile: the slot is then in tile i's phase or has completed it.
         warp_wait(&s_full[x], seen & 1, abort_flag);
+        warp_wait(&sc_full[i % L::kSlots], (uint32_t)(i / L::kSlots) & 1, abort_flag);
         tc_fence_after_sync();
         const float* sc = scales + (i % L::kSlots) * 16;
         const bool tail = k0 + kPaTile > ent.len;  // keys behind the sequence's end

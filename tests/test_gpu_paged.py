@@ -689,3 +689,31 @@ def test_numbers_beyond_32_bits_do_not_wrap():
         c.append(0, i32([0]), i32([9]), k, k, i32([0, 1]), max_new=2 ** 32 + 1)
     with pytest.raises(ValueError):
         mb.paged_attn(q, c, 0, i32([0]), i32([0, 1]), max_q=2 ** 32 + 1)
+
+
+# ---------------------------------------------------------------------------------------- prompts of short and full units
+def spread_scales(c, seed, lo=-12, hi=4):
+    """Scales of V that differ from page to page by far more than the codes do."""
+    g = torch.Generator().manual_seed(seed)
+    c.v_scale.copy_(2.0 ** torch.randint(lo, hi + 1, c.v_scale.shape, generator=g).float())
+
+
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("short,full", [(10, 40), (21, 22), (6, 43)])
+def test_short_units_of_many_tiles_in_front_of_full_ones(page, short, full):
+    """A short unit (up to 128 rows) leaves the second row tile out for dozens of tiles; then comes a unit of 129 to 256 rows."""
+    pairs = 150
+    c = make_cache([3001, 611], page, 1, seed=page + short, poison=False)
+    spread_scales(c, short)
+    n_q = [short, full] * pairs
+    cu = np.concatenate([[0], np.cumsum(n_q)]).tolist()
+    check_attn(c, strided_bf16(cu[-1], 6, 37), [0, 1] * pairs, cu)
+
+
+@pytest.mark.parametrize("window", [0, 4000])
+def test_full_units_over_many_tiles(window):
+    """Units of two row tiles over 9001 keys, each split over several blocks, behind remainders of up to 128 rows."""
+    c = make_cache([9001, 9000, 5003], 32, 2, seed=41, poison=False)
+    spread_scales(c, 3, -8, -4)
+    n_q = [100, 131, 43]
+    check_attn(c, strided_bf16(sum(n_q), 12, 43), [0, 1, 2], np.concatenate([[0], np.cumsum(n_q)]).tolist(), window=window)
