@@ -16,11 +16,12 @@ constexpr int kPaTileBytes = kPaTile * kHeadDim;
 constexpr int kPromptRows = 256;               // query rows of a block in the prompt form
 constexpr int kPaNear = 128;                   // entries with rows that a block's part can reach, kept in shared memory
 constexpr int kPaSpread = 48;                  // see plan_tiles
-// P = 2^(w - reference + 5).  The reference of a row is the exact maximum when it is set and stays while no weight exceeds
-// e4m3's 448 = 2^8.8, that is until the maximum has grown 14-fold: in nearly every tile the tensor core goes on summing in
-// TMEM, and the few-row form needs one vote of the group in place of the maxima.  The residual term is e5m2, whose smallest step is 2^-16:
-// a weight is dropped only below 2^-22 of the reference, so a long tail of small weights behind one large one keeps its mass.
-constexpr float kPaShift = 5.0f, kPaLimit = 8.8f;
+// P = 2^(w - reference + 12).  The reference of a row is the exact maximum when it is set and stays while no weight exceeds
+// e5m2's 57344 = 2^15.8, that is until the maximum has grown 14-fold: in nearly every tile the tensor core goes on summing in
+// TMEM, and the few-row form needs one vote of the group in place of the maxima.  A weight is carried as three e5m2 terms (see
+// split_weights): 2^-9 of it, and e5m2's smallest step, 2^-16, leaves 2^-17, which is 2^-29 of the reference.  So a long tail of
+// small weights behind one large one keeps its mass: at 2^-20 of the largest each is still within 2^-9 of its value.
+constexpr float kPaShift = 12.0f, kPaLimit = 15.8f;
 
 struct PagedAttnKernelParams {
   PagedView c;
@@ -429,13 +430,22 @@ __device__ __forceinline__ float split_query(uint2 raw, uint32_t* hi, uint32_t* 
   return __uint_as_float((uint32_t)(127 + e) << 23);
 }
 
-// P of four keys (or rows) as e4m3 and, of what that leaves (exact in fp16), as e5m2: the upper byte of an fp16, rounded.
-__device__ __forceinline__ void split_weights(float p0, float p1, float p2, float p3, uint32_t* hi, uint32_t* lo) {
-  const uint32_t h = pack4_e4m3(p0, p1, p2, p3);
-  const __half2 d01 = __hsub2(__floats2half2_rn(p0, p1), __half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)h, __NV_E4M3)));
-  const __half2 d23 = __hsub2(__floats2half2_rn(p2, p3), __half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(h >> 16), __NV_E4M3)));
-  *hi = h;
-  *lo = __byte_perm(*reinterpret_cast<const uint32_t*>(&d01) + 0x00800080u, *reinterpret_cast<const uint32_t*>(&d23) + 0x00800080u, 0x7531);
+// P of four keys (or rows) as three e5m2 terms, each taken from what those before it left.  An e5m2 is the upper byte of an fp16:
+// the first term is cut off, which keeps NaN, the other two are rounded.  The first leaves the lower 8 of fp16's 11 bits; the
+// second rounds these at 3 bits, the third what remains, 5 bits and a sign, at 3 again: at most 2^-10 of the weight beside the
+// 2^-11 of its rounding to fp16, 2^-9.4 in all, and 2^-17 where the last step is e5m2's smallest.  Remainders are exact in fp16.
+__device__ __forceinline__ void split_weights(float p0, float p1, float p2, float p3, uint32_t* t0, uint32_t* t1, uint32_t* t2) {
+  auto half2_of = [](uint32_t w) { return *reinterpret_cast<const __half2*>(&w); };
+  auto bits_of = [](__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); };
+  const uint32_t h01 = bits_of(__floats2half2_rn(p0, p1)), h23 = bits_of(__floats2half2_rn(p2, p3));
+  const uint32_t r01 = bits_of(__hsub2(half2_of(h01), half2_of(h01 & 0xff00ff00u)));
+  const uint32_t r23 = bits_of(__hsub2(half2_of(h23), half2_of(h23 & 0xff00ff00u)));
+  const uint32_t u01 = r01 + 0x00800080u, u23 = r23 + 0x00800080u;
+  const uint32_t v01 = bits_of(__hsub2(half2_of(r01), half2_of(u01 & 0xff00ff00u))) + 0x00800080u;
+  const uint32_t v23 = bits_of(__hsub2(half2_of(r23), half2_of(u23 & 0xff00ff00u))) + 0x00800080u;
+  *t0 = __byte_perm(h01, h23, 0x7531);
+  *t1 = __byte_perm(u01, u23, 0x7531);
+  *t2 = __byte_perm(v01, v23, 0x7531);
 }
 
 // Row `key` of a V tile in shared memory: its NaN codes become zero, their places go to bits (channel c: word c / 32).

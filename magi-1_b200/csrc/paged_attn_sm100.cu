@@ -8,12 +8,12 @@
 // few instructions whether a sequence has one new token (R = 16 covers 16 query heads of a kv head) or several (R = 32).  K8
 // is the K-major A operand of the first product, V8 - stored [key][channel] - the MN-major A operand of the second.
 //
-// Precision: Q and P are carried as two terms each (value + rounding residual; two instructions that accumulate into the
-// same columns).  bf16 has 8 significant bits and two e4m3 terms hold 8, so Q loses nothing except what lies 2^-17 below
-// its row's largest entry; P is e4m3 and an e5m2 residual, off by at most 2^-4 of 2^-3 of a weight (e5m2 for its range: see
-// kPaShift).  Sums and maxima are fp32 in registers, the output accumulator fp32 in TMEM.  The V scale is folded into the
-// exponent, w = s log2e + log2(sv), and a row's reference is taken over w: then P stays within e4m3 however different the
-// pages' scales are, O needs no scale per page and the denominator adds P / sv.
+// Precision: Q is carried as two e4m3 terms, P as three e5m2 ones (value, then what is left of it, added up by the tensor core).  bf16 has 8 significant bits and two e4m3 terms hold 8, so Q loses nothing except what
+// lies 2^-17 below its row's largest entry; P is off by 2^-9 of a weight and 2^-29 of the reference at most (two terms, e4m3 and
+// e5m2, kept 2^-7 of a weight down to 2^-11 of the reference and 2^-3 below 2^-16: where one key held 95 % of the mass of 8191 and
+// its values were small, the result was off by 3.8 %).  Sums and maxima are fp32 in registers, the output accumulator fp32 in TMEM.
+// The V scale is folded into the exponent, w = s log2e + log2(sv), and a row's reference is taken over w: then P stays within
+// e5m2 however different the pages' scales are, O needs no scale per page and the denominator adds P / sv.
 //
 // Work: the 128-key tiles of all (sequence, kv head, row tile) units in a row are dealt out to the blocks in equal
 // contiguous parts, so a long sequence is split over many blocks and ragged batches balance; the lengths are read on the
@@ -48,10 +48,19 @@ struct PaShared {
   static constexpr int kGroups = R / 16;                       // of four softmax warps, 16 rows each
   static constexpr int kThreads = 64 + 128 * kGroups;
   static constexpr int kRing = 0;
-  // P, a byte per (key, row) and term, two buffers: all four share the 128-byte rows [key] of one tile (term 0 of buffer 0 and
-  // 1, then term 1 of both, 32 bytes each)
+  // P, a byte per (key, row) and term, two buffers, in tiles of 128-byte rows [key], eight pieces of 16 bytes each; the lists of
+  // channels whose V is NaN (boundary tiles) are in pieces that P leaves free.
+  //   R = 16: one tile, term t of buffer b in piece 4 b + t, the list in piece 3
+  //   R = 32: terms 0 and 1 of buffer b in pieces 4 b and 4 b + 2 of the first tile (two pieces each), term 2 in 2 b of the second,
+  //           where lists 0 and 1 are in pieces 4 and 5
+  // Terms 0 and 1 side by side are one operand of 2 R rows: with an instruction for each term (12 instead of 8 a tile) 8 sequences
+  // of 10^5 tokens took 312 us instead of 290.
   static constexpr int kP = kRing + kStages * kPaTileBytes;
-  static constexpr int kQ = kP + kPaTileBytes;                 // [2 terms][R][128 bytes]
+  static constexpr int kPTiles = R / 16;
+  static constexpr int kQ = kP + kPTiles * kPaTileBytes;       // [2 terms][R][128 bytes]
+  __host__ __device__ static constexpr int piece(int term, int buffer) {  // of 16 bytes, its tile's 1024 included
+    return R == 16 ? buffer * 4 + term : term == 2 ? kPaTileBytes / 16 + buffer * 2 : buffer * 4 + term * 2;
+  }
   static constexpr int kScales = kQ + 2 * R * 128;             // [kSlots][2][8]
   static constexpr int kMax = kScales + kSlots * 64;           // [4][R] warp maxima, and sums at a unit's end
   static constexpr int kNegM = kMax + 4 * R * 4;               // [R]
@@ -60,8 +69,9 @@ struct PaShared {
   static constexpr int kRowKeys = kRowS + 2 * R * 4;           // [2][R] the keys it sees: first one, how many
   static constexpr int kInv = kRowKeys + 2 * R * 8;            // [4][R]
   static constexpr int kAt = kInv + 4 * R * 4;                 // [4][R] where a row of the result starts
-  static constexpr int kNan = kAt + 4 * R * 8;                 // [kGroups][128][4] channels whose V is NaN (boundary tiles)
-  static constexpr int kNanAny = kNan + kGroups * kPaTile * 16;  // [4] whether a warp's keys have any
+  static constexpr int kNan = kP + (kPTiles - 1) * kPaTileBytes;  // tile of the lists
+  static constexpr int kNanPiece = R == 16 ? 3 : 4;            // the first one's piece
+  static constexpr int kNanAny = kAt + 4 * R * 8;              // [kGroups][4] whether a warp's keys have any
   static constexpr int kNear = kNanAny + kGroups * 16;         // [kPaNear] entries
   static constexpr int kStart = kNear + kPaNear * 16;
   static constexpr int kBar = kStart + 64;
@@ -69,7 +79,7 @@ struct PaShared {
   static constexpr int kMisc = kBar + kNumBars * 8;
   static constexpr int kTotal = kMisc + 16;
   static constexpr int kDynamic = kTotal + 1024;
-  static constexpr uint32_t kTmemCols = 4 * R;                 // S twice, O (the allocation is a power of two)
+  static constexpr uint32_t kTmemCols = 4 * R;                 // S twice; O of the terms 0 and 2, O of term 1
   static_assert(kDynamic * kBlocksPerSm + 1024 * kBlocksPerSm <= 233472, "blocks of an SM share its memory");
   static_assert(kStages * kPaTileBytes >= kPlanScratch, "the plan's scratch is in the ring");
 };
@@ -165,7 +175,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
     // ------------------------------------------------------------------ UMMA issuer
     if (elect_one()) {
       constexpr uint32_t idesc_s = umma_idesc(kPaTile, R, 0, 0, 0, 0);
-      constexpr uint32_t idesc_o = umma_idesc(kHeadDim, R, 0, 0, 1, 1), idesc_r = umma_idesc(kHeadDim, R, 0, 1, 1, 1);  // B e4m3, e5m2
+      constexpr uint32_t idesc_o = umma_idesc(kHeadDim, 2 * R, 0, 1, 1, 1), idesc_r = umma_idesc(kHeadDim, R, 0, 1, 1, 1);  // V is e4m3, P e5m2
       constexpr uint32_t desc_hi = (1024u >> 4) | (1u << 14) | (2u << 29);  // 1024 bytes between groups of 8 rows, 128-byte swizzle
       const uint32_t ring = (smem_u32(smem + L::kRing) >> 4) | (1u << 16);
       const uint32_t q_lo = (smem_u32(smem + L::kQ) >> 4) | (1u << 16);
@@ -182,12 +192,13 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
         if (!ok) return;
         tc_fence_after_sync();
         const uint32_t d = tmem_base + 2 * R;
-        const uint32_t a = ring + stage * (kPaTileBytes >> 4), bb = p_lo + (k & 1) * 2;
+        const uint32_t a = ring + stage * (kPaTileBytes >> 4), bb = p_lo + L::piece(0, k & 1), br = p_lo + L::piece(2, k & 1);
         if (opens) umma_ss_f8_lh<0>(d, a, bb, desc_hi, idesc_o);
         else umma_ss_f8_lh<1>(d, a, bb, desc_hi, idesc_o);
 #pragma unroll
-        for (int s = 1; s < 8; ++s)  // 32 keys per instruction; then the residual term
-          umma_ss_f8_lh<1>(d, a + (s & 3) * 256, bb + (s & 3) * 256 + (s >> 2) * 4, desc_hi, s < 4 ? idesc_o : idesc_r);
+        for (int s = 1; s < 4; ++s) umma_ss_f8_lh<1>(d, a + s * 256, bb + s * 256, desc_hi, idesc_o);  // 32 keys per instruction
+#pragma unroll
+        for (int s = 0; s < 4; ++s) umma_ss_f8_lh<1>(d, a + s * 256, br + s * 256, desc_hi, idesc_r);
         umma_commit(&o_full[k & 1]);
         umma_commit(&kv_empty[stage]);
       };
@@ -366,45 +377,56 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
           if (x > 0) {  // what has been summed so far, here and by the tensor core
             warp_wait(&o_full[(i - 1) & 1], (uint32_t)((i - 1) >> 1) & 1, abort_flag);
             tc_fence_after_sync();
-            uint32_t o[RG];
-            tmem_ld16(t_o, o);
-            tmem_wait_ld();
 #pragma unroll
             for (int r = 0; r < RG; r += 4) {
               const float4 f = f4[r / 4];
               l2[r / 2] = f2_mul(l2[r / 2], f2_pack(f.x, f.y));
               l2[r / 2 + 1] = f2_mul(l2[r / 2 + 1], f2_pack(f.z, f.w));
-              o[r] = __float_as_uint(__uint_as_float(o[r]) * f.x);
-              o[r + 1] = __float_as_uint(__uint_as_float(o[r + 1]) * f.y);
-              o[r + 2] = __float_as_uint(__uint_as_float(o[r + 2]) * f.z);
-              o[r + 3] = __float_as_uint(__uint_as_float(o[r + 3]) * f.w);
             }
-            tmem_st16(t_o, o);
+#pragma unroll 1
+            for (uint32_t t = t_o; t <= t_o + R; t += R) {
+              uint32_t o[RG];
+              tmem_ld16(t, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int r = 0; r < RG; r += 4) {
+                const float4 f = f4[r / 4];
+                o[r] = __float_as_uint(__uint_as_float(o[r]) * f.x);
+                o[r + 1] = __float_as_uint(__uint_as_float(o[r + 1]) * f.y);
+                o[r + 2] = __float_as_uint(__uint_as_float(o[r + 2]) * f.z);
+                o[r + 3] = __float_as_uint(__uint_as_float(o[r + 3]) * f.w);
+              }
+              tmem_st16(t, o);
+            }
             tmem_wait_st();
           }
         }
-        // ---- weights, their sum, and P as two e4m3 terms
-        uint32_t hi[RG / 4], lo[RG / 4];
+        // ---- weights, their sum, and P as three terms
+        uint32_t t0[RG / 4], t1[RG / 4], t2[RG / 4];
         const uint64_t inv2 = f2_pack(inv_vs, inv_vs);
 #pragma unroll
         for (int r = 0; r < RG; r += 4) {
           const float p0 = ex2(w[r]), p1 = ex2(w[r + 1]), p2 = ex2(w[r + 2]), p3 = ex2(w[r + 3]);
           l2[r / 2] = f2_fma(f2_pack(p0, p1), inv2, l2[r / 2]);
           l2[r / 2 + 1] = f2_fma(f2_pack(p2, p3), inv2, l2[r / 2 + 1]);
-          split_weights(p0, p1, p2, p3, &hi[r / 4], &lo[r / 4]);
+          split_weights(p0, p1, p2, p3, &t0[r / 4], &t1[r / 4], &t2[r / 4]);
         }
         // the buffer of tile i - 2
         if (i >= 2) warp_wait(&o_full[i & 1], (uint32_t)((i - 2) >> 1) & 1, abort_flag);
         uint8_t* pb = smem + L::kP + key * 128;
-        const int chunk = (i & 1) * 2 + g;  // 16 rows
-        *reinterpret_cast<uint4*>(pb + ((chunk ^ (key & 7)) << 4)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        *reinterpret_cast<uint4*>(pb + (((chunk + 4) ^ (key & 7)) << 4)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        auto place = [&](int term) {  // 128-byte swizzle: a row's pieces change places by the key
+          const int at = L::piece(term, i & 1) + g;
+          return reinterpret_cast<uint4*>(pb + (at >> 10) * kPaTileBytes + (((at & 7) ^ (key & 7)) << 4));
+        };
+        *place(0) = make_uint4(t0[0], t0[1], t0[2], t0[3]);
+        *place(1) = make_uint4(t1[0], t1[1], t1[2], t1[3]);
+        *place(2) = make_uint4(t2[0], t2[1], t2[2], t2[3]);
         if (tail || edge) {
           // A weight of zero does not silence a NaN: V of keys behind the end becomes zero, and NaN codes of keys that only
           // some rows see are taken out of the product and come back through the sums of the rows that do see them.  The first
           // group does that; the second can be a tile behind it, not two, so the lists go by the tile's parity.
           const int v_fill = 2 * i + 1, v_stage = v_fill % kStages, buf = i & (L::kGroups - 1);
-          uint4* nan_sh = reinterpret_cast<uint4*>(smem + L::kNan) + buf * kPaTile;
+          auto nan_of = [&](int k) { return reinterpret_cast<uint4*>(smem + L::kNan + k * 128 + (((L::kNanPiece + buf) ^ (k & 7)) << 4)); };
           volatile uint32_t* nan_any = reinterpret_cast<uint32_t*>(smem + L::kNanAny) + buf * 4;
           if (g == 0) {
             warp_wait(&kv_full[v_stage], (uint32_t)(v_fill / kStages) & 1, abort_flag);
@@ -417,7 +439,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
             if (edge) {
               uint32_t bits[4] = {0, 0, 0, 0};
               if (pos < ent.len) take_nan(vrow, key, bits);
-              nan_sh[key] = make_uint4(bits[0], bits[1], bits[2], bits[3]);
+              *nan_of(key) = make_uint4(bits[0], bits[1], bits[2], bits[3]);
               nan_any[wq] = __any_sync(0xffffffffu, (bits[0] | bits[1] | bits[2] | bits[3]) != 0);  // every lane the same
             }
           }
@@ -426,10 +448,9 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
             asm volatile("bar.sync 3, %0;" ::"n"(128 * L::kGroups) : "memory");
             if (nan_any[0] | nan_any[1] | nan_any[2] | nan_any[3]) {
               // this thread's channel: the rows that see a key whose V is NaN there
-              const uint32_t* words = reinterpret_cast<const uint32_t*>(nan_sh) + quarter;
 #pragma unroll 1
               for (int kk = 0; kk < kPaTile; ++kk) {
-                if (!(words[kk * 4] >> lane & 1u)) continue;
+                if (!(reinterpret_cast<const uint32_t*>(nan_of(kk))[quarter] >> lane & 1u)) continue;
 #pragma unroll 1
                 for (int r = 0; r < RG; ++r) {
                   const int2 k = row_keys[g * RG + r];
@@ -448,8 +469,9 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       warp_wait(&o_full[(i - 1) & 1], (uint32_t)((i - 1) >> 1) & 1, abort_flag);
       const bool ok = *abort_flag == 0;
       tc_fence_after_sync();
-      float o[RG];
+      float o[RG], o1[RG];
       tmem_ld16(t_o, reinterpret_cast<uint32_t*>(o));
+      tmem_ld16(t_o + R, reinterpret_cast<uint32_t*>(o1));
       {
         float v[RG];
 #pragma unroll
@@ -473,6 +495,8 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
       const int row = g * RG + lane;  // of lanes < RG
       const float total = lane < RG ? (max_sh[lane] + max_sh[RG + lane]) + (max_sh[2 * RG + lane] + max_sh[3 * RG + lane]) : 0.f;
       tmem_wait_ld();
+#pragma unroll
+      for (int r = 0; r < RG; ++r) o[r] += o1[r];
       if (nan_rows) {
 #pragma unroll
         for (int r = 0; r < RG; ++r)

@@ -7,8 +7,8 @@
 // A block works on 256 rows (query tokens times the heads of a kv head, flattened), two tiles of 128 that take turns on the
 // tensor core.  K and V tiles are read once for all 256 rows.  Two warpgroups share a row tile, 64 keys each (and 64 channels of
 // the result): with one, the latencies of its conversions lay open, 7000 cycles a tile.  They exchange the row maxima through
-// shared memory, one barrier a tile.  P goes back over S in TMEM (32 keys: 8 columns of e4m3, 8 of the e5m2 residual) and is the
-// A operand of the second product from there.
+// shared memory, one barrier a tile.  P goes back over S in TMEM (32 keys: 8 columns for each of its three terms) and is the A
+// operand of the second product from there.
 //
 // What bounds it: power on even work (476 GFLOP over one prompt of 9001 tokens: 615 us, 775 TFLOP/s, 990 W at 1.85 GHz), else
 // issue slots (58 % busy, about 13 instructions per weight) and the latency of tensor memory between them; the tensor pipe is
@@ -118,7 +118,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     // ------------------------------------------------------------------ UMMA issuer
     if (elect_one()) {
       constexpr uint32_t idesc_s = umma_idesc(128, kPaTile, 0, 0, 0, 0);
-      constexpr uint32_t idesc_o = umma_idesc(128, kHeadDim, 0, 0, 0, 1), idesc_r = umma_idesc(128, kHeadDim, 1, 0, 0, 1);  // A e4m3, e5m2
+      constexpr uint32_t idesc_o = umma_idesc(128, kHeadDim, 1, 0, 0, 1);  // P is e5m2, V e4m3
       constexpr uint32_t desc_hi = (1024u >> 4) | (1u << 14) | (2u << 29);  // 1024 bytes between groups of 8 rows, 128-byte swizzle
       const uint32_t ring = (smem_u32(smem + L::kRing) >> 4) | (1u << 16);
       const uint32_t q_lo = (smem_u32(smem + L::kQ) >> 4) | (1u << 16);
@@ -157,8 +157,8 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             if (k == 0) umma_ts_f8_lh<0>(d, a, b, desc_hi, idesc_o);
             else umma_ts_f8_lh<1>(d, a, b, desc_hi, idesc_o);
 #pragma unroll
-            for (int s = 1; s < 8; ++s)  // 32 keys per instruction: 8 columns of P, 32 rows of V; then the residual term
-              umma_ts_f8_lh<1>(d, a + (s & 3) * 32 + (s >> 2) * 8, b + (s & 3) * 256, desc_hi, s < 4 ? idesc_o : idesc_r);
+            for (int s = 1; s < 12; ++s)  // 32 keys per instruction: 8 columns of P, 32 rows of V; then the other two terms
+              umma_ts_f8_lh<1>(d, a + (s & 3) * 32 + (s >> 2) * 8, b + (s & 3) * 256, desc_hi, idesc_o);
             if (!more) umma_commit(&o_full[x]);
             if (x == nx - 1) umma_commit(&kv_empty[v_fill % kStages]);
             if (more) {
@@ -338,10 +338,9 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             }
           }
         }
-        // ---- weights, their sum, and P as two terms: 32 keys at the first 16 of their scores' columns
+        // ---- weights, their sum, and P as three terms: 32 keys at the first 24 of their scores' columns
         const float plus = m == -INFINITY ? 0.f : kPaShift - m;
         auto weigh_keys = [&](int at) {
-          uint32_t w[16];
           float s[32], kc[kPer], bias[kPer], inv[kPer];
           uint64_t sum[kPer], kc2[kPer], bias2[kPer];
           tmem_ld32(t_s + at, reinterpret_cast<uint32_t*>(s));
@@ -354,10 +353,11 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             bias2[g] = f2_pack(bias[g], bias[g]);
           }
           tmem_wait_ld();
+          uint32_t w[12];
           auto weigh = [&](auto masked) {  // exponentials and conversions run in different pipes: four keys of each in turn
 #pragma unroll
             for (int c = 0; c < 32; c += 4) {
-              const int g = c / kGroup;
+              const int g = c / kGroup, k4 = c / 4 & 3;
               float p[4];
               f2_unpack(f2_fma(f2_pack(s[c], s[c + 1]), kc2[g], bias2[g]), p[0], p[1]);
               f2_unpack(f2_fma(f2_pack(s[c + 2], s[c + 3]), kc2[g], bias2[g]), p[2], p[3]);
@@ -367,7 +367,12 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                 if constexpr (decltype(masked)::value) p[e] = at + c + e <= last && at + c + e >= begin ? p[e] : 0.f;
               }
               sum[g] = f2_add(sum[g], f2_add(f2_pack(p[0], p[1]), f2_pack(p[2], p[3])));
-              split_weights(p[0], p[1], p[2], p[3], &w[c / 4], &w[8 + c / 4]);
+              split_weights(p[0], p[1], p[2], p[3], &w[k4], &w[4 + k4], &w[8 + k4]);
+              if (k4 == 3) {
+                tmem_st4(t_s + at + c / 16 * 4, w);
+                tmem_st4(t_s + at + 8 + c / 16 * 4, w + 4);
+                tmem_st4(t_s + at + 16 + c / 16 * 4, w + 8);
+              }
             }
           };
           if (border && mixed(at)) weigh(std::true_type());
@@ -378,7 +383,6 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             f2_unpack(sum[g], a, b);
             l = fmaf(a + b, inv[g], l);
           }
-          tmem_st16(t_s + at, w);
         };
         if (!border) {
           weigh_keys(half * 64);
@@ -391,6 +395,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
 #pragma unroll
               for (int c = 0; c < 16; ++c) w[c] = 0;
               tmem_st16(t_s + at, w);
+              tmem_st8(t_s + at + 16, w);
             } else {
               weigh_keys(at);
             }

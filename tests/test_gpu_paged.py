@@ -717,3 +717,71 @@ def test_full_units_over_many_tiles(window):
     spread_scales(c, 3, -8, -4)
     n_q = [100, 131, 43]
     check_attn(c, strided_bf16(sum(n_q), 12, 43), [0, 1, 2], np.concatenate([[0], np.cumsum(n_q)]).tolist(), window=window)
+
+
+# ---------------------------------------------------------------------------------------- one large weight and many small ones
+# What the kernel's own roundings may do to a row with weights p relative to the row's largest (times its page's scale of V):
+# three e5m2 terms of its fp16 value leave 2^-10 of a weight at most, beside 2^-11 of the rounding to fp16, and e5m2's smallest
+# step of 2^-16 is off by 2^-17 of a reference of 2^12 at least: 2^-29.  The queries' two terms change a score by ds (see paged_ref.attention), a weight by 2 ds of
+# it; the fp32 exponent and sums by 2^-14; the result is rounded to bf16, 2^-8 of it.
+def sink_case(n, n_q, entries, level, where, seed, v_sink=0.0):
+    """`entries` entries that all are the same rows of one sequence, so that a block's part of the work is a whole unit or
+    hundreds of tiles of it: key `where` has the largest score, the others `level` nats less each, their values are 1."""
+    c = make_cache([n], 128, 1, seed=seed, poison=False)
+    ids = c.page_table[0].long()
+    c.k8.view(torch.uint8).zero_()
+    c.v8.view(torch.uint8).fill_(0x38)          # 1.0
+    c.k_scale.fill_(1.0), c.v_scale.fill_(1.0)
+    page, off = int(ids[where // 128]), where % 128
+    c.k8.view(torch.uint8)[0, page, 0, off, 0] = 0x48      # 4.0
+    c.v8.view(torch.uint8)[0, page, 0, off] = 0
+    q = torch.zeros(n_q, 6, 128, dtype=torch.bfloat16, device="cuda")
+    q[:, :, 0] = level * math.sqrt(128) / 4
+    return c, q
+
+
+@pytest.mark.parametrize("n,n_q,entries", [(8191, 1, 600), (131072, 1, 128), (8191, 4, 600), (8191, 40, 150), (40000, 40, 40)])
+def test_small_weights_keep_their_bits(n, n_q, entries):
+    import magi_b200 as mb
+    for level in (7.0, 9.5, 10.6, 12.0, 13.3, 14.7):
+        for where in (0, n // 2, n - n_q):
+            c, q = sink_case(n, n_q, entries, level, where, n_q)
+            out, lse = mb.paged_attn(q.repeat(entries, 1, 1), c, 0, i32([0] * entries), i32((np.arange(entries + 1) * n_q).tolist()), max_q=n_q)
+            score = float(q[0, 0, 0]) * 4 / math.sqrt(128)
+            seen = n - n_q + np.arange(n_q)[:, None] + 0.0      # small ones: all keys up to the row's but the large one
+            total = seen * math.exp(-score) + 1
+            want = seen * math.exp(-score) / total
+            tol = (2.0 ** -8 + 2.0 ** -10 + 2.0 ** -11 + 2.0 ** -14) * want + 2.0 ** -29 * seen / total
+            err = np.abs(out.double().cpu().numpy().reshape(entries, n_q, -1) - want)
+            assert (err <= tol).all(), (level, where, float((err / want).max()))
+            assert (np.abs(lse.double().cpu().numpy().reshape(entries, n_q, 6) - (score + np.log(total))[None]) <= 2.0 ** -16 + 2.0 ** -20 * score).all()
+    assert status() == 0
+
+
+@pytest.mark.parametrize("n,n_q,entries", [(8191, 1, 600), (60001, 1, 128), (8191, 4, 600), (8191, 40, 150)])
+@pytest.mark.parametrize("mass", [0.55, 0.95])
+def test_a_key_that_holds_most_of_the_mass(n, n_q, entries, mass):
+    """Random scores and values; the large key's own values are small, so that the result is what the small weights bring.  The
+    roundings of the weights are independent: they move a row by sqrt(sum (dp v)^2), 2^-9.4 sqrt(sum (p v)^2) at most, which is
+    2^-9.4 of the row's own size up to the spread of such sums (taken as a factor of 2), beside bf16's 2^-8; 2^-29 of the
+    reference over n keys adds 2^-29 sqrt(n) to sqrt(sum p^2) >= (1 - mass) / sqrt(n).  The queries' entries are at most 2.5 and
+    sum |k| below 120, so a score is off by ds <= 2^-17 * 2.5 * 120 / sqrt(128) = 2^-12.3, a weight by 2^-11.3 of it."""
+    import magi_b200 as mb
+    c = make_cache([n], 64, 1, seed=n_q, poison=False)
+    ids = c.page_table[0].long()
+    c.k_scale.fill_(2.0 ** -7), c.v_scale.fill_(2.0 ** -7)
+    c.k8.view(torch.uint8)[0, :, 0, :, 0] = 0
+    page, off = int(ids[0]), 5
+    c.k8.view(torch.uint8)[0, page, 0] = 0                  # the others of its page: scores of zero
+    c.k8.view(torch.uint8)[0, page, 0, off, 0] = 0x7c       # 384
+    c.k_scale[0, page, 0] = 1.0
+    c.v8.view(torch.uint8)[0, page, 0, off] = 0
+    q = (torch.randn(n_q, 6, 128, generator=torch.Generator().manual_seed(5)) * 0.5).to(torch.bfloat16).cuda()
+    others = R.attention(R.Books(c), 0, q.double().cpu().numpy() * (np.arange(128) > 0), [0], [0, n_q], 1)[1]
+    q[:, :, 0] = torch.from_numpy((others + math.log(mass / (1 - mass))) * math.sqrt(128) / 384).to(torch.bfloat16).cuda()
+    ref, ref_l, _, tol_l = R.attention(R.Books(c), 0, q.double().cpu().numpy(), [0], [0, n_q], 1)
+    out, lse = mb.paged_attn(q.repeat(entries, 1, 1), c, 0, i32([0] * entries), i32((np.arange(entries + 1) * n_q).tolist()), max_q=n_q)
+    o = out.double().cpu().numpy().reshape(entries, n_q, 6, 128)
+    rel = np.sqrt(((o - ref) ** 2).sum(-1) / (ref ** 2).sum(-1))
+    assert (rel <= 2.0 ** -8 + 2 * (2.0 ** -9.4 + 2.0 ** -11.3 + 2.0 ** -29 * n / (1 - mass))).all(), float(rel.max())
+    assert float(q.abs().max()) <= 2.5 and (np.abs(lse.double().cpu().numpy().reshape(entries, n_q, 6) - ref_l) <= tol_l).all() and status() == 0
