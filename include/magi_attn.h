@@ -393,6 +393,11 @@ MAGI_API int magi_ulysses_a2a_out(magi_ulysses* u, const void* full, void* recv,
  *   seq_lens         int32 [max_seqs]
  *   page_refs        int32 [n_pages]: sequences that hold the page, 0 = free
  *   workspace        magi_token_cache_workspace_bytes() bytes of the cache's own scratch, 16-byte aligned
+ *   page_uses        int32 [n_pages]: 4 times how often reserve has taken the page, + 1 once something has been written to it since, + 2
+ *                    once a later reserve has continued it then
+ *   scale_uses       int32 [2 (K, V), n_layers, n_pages, n_kv_heads]: the use (page_uses / 4) that the page's scale belongs to.  Where they
+ *                    differ nothing has been written to the page in that layer since reserve took it, and the scale that its last
+ *                    owner left does not count.  Both zero at first: whoever fills pages without reserve need not mind them
  * page_tokens is 16, 32, 64 or 128.  One page id names the page of that number in every layer.  Index arguments (seqs,
  * starts, ...) are int32 device arrays of n <= 1024 entries.  Calls on one cache must be stream-ordered, except that
  * appends and attention of different layers may overlap.
@@ -412,6 +417,8 @@ typedef struct {
   int32_t* seq_lens;
   int32_t* page_refs;
   void* workspace;
+  int32_t* page_uses;
+  int32_t* scale_uses;
 } magi_token_cache;
 MAGI_API int64_t magi_token_cache_workspace_bytes(int32_t n_pages);
 /* Appends room for n_new[i] tokens to sequence seqs[i]: takes the pages, advances seq_lens and writes the position of the
@@ -422,7 +429,8 @@ MAGI_API int magi_token_cache_reserve(magi_ctx* ctx, const magi_token_cache* c, 
  * entry i owns rows [cu_new[i], cu_new[i+1]), at most max_new of them (cu_new NULL: one row each), which go to positions
  * starts[i], starts[i] + 1, ... of sequence seqs[i]; a negative start skips the entry.  The scale of a (page, head) is the
  * smallest power of two that keeps its finite values within +-448; tokens that the page already holds are re-quantised
- * when it grows.  NaN stays NaN, infinities saturate.  An entry that does not lie inside its sequence, and a page that
+ * when it grows.  What one reserve gave may be appended in parts, in any order; what an earlier one gave counts
+ * as appended in every layer once it is in one.  NaN stays NaN, infinities saturate.  An entry that does not lie inside its sequence, and a page that
  * other sequences share, is left alone and sets the status word to MAGI_E_RANGE. */
 MAGI_API int magi_token_cache_append(magi_ctx* ctx, const magi_token_cache* c, int layer, const int32_t* seqs,
                                      const int32_t* starts, const int32_t* cu_new, int n, int max_new, int total_new,

@@ -19,6 +19,9 @@ struct PagedView {
   int32_t* lens;
   int32_t* refs;
   int32_t* ws;  // see paged_cache.cu
+  int32_t* uses;        // [n_pages]  use * 4 + continued * 2 + written, see paged_cache.cu
+  int32_t* k_use;       // [n_layers][n_pages][n_kv_heads]
+  int32_t* v_use;
 };
 
 // Checks a cache description and fills the view; MAGI_OK or the error that was set on ctx.

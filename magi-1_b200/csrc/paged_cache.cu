@@ -8,6 +8,12 @@
 // it can be refused as a whole, and then, where pages have to be moved, a grid that copies them.  Free pages are those with
 // a reference count of zero, lowest number first, so the same calls give the same tables every time.
 //
+// A page that changes hands keeps its old scale until something is written to it.  Each time reserve takes a page it counts a use
+// of it (page_uses), and the scale of a (layer, page, head), K and V apart, carries the use that it was set in (scale_uses): where
+// the two differ the page is still empty in that layer, and append takes the scale that the new tokens need.  So a reservation can
+// be appended in parts, and reserve writes one number per page instead of a scale per layer and head.  Tokens in front of a later
+// reservation count as there in every layer, once the page has been written to in one: hence two bits beside the count.
+//
 // workspace (int32): [0] number of moves, [1] 1 = the call was accepted, [4 .. 4 + n_pages) source of each move,
 // [4 + n_pages .. 4 + 2 n_pages) its destination, [4 + 2 n_pages .. 4 + 3 n_pages) new number of a moved page.
 #include <cuda_bf16.h>
@@ -81,6 +87,9 @@ __device__ int find_free(const int32_t* refs, int n_pages, int need, int32_t* id
   return found < need ? found : need;
 }
 
+constexpr int kWritten = 1, kContinued = 2;  // page_uses: use * 4 and these
+__device__ __forceinline__ int next_use(int uses) { return (uses & ~3) + 4; }
+
 // ------------------------------------------------------------------------------------------------ reserve
 __global__ void __launch_bounds__(kPlanThreads) reserve_kernel(const PagedView c, const int32_t* __restrict__ seqs,
                                                                const int32_t* __restrict__ n_new, int n, int32_t* __restrict__ starts,
@@ -91,7 +100,7 @@ __global__ void __launch_bounds__(kPlanThreads) reserve_kernel(const PagedView c
   const int i = threadIdx.x;
   for (int w = i; w < (c.max_seqs + 31) / 32; w += kPlanThreads) named[w] = 0;
   __syncthreads();
-  int seq = 0, len = 0, add = 0, need = 0;
+  int seq = 0, len = 0, add = 0, need = 0, tail = -1;
   bool bad = false;
   if (i < n) {
     seq = seqs[i];
@@ -106,7 +115,7 @@ __global__ void __launch_bounds__(kPlanThreads) reserve_kernel(const PagedView c
       // more than there are is as good as one more than there are (and keeps the sum over the entries within 32 bits)
       need = min(pages_of((int64_t)len + add, c.page_tokens) - pages_of(len, c.page_tokens), c.n_pages + 1);
       if (add > 0 && len % c.page_tokens) {  // the page that is continued must be this sequence's alone
-        const int tail = c.table[(int64_t)seq * c.per_row + len / c.page_tokens];
+        tail = c.table[(int64_t)seq * c.per_row + len / c.page_tokens];
         bad = tail < 0 || tail >= c.n_pages || c.refs[tail] != 1;
       }
     }
@@ -129,12 +138,14 @@ __global__ void __launch_bounds__(kPlanThreads) reserve_kernel(const PagedView c
   if (i < n) {
     starts[i] = len;
     c.lens[seq] = len + add;
+    if (tail >= 0 && c.uses[tail] & kWritten) c.uses[tail] |= kContinued;
     // few pages each (one at most for a token): the entry's own thread places them
     if (need <= 4)
       for (int k = 0; k < need; ++k) {
         const int id = ids[before + k];
         c.table[(int64_t)seq * c.per_row + pages_of(len, c.page_tokens) + k] = id;
         c.refs[id] = 1;
+        c.uses[id] = next_use(c.uses[id]);
       }
   }
   if (!__syncthreads_or(need > 4)) return;
@@ -154,6 +165,7 @@ __global__ void __launch_bounds__(kPlanThreads) reserve_kernel(const PagedView c
     const int id = ids[k];
     c.table[(int64_t)s * c.per_row + last - taken + k - prefix[lo]] = id;
     c.refs[id] = 1;
+    c.uses[id] = next_use(c.uses[id]);
   }
 }
 
@@ -294,6 +306,22 @@ __device__ void move_pages(const PagedView& c) {
   const int32_t* to = from + c.n_pages;
   const int64_t page_bytes = (int64_t)c.n_kv_heads * c.page_tokens * kHeadDim;
   const int steps = (int)((page_bytes + kMoveBytes - 1) / kMoveBytes);
+  // scales, and whether they count: a page is as written, or as empty, as the one it comes from
+  const int64_t scales = (int64_t)n_moves * 2 * c.n_layers * c.n_kv_heads;
+  for (int64_t i = (int64_t)blockIdx.x * kMoveThreads + threadIdx.x; i < scales; i += (int64_t)gridDim.x * kMoveThreads) {
+    const int h = (int)(i % c.n_kv_heads);
+    int64_t r = i / c.n_kv_heads;
+    const bool kv = r & 1;
+    r >>= 1;
+    const int layer = (int)(r % c.n_layers), k = (int)(r / c.n_layers);
+    const int64_t s = ((int64_t)layer * c.n_pages + from[k]) * c.n_kv_heads + h, d = ((int64_t)layer * c.n_pages + to[k]) * c.n_kv_heads + h;
+    float* scale = kv ? c.v_scale : c.k_scale;
+    int32_t* use = kv ? c.v_use : c.k_use;
+    const int uses_s = c.uses[from[k]], use_d = c.uses[to[k]] >> 2;
+    scale[d] = scale[s];
+    use[d] = use[s] == uses_s >> 2 ? use_d : use_d - 1;
+    if (layer == 0 && !kv && h == 0) c.uses[to[k]] = use_d << 2 | (uses_s & 3);  // the use itself stays, which others read
+  }
   const int64_t total = (int64_t)n_moves * c.n_layers * 2 * steps;
   for (int64_t u = blockIdx.x; u < total; u += gridDim.x) {
     const int step = (int)(u % steps);
@@ -314,10 +342,6 @@ __device__ void move_pages(const PagedView& c) {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       if ((int)threadIdx.x + j * kMoveThreads < left) d[threadIdx.x + j * kMoveThreads] = v[j];
-    if (step == 0) {
-      float* sc = kv ? c.v_scale : c.k_scale;
-      for (int h = threadIdx.x; h < c.n_kv_heads; h += kMoveThreads) sc[pd * c.n_kv_heads + h] = sc[ps * c.n_kv_heads + h];
-    }
   }
 }
 
@@ -445,8 +469,10 @@ __global__ void __launch_bounds__(256, 5) paged_append_kernel(const PagedView c,
   bad = bad || (int64_t)start + count > len || len > (int64_t)c.per_row << page_shift || page < 0 || page >= c.n_pages;
   const int64_t block = ((int64_t)p.layer * c.n_pages + (bad ? 0 : page)) * c.n_kv_heads + head;
   float* scale = (kv ? c.v_scale : c.k_scale) + block;
+  int32_t* scale_use = (kv ? c.v_use : c.k_use) + block;
   uint8_t* codes = (kv ? c.v8 : c.k8) + block * P * kHeadDim;
   const int refs = bad ? 0 : c.refs[page];
+  const int uses = bad ? 0 : c.uses[page], use = uses >> 2, set_in = *scale_use;
   const float stored = *scale;
   // largest finite magnitude, as bits: two at a time, and one by one only where some are not finite
   uint32_t tops = 0;
@@ -477,9 +503,10 @@ __global__ void __launch_bounds__(256, 5) paged_append_kernel(const PagedView c,
     return;
   }
   const int held = min(len - base, P);                // tokens of the sequence in the page, new ones included
-  const bool others = lo > 0 || hi < held;
+  // Tokens beside the new ones.  An empty page has none, reserved or not, but for those that an earlier reservation covers.
+  const bool others = set_in == use ? lo > 0 || hi < held : lo > 0 && uses & kContinued;
   const float before = others ? stored : 0.f;
-  __syncthreads();  // every thread has read the scale before one of them replaces it
+  __syncthreads();  // every thread has read the scale and its use before one of them replaces them
 #pragma unroll
   for (int i = 0; i < 8; ++i) top = max(top, s_top[i]);
   const int e = scale_exponent(__uint_as_float(top << 16));
@@ -487,7 +514,11 @@ __global__ void __launch_bounds__(256, 5) paged_append_kernel(const PagedView c,
   const float after = fmaxf(before, needed);
   // both are powers of two, unless the caller's memory says otherwise: then the quotient is rounded once
   const float inv = __frcp_rn(after);
-  if (threadIdx.x == 0 && after != before) *scale = after;
+  if (threadIdx.x == 0) {
+    if (after != before) *scale = after;
+    if (set_in != use) *scale_use = use;
+    if (!(uses & kWritten) && head == 0 && !kv) atomicOr(&c.uses[page], kWritten);
+  }
 #pragma unroll
   for (int i = 0; i < kSlots; ++i) {
     const int r = first + r0 + i * 16;
@@ -547,8 +578,13 @@ int paged_view(magi_ctx* ctx, const magi_token_cache* c, PagedView* v) {
     return set_err(ctx, MAGI_E_ALIGN, "token cache: k8, v8 and workspace must be 16-byte aligned");
   *v = {c->n_layers, c->n_pages, c->page_tokens, c->n_kv_heads, c->max_seqs, c->max_pages_per_seq,
         static_cast<uint8_t*>(c->k8), static_cast<uint8_t*>(c->v8), c->k_scale, c->v_scale,
-        c->page_table, c->seq_lens, c->page_refs, static_cast<int32_t*>(c->workspace)};
+        c->page_table, c->seq_lens, c->page_refs, static_cast<int32_t*>(c->workspace), c->page_uses, c->scale_uses,
+        c->scale_uses ? c->scale_uses + (int64_t)c->n_layers * c->n_pages * c->n_kv_heads : nullptr};
   return MAGI_OK;
+}
+
+static int check_uses(magi_ctx* ctx, const PagedView& v) {
+  return v.uses && v.k_use ? MAGI_OK : set_err(ctx, MAGI_E_BADARG, "token cache: null page_uses or scale_uses");
 }
 
 static int check_entries(magi_ctx* ctx, const void* a, const void* b, int n, const char* what) {
@@ -577,6 +613,7 @@ extern "C" int magi_token_cache_reserve(magi_ctx* ctx, const magi_token_cache* c
   if (int rc = check_entries(ctx, seqs, n_new, n, "token cache reserve")) return rc;
   if (n == 0) return MAGI_OK;
   if (!starts) return set_err(ctx, MAGI_E_BADARG, "token cache reserve: null starts");
+  if (int rc = check_uses(ctx, v)) return rc;
   DeviceScope dev(ctx);
   reserve_kernel<<<1, kPlanThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(v, seqs, n_new, n, starts, status_word(ctx));
   return launched(ctx, "token cache reserve");
@@ -598,6 +635,7 @@ extern "C" int magi_token_cache_append(magi_ctx* ctx, const magi_token_cache* ca
   if (!k || !v) return set_err(ctx, MAGI_E_BADARG, "token cache append: null k or v");
   if (((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) || ((k_stride_t | k_stride_h | v_stride_t | v_stride_h) & 7))
     return set_err(ctx, MAGI_E_ALIGN, "token cache append: k and v must be 16-byte aligned with strides multiples of 8 elements");
+  if (int rc = check_uses(ctx, view)) return rc;
   AppendParams p = {{static_cast<const __nv_bfloat16*>(k), static_cast<const __nv_bfloat16*>(v)}, {k_stride_t, v_stride_t},
                     {k_stride_h, v_stride_h}, seqs, starts, cu_new, n, max_new, total_new, layer};
   // pages that max_new tokens can touch, no more than a sequence can hold
@@ -619,6 +657,7 @@ extern "C" int magi_token_cache_branch(magi_ctx* ctx, const magi_token_cache* ca
   if (int rc = paged_view(ctx, cache, &v)) return rc;
   if (int rc = check_entries(ctx, src, dst, n, "token cache branch")) return rc;
   if (n == 0) return MAGI_OK;
+  if (int rc = check_uses(ctx, v)) return rc;
   DeviceScope dev(ctx);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   branch_plan_kernel<<<1, kPlanThreads, 0, st>>>(v, src, dst, n, share, status_word(ctx));
@@ -641,6 +680,7 @@ extern "C" int magi_token_cache_compact(magi_ctx* ctx, const magi_token_cache* c
   if (!ctx) return MAGI_E_BADARG;
   PagedView v;
   if (int rc = paged_view(ctx, cache, &v)) return rc;
+  if (int rc = check_uses(ctx, v)) return rc;
   DeviceScope dev(ctx);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   compact_plan_kernel<<<1, kPlanThreads, 0, st>>>(v);

@@ -102,6 +102,7 @@ class TokenCache(C.Structure):
         ("max_seqs", C.c_int32), ("max_pages_per_seq", C.c_int32),
         ("k8", C.c_void_p), ("v8", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
         ("page_table", C.c_void_p), ("seq_lens", C.c_void_p), ("page_refs", C.c_void_p), ("workspace", C.c_void_p),
+        ("page_uses", C.c_void_p), ("scale_uses", C.c_void_p),
     ]
 
 

@@ -74,6 +74,8 @@ class TokenPagedKVCache:
     together, e.g. to rewind):
       k8, v8 [n_layers, n_pages, n_kv_heads, page_tokens, 128] float8_e4m3fn; k_scale, v_scale [n_layers, n_pages, n_kv_heads]
       page_table [max_seqs, max_pages_per_seq] int32 (-1 = none); seq_lens [max_seqs] int32; page_refs [n_pages] int32
+      page_uses [n_pages] int32, scale_uses [2, n_layers, n_pages, n_kv_heads] int32: the uses that reserve made of a page, and the one its
+      scale was set in (whoever puts codes and scales back puts these back with them)
     A page id names the same page in every layer.  The index arguments of the methods are int32 tensors on the cache's
     device, at most 1024 entries, no sequence twice (attention excepted); they and the books stay as they are while a call
     that reads them runs.  A book-keeping call that cannot be served - an index out of range, a sequence named twice or longer
@@ -101,12 +103,14 @@ class TokenPagedKVCache:
         self.page_table = torch.full((self.max_seqs, self.max_pages_per_seq), -1, dtype=torch.int32, device=dev)
         self.seq_lens = torch.zeros(self.max_seqs, dtype=torch.int32, device=dev)
         self.page_refs = torch.zeros(self.n_pages, dtype=torch.int32, device=dev)
+        self.page_uses = torch.zeros(self.n_pages, dtype=torch.int32, device=dev)
+        self.scale_uses = torch.zeros((2,) + shape[:3], dtype=torch.int32, device=dev)
         self._workspace = torch.empty(lib.magi_token_cache_workspace_bytes(self.n_pages) // 4, dtype=torch.int32, device=dev)
         c = self._view = TokenCache()
         c.struct_size = C.sizeof(TokenCache)
         for name in sizes:
             setattr(c, name, getattr(self, name))
-        for name in ("k8", "v8", "k_scale", "v_scale", "page_table", "seq_lens", "page_refs"):
+        for name in ("k8", "v8", "k_scale", "v_scale", "page_table", "seq_lens", "page_refs", "page_uses", "scale_uses"):
             setattr(c, name, getattr(self, name).data_ptr())
         c.workspace = self._workspace.data_ptr()
         self._view_ref = C.byref(c)
@@ -116,7 +120,8 @@ class TokenPagedKVCache:
     def nbytes(self) -> int:
         """Bytes of device memory the cache holds."""
         return sum(t.numel() * t.element_size() for t in (self.k8, self.v8, self.k_scale, self.v_scale, self.page_table,
-                                                          self.seq_lens, self.page_refs, self._workspace))
+                                                          self.seq_lens, self.page_refs, self.page_uses, self.scale_uses,
+                                                          self._workspace))
 
     def _entries(self, t, name, n=None):
         t = _index(t, name, self.device, n)
@@ -142,7 +147,8 @@ class TokenPagedKVCache:
         at most max_new of them (cu_new None: one row each), which go to positions starts[i], starts[i]+1, ... of sequence
         seqs[i]; entries with a negative start are skipped.  The scale of a (page, head) is the smallest power of two that
         keeps its finite values within +-448 (and lies in [2^-60, 2^60]); tokens already in the page are re-quantised when
-        it grows.  Positions outside the sequence, and pages that other sequences share, are left alone: status E_RANGE."""
+        it grows.  What one reserve gave may be appended in parts, in any order; what an earlier one gave counts as appended
+        in every layer once it is in one.  Positions outside the sequence, and pages that other sequences share, are left alone: status E_RANGE."""
         seqs = self._entries(seqs, "seqs")
         starts = self._entries(starts, "starts", seqs.shape[0])
         _rows(k, "k", self.device, self.n_kv_heads), _rows(v, "v", self.device, self.n_kv_heads)

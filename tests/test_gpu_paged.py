@@ -785,3 +785,101 @@ def test_a_key_that_holds_most_of_the_mass(n, n_q, entries, mass):
     rel = np.sqrt(((o - ref) ** 2).sum(-1) / (ref ** 2).sum(-1))
     assert (rel <= 2.0 ** -8 + 2 * (2.0 ** -9.4 + 2.0 ** -11.3 + 2.0 ** -29 * n / (1 - mass))).all(), float(rel.max())
     assert float(q.abs().max()) <= 2.5 and (np.abs(lse.double().cpu().numpy().reshape(entries, n_q, 6) - ref_l) <= tol_l).all() and status() == 0
+
+
+# ---------------------------------------------------------------------------------------- reservations appended in parts
+@pytest.mark.parametrize("page", [16, 64, 128])
+@pytest.mark.parametrize("parts", [[(0, 24), (24, 32)], [(0, 1), (1, 2), (2, 200)], [(100, 180), (0, 100)], [(17, 40), (60, 75), (0, 17), (40, 60), (75, 80)]])
+def test_a_reservation_appended_in_parts(page, parts):
+    """Pages whose last owner left scales of 2^40 behind take the scale of what is appended now, in any order of the parts, and
+    layer by layer."""
+    import magi_b200 as mb
+    hkv, layers, total = 2, 2, max(b for _, b in parts)
+    c = mb.TokenPagedKVCache(layers, 40, page, hkv, 4, 20)
+    big = torch.full((300, hkv, 128), 2.0 ** 40, device="cuda").to(torch.bfloat16)
+    c.reserve(i32([3]), i32([300]))
+    for layer in range(layers):
+        c.append(layer, i32([3]), i32([0]), big, big, i32([0, 300]), max_new=300)
+    c.free(i32([3]))
+    start = 5
+    assert c.reserve(i32([1]), i32([start])).tolist() == [0]
+    g = torch.Generator().manual_seed(page)
+    k, v = [(torch.randn(start + total, hkv, 128, generator=g) * torch.exp(torch.randn(start + total, 1, 1, generator=g))).to(torch.bfloat16).cuda() for _ in range(2)]
+    for layer in range(layers):
+        c.append(layer, i32([1]), i32([0]), k[:start], v[:start], i32([0, start]), max_new=start)
+    assert c.reserve(i32([1]), i32([total])).tolist() == [start]
+    for layer in range(layers):
+        books = R.Books(c)
+        for s in (books.ks, books.vs):
+            s[layer, books.table[1][1 if start % page else 0:]] = 2.0 ** -60   # pages that nothing has been written to
+        for a, b in parts:
+            c.append(layer, i32([1]), i32([start + a]), k[start + a:start + b], v[start + a:start + b], i32([0, b - a]), max_new=b - a)
+            books.append(layer, 1, start + a, *[t[start + a:start + b].double().cpu().numpy() for t in (k, v)])
+        got = R.Books(c)
+        for name in ("k8", "v8", "ks", "vs"):
+            for slot, p in enumerate(books.table[1]):
+                held = min(start + total - slot * page, page)
+                a, b = getattr(books, name)[layer, p], getattr(got, name)[layer, p]
+                if name[1] == "8":
+                    a, b = a[:, :held], b[:, :held]
+                assert np.array_equal(a, b), (layer, name, slot)
+        for h in range(hkv):
+            gk, gv = got.kv(layer, 1, h)
+            for x, y in ((gk, k), (gv, v)):
+                y = y[:, h].double().cpu().numpy()
+                # a code is off by 2^-4 of its value, or 2^-10 of the page's scale, each time it is rounded (part by part)
+                top = np.concatenate([np.full((min(page, len(y) - at), 1), np.abs(y[at:at + page]).max()) for at in range(0, len(y), page)])
+                assert (np.abs(x - y) <= 2.0 ** -4 * np.abs(y) * (1 + 2.0 ** -3) + len(parts) * 2.0 ** -10 * top * 2 / 224).all()
+    assert status() == 0
+
+
+@pytest.mark.parametrize("how", ["fork", "copy", "compact"])
+def test_pages_that_move_before_they_are_written(how):
+    """A page that is reserved, not yet written, and then copied or moved takes no scale from its past either."""
+    import magi_b200 as mb
+    page = 32
+    c = mb.TokenPagedKVCache(1, 12, page, 1, 4, 6)
+    big = torch.full((12 * page, 1, 128), 2.0 ** 40, device="cuda").to(torch.bfloat16)
+    c.reserve(i32([3, 2]), i32([6 * page, 6 * page]))
+    c.append(0, i32([3, 2]), i32([0, 0]), big, big, i32([0, 6 * page, 12 * page]), max_new=6 * page)
+    c.free(i32([3, 2]))
+    if how == "compact":
+        c.reserve(i32([3]), i32([2 * page]))   # in front, and gone before the move
+    x = torch.randn(page + 20, 1, 128, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).cuda()
+    c.reserve(i32([0]), i32([page + 20]))
+    c.append(0, i32([0]), i32([0]), x[:page], x[:page], i32([0, page]), max_new=page)   # its first page only
+    row = 0
+    if how == "compact":
+        c.free(i32([3]))
+        c.compact()
+    else:
+        getattr(c, how)(i32([0]), i32([1]))
+        row = 1
+    for a, b in ((page, page + 8), (page + 8, page + 20)):
+        c.append(0, i32([row]), i32([a]), x[a:b], x[a:b], i32([0, b - a]), max_new=b - a)
+    assert status() == 0
+    got = R.Books(c)
+    k, v = got.kv(0, row, 0)
+    want = x[:, 0].double().cpu().numpy()
+    for t in (k, v):   # the scale is at most 2^-6 (values below 7): codes are off by 2^-4 of a value or half a step, 2^-10, of it
+        assert (np.abs(t - want) <= 2.0 ** -4 * np.abs(want) + 2 * 2.0 ** -16).all()
+
+
+def test_two_reservations_appended_the_later_one_first():
+    import magi_b200 as mb
+    c = mb.TokenPagedKVCache(2, 2, 32, 1, 2, 2)
+    big = torch.full((64, 1, 128), 2.0 ** 40, device="cuda").to(torch.bfloat16)
+    c.reserve(i32([1]), i32([64]))
+    for layer in range(2):
+        c.append(layer, i32([1]), i32([0]), big, big, i32([0, 64]), max_new=64)
+    c.free(i32([1]))
+    x = torch.randn(30, 1, 128, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16).cuda()
+    c.reserve(i32([0]), i32([20]))
+    c.reserve(i32([0]), i32([10]))
+    for layer, parts in enumerate((((20, 30), (0, 20)), ((0, 20), (20, 30)))):   # the second layer in order: the page is continued by then
+        for a, b in parts:
+            c.append(layer, i32([0]), i32([a]), x[a:b], x[a:b], i32([0, b - a]), max_new=b - a)
+        for t in R.Books(c).kv(layer, 0, 0):
+            want = x[:, 0].double().cpu().numpy()
+            assert (np.abs(t - want) <= 2.0 ** -4 * np.abs(want) + 2 * 2.0 ** -16).all()
+    assert status() == 0

@@ -167,3 +167,14 @@ def test_the_reference_quantiser_agrees_with_torch():
     y = np.concatenate([pos, ties, np.nextafter(ties, 0), np.nextafter(ties, 1e9), -ties, [0.0, 2.0 ** -10, 1e-30, 460.0]])
     y = y[np.abs(y) <= 448].astype(np.float32)
     assert np.array_equal(torch.from_numpy(y).to(torch.float8_e4m3fn).view(torch.uint8).numpy(), R.to_code(y.astype(np.float64)))
+
+
+def test_a_cache_without_its_use_counts_is_refused():
+    for missing in ("page_uses", "scale_uses"):
+        c, x = cache(page_uses=4096, scale_uses=4096), ctx()
+        setattr(c, missing, None)
+        assert L.lib.magi_token_cache_reserve(C.byref(x), C.byref(c), 4096, 4096, 1, 4096, None) == E_BADARG
+        assert L.lib.magi_token_cache_append(C.byref(x), C.byref(c), 0, 4096, 4096, None, 1, 1, 1, 4096, 256, 128, 4096, 256, 128, None) == E_BADARG
+        assert L.lib.magi_token_cache_branch(C.byref(x), C.byref(c), 4096, 4096, 1, 1, None) == E_BADARG
+        assert L.lib.magi_token_cache_compact(C.byref(x), C.byref(c), None) == E_BADARG
+        assert b"uses" in x.err
