@@ -99,6 +99,12 @@ __device__ __forceinline__ PaEntry load_entry(const PagedAttnKernelParams& p, in
   return e;
 }
 
+// First position that a row at `pos` sees.  Rows in front of a sequence have negative positions, and a window may be as large as
+// 32 bits hold: nothing is subtracted that could wrap.
+__device__ __forceinline__ int window_begin(const PagedAttnKernelParams& p, int pos) {
+  return p.window > 0 && pos >= p.window ? pos - p.window + 1 : 0;
+}
+
 // Row tile j of an entry: query rows (token, head of the group) flattened, kRows at a time.
 struct PaUnit {
   int first, rows;      // flattened rows [first, first + rows)
@@ -113,7 +119,7 @@ __device__ __forceinline__ int unit_tiles(const PagedAttnKernelParams& p, const 
   const int pos_a = e.len - e.n_q + by_group(p, first);
   const int pos_z = e.len - e.n_q + by_group(p, first + rows - 1);
   const int end = p.causal ? pos_z + 1 : e.len;
-  const int begin = p.window > 0 ? max(0, pos_a - p.window + 1) : 0;
+  const int begin = window_begin(p, pos_a);
   int tile0 = 0, tiles = 1;
   if (end > begin) {
     tile0 = begin / kPaTile;

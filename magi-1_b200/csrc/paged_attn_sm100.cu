@@ -278,7 +278,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
           *reinterpret_cast<uint32_t*>(to) = hi;
           *reinterpret_cast<uint32_t*>(to + R * 128) = lo;
           row_s[r] = scale * p.scale_log2;  // every lane the same
-          const int at = ent.len - ent.n_q + toks[x], from = p.window > 0 ? max(at - p.window + 1, 0) : 0;
+          const int at = ent.len - ent.n_q + toks[x], from = window_begin(p, at);
           row_keys[r] = make_int2(from, max((p.causal ? min(at + 1, ent.len) : ent.len) - from, 0));
         }
       }
@@ -299,7 +299,7 @@ paged_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
         warp_wait(&s_full[i & 1], (uint32_t)(i >> 1) & 1, abort_flag);
         const bool tail = k0 + kPaTile > ent.len;                                             // keys behind the sequence's end
         // keys before it that not every row sees
-        const bool edge = (p.causal && min(k0 + kPaTile, ent.len) - 1 > unit.pos_a) || (p.window > 0 && k0 <= unit.pos_z - p.window);
+        const bool edge = (p.causal && min(k0 + kPaTile, ent.len) - 1 > unit.pos_a) || k0 < window_begin(p, unit.pos_z);
         tc_fence_after_sync();
         const uint32_t t_s = tmem_base + lane_base + (i & 1) * R + g * RG;
         float w[RG];  // exponents of the weights: s log2e + log2(sv) - reference + kPaShift

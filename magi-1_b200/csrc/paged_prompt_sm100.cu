@@ -237,7 +237,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
       warp_arrive(&q_full[x]);
       warp_wait(&q_full[x], units & 1, abort_flag);  // the other half's row scales
       const float c1 = row_s[row] * p.scale_log2;
-      const int at_pos = ent.len - ent.n_q + tok;
+      const int at_pos = ent.len - ent.n_q + tok, from = window_begin(p, at_pos);
       float m = -INFINITY;                  // reference maximum, at most kPaLimit - kPaShift below the running one
       float l = 0.f;                        // sum of the weights
       uint32_t nan_ch[4] = {0, 0, 0, 0};    // channels of this row that are NaN (boundary tiles)
@@ -253,10 +253,10 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         const float* sc = scales + (i % L::kSlots) * 16;
         const bool tail = k0 + kPaTile > ent.len;  // keys behind the sequence's end
         // keys before it that not every row sees
-        const bool edge = (p.causal && min(k0 + kPaTile, ent.len) - 1 > unit.pos_a) || (p.window > 0 && k0 <= unit.pos_z - p.window);
+        const bool edge = (p.causal && min(k0 + kPaTile, ent.len) - 1 > unit.pos_a) || k0 < window_begin(p, unit.pos_z);
         const bool border = __any_sync(0xffffffffu, tail || edge);  // the vote lets the branches on it be uniform ones
         const int last = min(p.causal ? at_pos : ent.len - 1, ent.len - 1) - k0;               // columns [begin, last] are seen
-        const int begin = p.window > 0 ? max(at_pos - p.window + 1 - k0, 0) : 0;
+        const int begin = max(from - k0, 0);
         // 32 keys at a time, twice over: the scores stay in TMEM in between, so that a thread holds 32 of them and not all.
         // w = s log2e + log2(sv) = raw * kc + bias; the sum adds P / sv.
         constexpr int kPer = 32 / kGroup;

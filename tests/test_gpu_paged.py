@@ -883,3 +883,15 @@ def test_two_reservations_appended_the_later_one_first():
             want = x[:, 0].double().cpu().numpy()
             assert (np.abs(t - want) <= 2.0 ** -4 * np.abs(want) + 2 * 2.0 ** -16).all()
     assert status() == 0
+
+
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 120])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("hq,n_q,n", [(6, 2, 0), (6, 2, 200), (6, 5, 1), (6, 5, 131), (6, 60, 20), (6, 300, 200), (6, 300, 300), (6, 129, 700)])
+def test_the_largest_windows_are_none(window, causal, hq, n_q, n):
+    """With more rows than keys, too, so that positions are negative; in every form."""
+    import magi_b200 as mb
+    c = make_cache([n], 64, 1, seed=n + n_q)
+    q = strided_bf16(n_q, hq, 47)
+    wide = check_attn(c, q, [0], [0, n_q], window=window, causal=causal)
+    assert np.array_equal(wide, check_attn(c, q, [0], [0, n_q], causal=causal))
