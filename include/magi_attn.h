@@ -461,7 +461,7 @@ typedef struct {
   const int32_t* seqs;           /* device int32 [n]; an entry may repeat                                */
   const int32_t* cu_q;           /* device int32 [n + 1], or NULL                                        */
   int32_t n, total_q, max_q, n_q_heads;
-  float softmax_scale;           /* <= 0: 1/sqrt(128)                                                    */
+  float softmax_scale;           /* <= 0: 1/sqrt(128); at most 2e38, no NaN                               */
   int32_t causal, window;
   void* workspace;               /* magi_paged_attn_workspace_bytes() bytes, 16-byte aligned, this call's own */
 } magi_paged_attn_params;

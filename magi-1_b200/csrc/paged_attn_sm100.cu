@@ -664,6 +664,8 @@ extern "C" int magi_paged_attn_fwd(magi_ctx* ctx, const magi_token_cache* cache,
   if (p->layer < 0 || p->layer >= k.c.n_layers) return set_err(ctx, MAGI_E_BADARG, "paged attn: no layer %d", p->layer);
   if (p->n < 0 || p->total_q < 0 || p->max_q < 0 || p->n_q_heads <= 0 || p->window < 0)
     return set_err(ctx, MAGI_E_BADARG, "paged attn: negative size");
+  if (!(p->softmax_scale <= 2e38f))  // times log2 e it has to be finite
+    return set_err(ctx, MAGI_E_BADARG, "paged attn: softmax_scale must be a number up to 2e38");
   if (p->n_q_heads % k.c.n_kv_heads) return set_err(ctx, MAGI_E_BADARG, "paged attn: n_q_heads must be a multiple of the cache's kv heads");
   if (p->n > kPgMaxEntries) return set_err(ctx, MAGI_E_NOMEM, "paged attn: more than %d entries", kPgMaxEntries);
   if (!p->cu_q && (p->max_q != 1 || p->total_q != p->n))

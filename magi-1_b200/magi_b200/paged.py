@@ -222,8 +222,12 @@ def paged_attn(q: torch.Tensor, cache: TokenPagedKVCache, layer: int, seqs: torc
     layer, window, max_q = _layer(layer, cache), int(window), int(max_q)
     if not 0 <= window <= _INT32_MAX or not 0 <= max_q <= _INT32_MAX:
         raise ValueError("window and max_q must be non-negative 32-bit numbers")
-    if softmax_scale is not None and not 0.0 < softmax_scale < math.inf:
-        raise ValueError("softmax_scale must be a positive number")
+    if softmax_scale is None:
+        scale = 0.0  # the library's default
+    else:
+        scale = C.c_float(softmax_scale).value  # as the library gets it
+        if not 0.0 < scale <= 2e38:
+            raise ValueError("softmax_scale must be a positive number that 32 bits hold, at most 2e38")
     raw = _on(stream, dev)
     rows, heads, _ = shape = q.shape
     stride_t, stride_h, _ = q.stride()
@@ -247,7 +251,7 @@ def paged_attn(q: torch.Tensor, cache: TokenPagedKVCache, layer: int, seqs: torc
         struct_size=_ATTN_BYTES, layer=layer, q=q.data_ptr(), q_stride_t=stride_t, q_stride_h=stride_h, out=out.data_ptr(),
         o_stride_t=out_t, o_stride_h=out_h, lse=lse.data_ptr() if return_lse else None, seqs=seqs.data_ptr(),
         cu_q=cu_q.data_ptr() if cu_q is not None else None, n=seqs.shape[0], total_q=rows, max_q=max_q, n_q_heads=heads,
-        softmax_scale=softmax_scale or 0.0, causal=bool(causal), window=window, workspace=ws.data_ptr())
+        softmax_scale=scale, causal=bool(causal), window=window, workspace=ws.data_ptr())
     check(lib.magi_paged_attn_fwd(handle, cache._view_ref, C.byref(p), raw), handle)
     KERNEL_LAUNCHES[0] += 2  # attention and join
     return out, lse

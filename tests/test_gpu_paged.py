@@ -895,3 +895,15 @@ def test_the_largest_windows_are_none(window, causal, hq, n_q, n):
     q = strided_bf16(n_q, hq, 47)
     wide = check_attn(c, q, [0], [0, n_q], window=window, causal=causal)
     assert np.array_equal(wide, check_attn(c, q, [0], [0, n_q], causal=causal))
+
+
+def test_a_scale_that_32_bits_do_not_hold_is_refused():
+    import magi_b200 as mb
+    c = make_cache([300], 16, 1, seed=1)
+    q = strided_bf16(1, 6, 1)
+    for scale in (1e-46, 1e-300, 3.1e38, 1e39, 1e300):
+        with pytest.raises(ValueError):
+            mb.paged_attn(q, c, 0, i32([0]), softmax_scale=scale)
+    # the smallest that it holds: every key weighs the same
+    check_attn(c, q, [0], [0, 1], softmax_scale=2.0 ** -149)
+    check_attn(c, q, [0], [0, 1], softmax_scale=2.0 ** -126)

@@ -178,3 +178,13 @@ def test_a_cache_without_its_use_counts_is_refused():
         assert L.lib.magi_token_cache_branch(C.byref(x), C.byref(c), 4096, 4096, 1, 1, None) == E_BADARG
         assert L.lib.magi_token_cache_compact(C.byref(x), C.byref(c), None) == E_BADARG
         assert b"uses" in x.err
+
+
+def test_scales_that_are_no_number_are_refused():
+    c, x = cache(), ctx()
+    for scale, code in ((math.nan, E_BADARG), (math.inf, E_BADARG), (2.5e38, E_BADARG), (2e38, 0), (1e-45, 0), (0.0, 0), (-1.0, 0), (-math.inf, 0)):
+        p = L.PagedAttnParams()
+        p.struct_size = C.sizeof(L.PagedAttnParams)
+        p.n_q_heads, p.softmax_scale = 4, scale   # no entries: nothing runs
+        p.cu_q = 4096
+        assert L.lib.magi_paged_attn_fwd(C.byref(x), C.byref(c), C.byref(p), None) == code, scale
