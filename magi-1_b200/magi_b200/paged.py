@@ -67,6 +67,46 @@ def _one_place_each(t: torch.Tensor, name: str) -> None:
             span = stride * (size - 1) + span
 
 
+def _same_view(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """b's elements are a's (b may have more rows): the strides count where there is more than one element."""
+    return a.data_ptr() == b.data_ptr() and all(n == 1 or s == t for n, s, t in zip(a.shape, a.stride(), b.stride()))
+
+
+def _reach(t: torch.Tensor) -> int:
+    """Elements from a view's first to its last, both counted."""
+    return 1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two views of one type may share memory, b one without an element twice.  Exact where their strides are the same (two
+    groups of heads of a packed tensor lie between each other); views that reach into each other with other strides count as
+    sharing."""
+    if not a.numel() or not b.numel():
+        return False
+    size = a.element_size()
+    gap = b.data_ptr() - a.data_ptr()
+    if gap >= _reach(a) * size or -gap >= _reach(b) * size:
+        return False
+    dims = [(n, m, s, t) for n, m, s, t in zip(a.shape, b.shape, a.stride(), b.stride()) if n > 1 or m > 1]
+    if gap % size or any(s != t and n > 1 and m > 1 for n, m, s, t in dims):
+        return True
+    # a's index minus b's, per dim, has to make up the gap: from the widest stride down, what the narrower ones cannot reach rules out
+    dims = sorted(((s if n > 1 else t, n, m) for n, m, s, t in dims), reverse=True)
+
+    def meets(gap, k):
+        if k == len(dims):
+            return gap == 0
+        stride, n, m = dims[k]
+        up = sum(s * (x - 1) for s, x, _ in dims[k + 1:])
+        down = sum(s * (y - 1) for s, _, y in dims[k + 1:])
+        if stride == 0:
+            return meets(gap, k + 1)
+        lo, hi = max(-((up - gap) // stride), 1 - m), min((gap + down) // stride, n - 1)
+        return any(meets(gap - d * stride, k + 1) for d in range(lo, hi + 1))
+
+    return meets(gap // size, 0)
+
+
 class TokenPagedKVCache:
     """Pages of page_tokens tokens, e4m3 codes with a power-of-two scale per (page, kv head), K and V separate.
 
@@ -209,7 +249,8 @@ def paged_attn(q: torch.Tensor, cache: TokenPagedKVCache, layer: int, seqs: torc
     positions of sequence seqs[i] - the new tokens are appended first.  Row at position p sees the cached positions <= p
     (causal) and > p - window (window > 0).  Head h reads kv head h // (Hq // n_kv_heads).  fp32 softmax; returns
     (out bf16 like q, lse fp32 [tokens, Hq] or None) as chunk_attn does.  A row that sees nothing is zero with lse -inf;
-    rows that no entry owns are left as they are in `out` (and undefined in a new one, and in lse)."""
+    rows that no entry owns are left as they are in `out` (and undefined in a new one, and in lse).  out may be q itself, or
+    memory apart from it (other heads of the same packed tensor, say)."""
     dev = cache.device
     _rows(q, "q", dev)
     seqs = cache._entries(seqs, "seqs")
@@ -239,6 +280,8 @@ def paged_attn(q: torch.Tensor, cache: TokenPagedKVCache, layer: int, seqs: torc
         if out.shape[0] < rows:
             raise ValueError("out must have at least q's rows")
         _one_place_each(out, "out")
+        if not _same_view(q, out) and _overlap(q, out):
+            raise ValueError("out may be q itself, or memory apart from it")
         out_t, out_h, _ = out.stride()
     lse = _empty_on(stream, (rows, heads), torch.float32, dev) if return_lse else None
     handle = cache.ctx.handle
@@ -306,7 +349,8 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, lay
     The first 2 * len(inv_freq) channels of every head are turned by positions[t] * inv_freq[i] (pair i) and multiplied by
     mscale, the others are copied.  layout "half" pairs channels (i, i + half), "interleaved" (2i, 2i + 1).  positions int32
     or int64 [tokens]; inv_freq fp64 (rotary_frequencies).  inverse=True turns backwards: the transposed operator, which maps
-    the gradient of the result to the gradient of x.  out may be x itself.  qk_norm_rope is the table-driven form of the DiT."""
+    the gradient of the result to the gradient of x.  out may be x itself, or memory apart from it.  qk_norm_rope is the
+    table-driven form of the DiT."""
     if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dtype not in _ROTARY_DTYPES or x.dim() != 3 or (x.shape[2] > 1 and x.stride(2) != 1):
         raise ValueError("x must be a CUDA bf16, fp16 or fp32 [tokens, heads, head_dim] tensor with a contiguous last dim")
     if layout not in ("half", "interleaved"):
@@ -324,10 +368,10 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, lay
         out = _empty_on(stream, (T, H, D), x.dtype, dev)
     elif out.device != dev or out.dtype != x.dtype or out.shape != x.shape or (D > 1 and out.stride(2) != 1):
         raise ValueError("out must have x's shape, dtype and device and a contiguous last dim")
-    elif out.data_ptr() == x.data_ptr() and out.stride() != x.stride():
-        raise ValueError("out may be x itself, not another view of its memory")
     else:
         _one_place_each(out, "out")
+        if not _same_view(x, out) and _overlap(x, out):
+            raise ValueError("out may be x itself, or memory apart from it, not another view of the same")
     if T == 0 or H == 0 or D == 0:
         return out
     (x_t, x_h, _), (out_t, out_h, _) = x.stride(), out.stride()

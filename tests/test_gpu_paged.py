@@ -907,3 +907,25 @@ def test_a_scale_that_32_bits_do_not_hold_is_refused():
     # the smallest that it holds: every key weighs the same
     check_attn(c, q, [0], [0, 1], softmax_scale=2.0 ** -149)
     check_attn(c, q, [0], [0, 1], softmax_scale=2.0 ** -126)
+
+
+def test_results_that_share_memory_with_the_queries():
+    """out may be q itself, or lie apart from it, between q's own heads too; anything else is refused."""
+    import magi_b200 as mb
+    c = make_cache([300, 5000, 77], 64, 2, seed=3)
+    for n_q in (1, 8, 70):
+        cu = [0, n_q, 2 * n_q, 3 * n_q]
+        args = (c, 0, i32([0, 1, 2]), i32(cu), n_q)
+        packed = strided_bf16(3 * n_q + 1, 8, 51).contiguous()
+        q = packed[:-1, :4]
+        want, _ = mb.paged_attn(q, *args)
+        beside, rest = packed.clone(), packed.clone()
+        got, _ = mb.paged_attn(beside[:-1, :4], *args, out=beside[:-1, 4:])
+        rest[:-1, 4:] = want
+        assert torch.equal(got, want) and torch.equal(beside, rest)
+        for bad in (packed[1:, :4], packed[:-1, 1:5], packed[:-1, 3:7], packed.view(-1, 16, 64)[:-1, ::2].as_strided((3 * n_q, 4, 128), (1024, 256, 1))):
+            with pytest.raises(ValueError):
+                mb.paged_attn(q, *args, out=bad)
+        again, _ = mb.paged_attn(q, *args, out=q)
+        assert again is q and torch.equal(q, want)
+    assert status() == 0

@@ -135,3 +135,29 @@ def test_walks_over_odd_shapes(layout, T, H, D, rot):
         x = torch.randn(T, H, D, generator=torch.Generator().manual_seed(D)).to(dtype).cuda()
         want = check(x, pos, freq, layout, 0.9)
         assert mb.rotary(x, pos, freq, layout=layout, mscale=0.9, out=x) is x and torch.equal(x, want)
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_results_that_share_memory_with_x(layout):
+    """out may be x itself, or lie apart from it, between x's own heads too; any other view of its memory is refused."""
+    import magi_b200 as mb
+    freq, _ = mb.rotary_frequencies(64)
+    pos = torch.arange(20, device="cuda")
+    packed = torch.randn(21, 6, 200, device="cuda").to(torch.bfloat16)
+    x = packed[:20, :2, :80]
+    want = mb.rotary(x, pos, freq, layout=layout)
+    for apart in (packed[:20, 2:4, :80], packed[:20, :2, 80:160], packed[:20, 4:, 100:180]):
+        keep, rest = packed.clone(), packed.clone()
+        assert torch.equal(mb.rotary(x, pos, freq, layout=layout, out=apart), want)
+        there = apart.storage_offset()
+        rest.as_strided(apart.shape, apart.stride(), there).copy_(want)
+        assert torch.equal(packed, rest)
+        packed.copy_(keep)
+    before = packed.clone()
+    for bad in (packed[1:, :2, :80], packed[:20, 1:3, :80], packed[:20, :2, 8:88], packed[:20, :2, 79:159], packed[1:, 1:3, 40:120],
+                packed.view(-1)[8:].as_strided((20, 2, 80), (160, 80, 1), 8), packed.transpose(0, 1)[:2, :20].as_strided((20, 2, 80), (200, 4200, 1), 200)):
+        with pytest.raises(ValueError):
+            mb.rotary(x, pos, freq, layout=layout, out=bad)
+    assert torch.equal(packed, before)
+    one = packed[3:4, :2, :80]   # one token: its stride says nothing
+    assert mb.rotary(one, pos[:1], freq, layout=layout, out=one) is one

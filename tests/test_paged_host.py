@@ -188,3 +188,37 @@ def test_scales_that_are_no_number_are_refused():
         p.n_q_heads, p.softmax_scale = 4, scale   # no entries: nothing runs
         p.cu_q = 4096
         assert L.lib.magi_paged_attn_fwd(C.byref(x), C.byref(c), C.byref(p), None) == code, scale
+
+
+def test_views_that_share_memory_are_told_apart():
+    """Against the sets of places themselves, for views of one buffer with the same strides; with others never too trusting."""
+    from magi_b200.paged import _one_place_each, _overlap, _same_view
+    rng = np.random.RandomState(0)
+    buf = torch.zeros(4000, dtype=torch.float16)
+    seen = {True: 0, False: 0}
+    for i in range(4000):
+        def view(shape=None, strides=None):
+            shape = shape or (int(rng.randint(1, 6)), int(rng.randint(1, 5)), int(rng.randint(1, 9)))
+            if strides is None:
+                h = int(shape[2] + rng.randint(0, 6))
+                strides = (int((shape[1] - 1) * h + shape[2] + rng.randint(0, 10)), h, 1)
+                if rng.rand() < 0.3:   # heads outside
+                    strides = (h, int((shape[0] - 1) * h + shape[2] + rng.randint(0, 10)), 1)
+            return buf.as_strided(shape, strides, int(rng.randint(0, 300)))
+        a = view()
+        same = rng.rand() < 0.7
+        b = view((int(a.shape[0] + rng.randint(0, 3)) if a.stride(0) >= a.stride(1) else a.shape[0],) + tuple(a.shape[1:]), a.stride()) if same else view(a.shape)
+        try:
+            _one_place_each(b, "b")
+        except ValueError:   # a row more than its strides have room for: refused before
+            continue
+        places = [set((t.data_ptr() + 2 * (np.arange(t.shape[0])[:, None, None] * t.stride(0) + np.arange(t.shape[1])[:, None] * t.stride(1)
+                                           + np.arange(t.shape[2]))).ravel().tolist()) for t in (a, b)]
+        real = bool(places[0] & places[1])
+        assert _overlap(a, b) == real if same else _overlap(a, b) >= real, (a.shape, a.stride(), a.storage_offset(), b.shape, b.stride(), b.storage_offset())
+        seen[real] += 1
+        if same and a.data_ptr() == b.data_ptr():
+            assert _same_view(a, b)
+    assert min(seen.values()) > 500
+    assert not _overlap(buf[:0].view(0, 1, 1), buf.view(4000, 1, 1)) and _same_view(buf[:8].view(1, 1, 8), buf.as_strided((1, 1, 8), (3, 5, 1)))
+    assert not _overlap(buf.view(4000, 1, 1), torch.zeros(4000, 1, 1, dtype=torch.float16))
