@@ -59,6 +59,8 @@ def _layer(layer, cache) -> int:
 
 def _one_place_each(t: torch.Tensor, name: str) -> None:
     """Refuse a result tensor in which two elements share memory (a broadcast view)."""
+    if t.is_contiguous():
+        return
     span = 1
     for size, stride in sorted(zip(t.shape, t.stride()), key=lambda d: d[1]):
         if size > 1:
@@ -105,6 +107,18 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
         return any(meets(gap - d * stride, k + 1) for d in range(lo, hi + 1))
 
     return meets(gap // size, 0)
+
+
+def _itself_or_apart(x: torch.Tensor, out: torch.Tensor, name: str) -> None:
+    """Refuse an `out` that shares memory with x in another way than being x.  The usual cases come first and cost little."""
+    gap = out.data_ptr() - x.data_ptr()
+    if gap == 0 and x.stride() == out.stride():
+        return
+    first = x if gap > 0 else out
+    (n, h, d), (t, s, _) = first.shape, first.stride()
+    if abs(gap) >= ((n - 1) * t + (h - 1) * s + d) * x.element_size() or _same_view(x, out) or not _overlap(x, out):
+        return
+    raise ValueError(f"out may be {name} itself, or memory apart from it, not another view of the same")
 
 
 class TokenPagedKVCache:
@@ -280,8 +294,7 @@ def paged_attn(q: torch.Tensor, cache: TokenPagedKVCache, layer: int, seqs: torc
         if out.shape[0] < rows:
             raise ValueError("out must have at least q's rows")
         _one_place_each(out, "out")
-        if not _same_view(q, out) and _overlap(q, out):
-            raise ValueError("out may be q itself, or memory apart from it")
+        _itself_or_apart(q, out, "q")
         out_t, out_h, _ = out.stride()
     lse = _empty_on(stream, (rows, heads), torch.float32, dev) if return_lse else None
     handle = cache.ctx.handle
@@ -370,8 +383,7 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, lay
         raise ValueError("out must have x's shape, dtype and device and a contiguous last dim")
     else:
         _one_place_each(out, "out")
-        if not _same_view(x, out) and _overlap(x, out):
-            raise ValueError("out may be x itself, or memory apart from it, not another view of the same")
+        _itself_or_apart(x, out, "x")
     if T == 0 or H == 0 or D == 0:
         return out
     (x_t, x_h, _), (out_t, out_h, _) = x.stride(), out.stride()
