@@ -45,11 +45,19 @@ def _index(t, name: str, device, n: Optional[int] = None) -> torch.Tensor:
     return t
 
 
+def _fit(t, name: str) -> None:
+    """The library counts in 32 bits."""
+    rows, heads, _ = t.shape
+    if rows > _INT32_MAX or heads > _INT32_MAX:
+        raise ValueError(f"{name} is beyond 32-bit sizes")
+
+
 def _rows(t, name: str, device, heads: Optional[int] = None) -> torch.Tensor:
     if not isinstance(t, torch.Tensor) or t.device != device or t.dtype != torch.bfloat16 or t.dim() != 3 or t.shape[2] != HEAD_DIM \
             or t.stride(2) != 1 or (heads is not None and t.shape[1] != heads):
         raise ValueError(f"{name} must be a bf16 [tokens, {heads if heads is not None else 'heads'}, {HEAD_DIM}] tensor on {device} "
                          "with a contiguous last dim")
+    _fit(t, name)
     return t
 
 
@@ -368,6 +376,7 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, lay
         raise ValueError("x must be a CUDA bf16, fp16 or fp32 [tokens, heads, head_dim] tensor with a contiguous last dim")
     if layout not in ("half", "interleaved"):
         raise ValueError(f"layout must be 'half' or 'interleaved', got {layout!r}")
+    _fit(x, "x")
     dev = x.device
     T, H, D = x.shape
     if not isinstance(positions, torch.Tensor) or positions.device != dev or positions.dtype not in (torch.int32, torch.int64) \

@@ -929,3 +929,15 @@ def test_results_that_share_memory_with_the_queries():
         again, _ = mb.paged_attn(q, *args, out=q)
         assert again is q and torch.equal(q, want)
     assert status() == 0
+
+
+def test_rows_beyond_32_bits_do_not_wrap():
+    import magi_b200 as mb
+    c = make_cache([10], 16, 1, seed=1)
+    before = R.Books(c)
+    k = torch.zeros(1, 1, 128, dtype=torch.bfloat16, device="cuda").expand(2 ** 32 + 1, 1, 128)
+    with pytest.raises(ValueError, match="32-bit"):
+        c.append(0, i32([0]), i32([9]), k, k, i32([0, 1]), max_new=1)
+    with pytest.raises(ValueError, match="32-bit"):
+        mb.paged_attn(k, c, 0, i32([0]), i32([0, 1]), max_q=1, out=torch.empty(1, 1, 128, dtype=torch.bfloat16, device="cuda"))
+    assert status() == 0 and before.same(c) is None

@@ -161,3 +161,13 @@ def test_results_that_share_memory_with_x(layout):
     assert torch.equal(packed, before)
     one = packed[3:4, :2, :80]   # one token: its stride says nothing
     assert mb.rotary(one, pos[:1], freq, layout=layout, out=one) is one
+
+
+def test_sizes_beyond_32_bits_do_not_wrap():
+    import magi_b200 as mb
+    none = torch.empty(0, dtype=torch.float64, device="cuda")
+    x = torch.zeros(1, 1, 1, device="cuda", dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="32-bit"):
+        mb.rotary(x.expand(1, 2 ** 32 + 3, 1), torch.zeros(1, dtype=torch.int32, device="cuda"), none)
+    with pytest.raises(ValueError, match="32-bit"):
+        mb.rotary(x.expand(2 ** 31, 1, 1), torch.zeros(1, dtype=torch.int32, device="cuda"), none)
