@@ -172,19 +172,25 @@ __device__ __forceinline__ float warp_max(float v) {
 }
 
 // A whole warp waits, its lanes staying together (the warp-wide instructions that follow need all lanes at once, and a branch
-// on the lane left lane 0 behind on its own): all ask, the warp votes.  Bounded; gives up at once where another warp did.
-__device__ __forceinline__ bool warp_wait_long(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
-  const long long t0 = clock64();
+// on the lane left lane 0 behind on its own): all ask, the warp votes.  Bounded; gives up at once where another warp did.  A warp
+// that sits out other warps' work is given the word that this work counts in: its time starts again when that moves.
+__device__ __forceinline__ bool warp_wait_long(uint64_t* bar, uint32_t parity, volatile int* abort_flag, const volatile int* progress) {
+  long long t0 = clock64();
+  int seen = 0;
   while (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) {
+    if (progress && *progress != seen) {
+      seen = *progress;
+      t0 = clock64();
+    }
     if (__any_sync(0xffffffffu, clock64() - t0 > 1000000000LL)) *abort_flag = 1;
     __syncwarp();
     if (__any_sync(0xffffffffu, *abort_flag != 0)) return false;
   }
   return true;
 }
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, const volatile int* progress = nullptr) {
   if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
-  return warp_wait_long(bar, parity, abort_flag);
+  return warp_wait_long(bar, parity, abort_flag, progress);
 }
 // One arrival for the warp, after what all its lanes did before.
 __device__ __forceinline__ void warp_arrive(uint64_t* bar) {

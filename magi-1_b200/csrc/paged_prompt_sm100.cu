@@ -73,6 +73,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
   uint64_t* drain_bar = o_full + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kMisc + 4);
+  volatile int* progress = reinterpret_cast<volatile int*>(smem + L::kMisc + 8);  // tiles whose weights are through
   PaStart* start = reinterpret_cast<PaStart*>(smem + L::kStart);
   PaEntry* near = reinterpret_cast<PaEntry*>(smem + L::kNear);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -92,6 +93,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     }
     mbar_init(drain_bar, 1);
     *abort_flag = 0;
+    *progress = 0;
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -145,6 +147,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         }
         if (ok) umma_commit(&kv_empty[(2 * i) % kStages]);
         for (int k = 0; k < walk.n_seg && ok; ++k, ++i) {
+          *progress = i;
           const bool more = k + 1 < walk.n_seg;
           const int v_fill = 2 * i + 1, k_fill = 2 * i + 2;
           ok = mbar_wait(&kv_full[v_fill % kStages], (uint32_t)(v_fill / kStages) & 1, abort_flag);
@@ -247,7 +250,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         // The scores first: row tile 1 leaves short units out without waiting for their tiles, so that its slot of the scales may be
         // more than one fill behind, which the parity does not show.  Scores of tile i are issued behind row tile 0's weights of the
         // tile before, and row tile 0 waits for the scales of every tile: the slot is then in tile i's phase or has completed it.
-        warp_wait(&s_full[x], seen & 1, abort_flag);
+        warp_wait(&s_full[x], seen & 1, abort_flag, progress);  // row tile 1 sits out any number of short units
         warp_wait(&sc_full[i % L::kSlots], (uint32_t)(i / L::kSlots) & 1, abort_flag);
         tc_fence_after_sync();
         const float* sc = scales + (i % L::kSlots) * 16;

@@ -941,3 +941,40 @@ def test_rows_beyond_32_bits_do_not_wrap():
     with pytest.raises(ValueError, match="32-bit"):
         mb.paged_attn(k, c, 0, i32([0]), i32([0, 1]), max_q=1, out=torch.empty(1, 1, 128, dtype=torch.bfloat16, device="cuda"))
     assert status() == 0 and before.same(c) is None
+
+
+def test_a_second_row_tile_that_waits_longer_than_a_wait_may_last():
+    """Every block has short units for about a second; the full unit behind them finds its second row tile still there."""
+    import magi_b200 as mb
+    n, entries, n_q = 6_000_000, 1000, 21
+    pages = -(-n // 128)
+    c = mb.TokenPagedKVCache(1, pages + 6, 128, 1, 2, pages)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    for t in (c.k8, c.v8):
+        for part in t.view(-1, 128).split(1 << 20):
+            part.copy_(torch.randn(part.shape, generator=g, device="cuda") * 60)
+    c.k_scale.fill_(2.0 ** -6), c.v_scale.fill_(2.0 ** -6)
+    assert c.reserve(i32([0, 1]), i32([n, 700])).tolist() == [0, 0]
+    cu = [n_q * i for i in range(entries + 1)] + [n_q * entries + 43]
+    q = strided_bf16(n_q, 6, 53).repeat(entries, 1, 1)
+    q = torch.cat([q, strided_bf16(43, 6, 54)])
+    args = (c, 0, i32([0] * entries + [1]), i32(cu))
+    start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    start.record()
+    out, lse = mb.paged_attn(q, *args, max_q=43)
+    end.record()
+    torch.cuda.synchronize()
+    assert status() == 0
+    assert start.elapsed_time(end) > 600, "too little work to show it"
+    for rows in (out[:-43].view(entries, n_q, 6, 128), lse[:-43].view(entries, n_q, 6)):
+        assert rows.isfinite().all()
+    assert float((lse[:-43].view(entries, n_q, 6) - lse[:n_q]).abs().max()) <= 2.0 ** -15 + 2.0 ** -19 * 20   # the same rows, in other parts
+    ids = c.page_table[1, :6].long()
+    k, v = [(t[0, ids, 0].double() * s[0, ids, 0].double()[:, None, None]).reshape(-1, 128)[:700] for t, s in ((c.k8, c.k_scale), (c.v8, c.v_scale))]
+    score = torch.einsum("thd,kd->thk", q[-43:].double(), k) / math.sqrt(128)
+    seen = torch.arange(700, device="cuda")[None, None] <= 657 + torch.arange(43, device="cuda")[:, None, None]
+    p = torch.softmax(score.masked_fill(~seen, -math.inf), -1)
+    want, size = p @ v, p @ v.abs()
+    # queries below 4.5, sum |k| below 130: ds <= 2^-17 * 4.5 * 130 / sqrt(128); 2^-9.4 of a weight, 2 ds, 2^-14: below 2^-8 in all
+    assert float(q.abs().max()) < 4.5 and float(k.abs().sum(1).max()) < 130
+    assert ((out[-43:].double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -8 * size).all()
