@@ -8,11 +8,11 @@
 // few instructions whether a sequence has one new token (R = 16 covers 16 query heads of a kv head) or several (R = 32).  K8
 // is the K-major A operand of the first product, V8 - stored [key][channel] - the MN-major A operand of the second.
 //
-// Precision: Q is carried as two e4m3 terms, P as three e5m2 ones (value, then what is left of it, added up by the tensor core).  bf16 has 8 significant bits and two e4m3 terms hold 8, so Q loses nothing except what
-// lies 2^-17 below its row's largest entry; P is off by 2^-9 of a weight and 2^-29 of the reference at most (two terms, e4m3 and
-// e5m2, kept 2^-7 of a weight down to 2^-11 of the reference and 2^-3 below 2^-16: where one key held 95 % of the mass of 8191 and
-// its values were small, the result was off by 3.8 %).  Sums and maxima are fp32 in registers, the output accumulator fp32 in TMEM.
-// The V scale is folded into the exponent, w = s log2e + log2(sv), and a row's reference is taken over w: then P stays within
+// Precision: Q is carried as two e4m3 terms, P as three e5m2 ones (value, then what is left of it, added up by the tensor core).
+// bf16 has 8 significant bits and two e4m3 terms hold 8, so Q loses nothing except what lies 2^-17 below its row's largest entry;
+// P is off by 2^-9 of a weight and 2^-29 of the reference at most (two terms, e4m3 and e5m2, kept 2^-7 of a weight down to 2^-11
+// of the reference and 2^-3 below 2^-16: a result that many small weights bring, behind one key that holds most of the mass, was
+// off by several per cent).  Sums and maxima are fp32 in registers, the output accumulator fp32 in TMEM.  The V scale is folded into the exponent, w = s log2e + log2(sv), and a row's reference is taken over w: then P stays within
 // e5m2 however different the pages' scales are, O needs no scale per page and the denominator adds P / sv.
 //
 // Work: the 128-key tiles of all (sequence, kv head, row tile) units in a row are dealt out to the blocks in equal
@@ -21,8 +21,8 @@
 // and accumulator in the workspace, and a second kernel joins them in the order of the keys (no atomics: the same bits
 // every time).
 //
-// What bounds it: HBM, once the batch fills the machine (8 sequences of 10^5 tokens, 1.9 GB: 292 us, the copy rate; 64 of
-// 300 to 8191: 98 us, of which 7 pass until the first tile is in and 3 in the join), else the latencies of one tile: plan 2 us,
+// What bounds it: HBM, once the batch fills the machine (8 sequences of 10^5 tokens, 1.9 GB: 303 us, 97 % of the copy rate;
+// 64 of 300 to 8191: 104 us, of which 7 pass until the first tile is in and 3 in the join), else the latencies of one tile: plan 2 us,
 // first tile 2, softmax and output 2, join 2.  Two blocks per SM with five stages of 16 KB: one's softmax hides behind the
 // other's loads (three with three stages: 121 us for the batch, against 108 then).
 //

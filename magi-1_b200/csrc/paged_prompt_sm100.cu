@@ -10,12 +10,14 @@
 // shared memory, one barrier a tile.  P goes back over S in TMEM (32 keys: 8 columns for each of its three terms) and is the A
 // operand of the second product from there.
 //
-// What bounds it: power on even work (476 GFLOP over one prompt of 9001 tokens: 615 us, 775 TFLOP/s, 990 W at 1.85 GHz), else
-// issue slots (58 % busy, about 13 instructions per weight) and the latency of tensor memory between them; the tensor pipe is
-// busy 35 %.  428 GFLOP over ragged prompts: 600 us (629 with products and sums one at a time instead of in pairs).  A tile's
-// weights against the reference as it stands, checked afterwards, would save the pass for the maximum, but one of 128 rows asks
-// for a new reference in most tiles: 926 us against 669 then.  A unit costs about five tiles to begin and end (ragged prompts: 739 us counted as 3 tiles and with the
-// queries split 16 rows at a time, 674 at 4, 669 at 5, 677 at 6).
+// What bounds it: issue slots (56 % busy, about 14 instructions per weight) and the latency of tensor memory between them; the
+// tensor pipe is busy 41 %, a fifth of that for the third term of P.  428 GFLOP over ragged prompts: 700 us; 996 GFLOP over one
+// prompt of 9001 tokens: 1393 us, 715 TFLOP/s.  Steps on the way, on the ragged prompts: with two terms of P, which lost the
+// weights of a long tail, 616 us, 629 with products and sums one at a time instead of in pairs; the third term with P stored 24
+// words at a time (spills) 741, four at a time 684.  A tile's weights against the reference as it stands, checked afterwards, would
+// save the pass for the maximum, but one of 128 rows asks for a new reference in most tiles: 926 us against 669 then.  A unit
+// costs about five tiles to begin and end (739 us counted as 3 tiles and with the queries split 16 rows at a time, 674 at 4, 669
+// at 5, 677 at 6).
 //
 //   warp 0 TMA, warp 1 UMMA issuer, warps 2, 3 idle, warps 4-19 softmax (warpgroup 2 x + half: row tile x, keys 64 half ..)
 //   TMEM columns: S of row tile 0, 1 at 0, 128; O at 256, 384

@@ -5,7 +5,8 @@
 // fraction of a turn before it becomes fp32: at position 10^6 a 32-bit product alone would be 0.03 radians off) and applies
 // them to every head.  What takes time beside the memory is instructions: threads walk over their pieces by adding steps,
 // without a division, and 16-bit results are rounded two at a time.  21600 x 24 x 128: bf16 49 us (5.4 TB/s), fp32 86 us
-// (6.2 TB/s).
+// (6.2 TB/s).  Off the 16-byte grid elements move one at a time: the same sizes from an odd start 139 and 143 us, 21600 x 24 x 96
+// with 50 channels turned 130 and 134 us.
 #include <algorithm>
 #include <type_traits>
 

@@ -133,7 +133,8 @@ class TokenPagedKVCache:
     """Pages of page_tokens tokens, e4m3 codes with a power-of-two scale per (page, kv head), K and V separate.
 
     Device state, all of it plain tensors that may be read at any time (and saved and put back with copy_, all three books
-    together, e.g. to rewind):
+    together, to rewind all sequences at once; a page keeps the scale that it had grown to.  A length alone is not to be changed:
+    the pages behind it would stay taken):
       k8, v8 [n_layers, n_pages, n_kv_heads, page_tokens, 128] float8_e4m3fn; k_scale, v_scale [n_layers, n_pages, n_kv_heads]
       page_table [max_seqs, max_pages_per_seq] int32 (-1 = none); seq_lens [max_seqs] int32; page_refs [n_pages] int32
       page_uses [n_pages] int32, scale_uses [2, n_layers, n_pages, n_kv_heads] int32: the uses that reserve made of a page, and the one its
@@ -272,7 +273,7 @@ def paged_attn(q: torch.Tensor, cache: TokenPagedKVCache, layer: int, seqs: torc
     (causal) and > p - window (window > 0).  Head h reads kv head h // (Hq // n_kv_heads).  fp32 softmax; returns
     (out bf16 like q, lse fp32 [tokens, Hq] or None) as chunk_attn does.  A row that sees nothing is zero with lse -inf;
     rows that no entry owns are left as they are in `out` (and undefined in a new one, and in lse).  out may be q itself, or
-    memory apart from it (other heads of the same packed tensor, say)."""
+    memory apart from it (other heads of the same packed tensor, say).  There is no backward pass: the result carries no graph."""
     dev = cache.device
     _rows(q, "q", dev)
     seqs = cache._entries(seqs, "seqs")
@@ -370,8 +371,8 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, lay
     The first 2 * len(inv_freq) channels of every head are turned by positions[t] * inv_freq[i] (pair i) and multiplied by
     mscale, the others are copied.  layout "half" pairs channels (i, i + half), "interleaved" (2i, 2i + 1).  positions int32
     or int64 [tokens]; inv_freq fp64 (rotary_frequencies).  inverse=True turns backwards: the transposed operator, which maps
-    the gradient of the result to the gradient of x.  out may be x itself, or memory apart from it.  qk_norm_rope is the
-    table-driven form of the DiT."""
+    the gradient of the result to the gradient of x.  out may be x itself, or memory apart from it.  No graph is
+    recorded: a training step makes the inverse call itself.  qk_norm_rope is the table-driven form of the DiT."""
     if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dtype not in _ROTARY_DTYPES or x.dim() != 3 or (x.shape[2] > 1 and x.stride(2) != 1):
         raise ValueError("x must be a CUDA bf16, fp16 or fp32 [tokens, heads, head_dim] tensor with a contiguous last dim")
     if layout not in ("half", "interleaved"):
