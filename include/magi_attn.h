@@ -448,7 +448,8 @@ MAGI_API int magi_token_cache_compact(magi_ctx* ctx, const magi_token_cache* c, 
 /* Attention over the token-paged cache, for one new token per sequence up to whole prompts.  Query row r of sequence
  * entry i (rows [cu_q[i], cu_q[i+1]) of q, at most max_q; cu_q NULL: one row each) stands at position
  * p = seq_lens[seqs[i]] - n_q + r and sees the cached positions < seq_lens that are <= p (causal) and > p - window
- * (window > 0): out = softmax(scale q k^T) v in fp32, head h reading kv head h / (n_q_heads / n_kv_heads).  A row that sees
+ * (window > 0): out = softmax(scale q k^T) v in fp32, head h reading kv head h / (n_q_heads / n_kv_heads).  The weights of v
+ * are held to 2^-9.4 of each, and to 2^-29 of the row's largest product of a weight and its page's v_scale.  A row that sees
  * nothing is zero with lse = -inf; rows of q that no entry owns are not written. */
 typedef struct {
   uint32_t struct_size;

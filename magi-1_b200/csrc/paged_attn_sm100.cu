@@ -10,9 +10,10 @@
 //
 // Precision: Q is carried as two e4m3 terms, P as three e5m2 ones (value, then what is left of it, added up by the tensor core).
 // bf16 has 8 significant bits and two e4m3 terms hold 8, so Q loses nothing except what lies 2^-17 below its row's largest entry;
-// P is off by 2^-9 of a weight and 2^-29 of the reference at most (two terms, e4m3 and e5m2, kept 2^-7 of a weight down to 2^-11
-// of the reference and 2^-3 below 2^-16: a result that many small weights bring, behind one key that holds most of the mass, was
-// off by several per cent).  Sums and maxima are fp32 in registers, the output accumulator fp32 in TMEM.  The V scale is folded into the exponent, w = s log2e + log2(sv), and a row's reference is taken over w: then P stays within
+// P is off by 2^-9 of a weight and 2^-29 of the reference at most, V's scale included (two terms, e4m3 and e5m2, kept 2^-7 of a
+// weight down to 2^-11 of the reference and 2^-3 below 2^-16: a result that many small weights bring, behind one key that holds
+// most of the mass, was off by several per cent).  Sums and maxima are fp32 in registers, the output accumulator fp32 in TMEM.
+// The V scale is folded into the exponent, w = s log2e + log2(sv), and a row's reference is taken over w: then P stays within
 // e5m2 however different the pages' scales are, O needs no scale per page and the denominator adds P / sv.
 //
 // Work: the 128-key tiles of all (sequence, kv head, row tile) units in a row are dealt out to the blocks in equal

@@ -270,7 +270,8 @@ def paged_attn(q: torch.Tensor, cache: TokenPagedKVCache, layer: int, seqs: torc
 
     Entry i owns query rows cu_q[i]:cu_q[i+1], at most max_q of them (cu_q None: one row each), which stand at the last
     positions of sequence seqs[i] - the new tokens are appended first.  Row at position p sees the cached positions <= p
-    (causal) and > p - window (window > 0).  Head h reads kv head h // (Hq // n_kv_heads).  fp32 softmax; returns
+    (causal) and > p - window (window > 0).  Head h reads kv head h // (Hq // n_kv_heads).  fp32 softmax, the
+    weights of V held to 2^-9.4 of each and 2^-29 of the row's largest product of a weight and its page's v_scale; returns
     (out bf16 like q, lse fp32 [tokens, Hq] or None) as chunk_attn does.  A row that sees nothing is zero with lse -inf;
     rows that no entry owns are left as they are in `out` (and undefined in a new one, and in lse).  out may be q itself, or
     memory apart from it (other heads of the same packed tensor, say).  There is no backward pass: the result carries no graph."""

@@ -724,28 +724,31 @@ def test_full_units_over_many_tiles(window):
 # three e5m2 terms of its fp16 value leave 2^-10 of a weight at most, beside 2^-11 of the rounding to fp16, and e5m2's smallest
 # step of 2^-16 is off by 2^-17 of a reference of 2^12 at least: 2^-29.  The queries' two terms change a score by ds (see paged_ref.attention), a weight by 2 ds of
 # it; the fp32 exponent and sums by 2^-14; the result is rounded to bf16, 2^-8 of it.
-def sink_case(n, n_q, entries, level, where, seed, v_sink=0.0):
-    """`entries` entries that all are the same rows of one sequence, so that a block's part of the work is a whole unit or
-    hundreds of tiles of it: key `where` has the largest score, the others `level` nats less each, their values are 1."""
+def flat_cache(n, seed):
+    """A sequence of n keys that are zero, values one."""
     c = make_cache([n], 128, 1, seed=seed, poison=False)
-    ids = c.page_table[0].long()
     c.k8.view(torch.uint8).zero_()
     c.v8.view(torch.uint8).fill_(0x38)          # 1.0
     c.k_scale.fill_(1.0), c.v_scale.fill_(1.0)
-    page, off = int(ids[where // 128]), where % 128
-    c.k8.view(torch.uint8)[0, page, 0, off, 0] = 0x48      # 4.0
-    c.v8.view(torch.uint8)[0, page, 0, off] = 0
-    q = torch.zeros(n_q, 6, 128, dtype=torch.bfloat16, device="cuda")
-    q[:, :, 0] = level * math.sqrt(128) / 4
-    return c, q
+    return c
 
 
 @pytest.mark.parametrize("n,n_q,entries", [(8191, 1, 600), (131072, 1, 128), (8191, 4, 600), (8191, 40, 150), (40000, 40, 40)])
 def test_small_weights_keep_their_bits(n, n_q, entries):
     import magi_b200 as mb
+    # `entries` entries that all are the same rows of one sequence, so that a block's part of the work is a whole unit or hundreds
+    # of tiles of it: key `where` has the largest score and no values, the others `level` nats less each
+    c = flat_cache(n, n_q)
+    ids = c.page_table[0].long()
     for level in (7.0, 9.5, 10.6, 12.0, 13.3, 14.7):
         for where in (0, n // 2, n - n_q):
-            c, q = sink_case(n, n_q, entries, level, where, n_q)
+            page, off = int(ids[where // 128]), where % 128
+            c.k8.view(torch.uint8).zero_()
+            c.v8.view(torch.uint8).fill_(0x38)
+            c.k8.view(torch.uint8)[0, page, 0, off, 0] = 0x48      # 4.0
+            c.v8.view(torch.uint8)[0, page, 0, off] = 0
+            q = torch.zeros(n_q, 6, 128, dtype=torch.bfloat16, device="cuda")
+            q[:, :, 0] = level * math.sqrt(128) / 4
             out, lse = mb.paged_attn(q.repeat(entries, 1, 1), c, 0, i32([0] * entries), i32((np.arange(entries + 1) * n_q).tolist()), max_q=n_q)
             score = float(q[0, 0, 0]) * 4 / math.sqrt(128)
             seen = n - n_q + np.arange(n_q)[:, None] + 0.0      # small ones: all keys up to the row's but the large one
@@ -978,3 +981,140 @@ def test_a_second_row_tile_that_waits_longer_than_a_wait_may_last():
     # queries below 4.5, sum |k| below 130: ds <= 2^-17 * 4.5 * 130 / sqrt(128); 2^-9.4 of a weight, 2 ds, 2^-14: below 2^-8 in all
     assert float(q.abs().max()) < 4.5 and float(k.abs().sum(1).max()) < 130
     assert ((out[-43:].double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -8 * size).all()
+
+
+# ---------------------------------------------------------------------------------------- far pages, streams, rewinding
+def test_pages_beyond_32_bits():
+    """A pool of 5 GB each for K and V in two layers, the pages in use at its far end."""
+    import magi_b200 as mb
+    page, hkv, n_pages = 128, 2, 82000
+    c = mb.TokenPagedKVCache(2, n_pages, page, hkv, 4, 40)
+    assert c.k8.numel() > 2 ** 32 + 2 ** 29
+    c.page_refs[:n_pages - 20] = 1
+    rng = np.random.RandomState(0)
+    n = [300, 1, 129]
+    starts = c.reserve(i32([0, 1, 2]), i32(n))
+    assert starts.tolist() == [0, 0, 0]
+    cu = [0, 300, 301, 430]
+    k, v = [torch.from_numpy(rng.randn(430, hkv, 128)).to(torch.bfloat16).cuda() for _ in range(2)]
+    for layer in (1, 0):
+        c.append(layer, i32([0, 1, 2]), starts, k * (layer + 1), v, i32(cu), max_new=300)
+    c.copy(i32([0]), i32([3]))
+
+    def check(rows):
+        q = strided_bf16(len(rows), 6, 61)
+        for layer in range(2):
+            out, lse = mb.paged_attn(q, c, layer, i32(rows))
+            for i, s in enumerate(rows):
+                ids = c.page_table[s, :-(-int(c.seq_lens[s]) // page)].long()
+                at = (0, 1, 2, 0)[s]
+                for h in range(hkv):
+                    kk, vv = [(t[layer, ids, h].double() * z[layer, ids, h].double()[:, None, None]).reshape(-1, 128)[:n[at]] for t, z in ((c.k8, c.k_scale), (c.v8, c.v_scale))]
+                    # what was appended, to within a code's half step
+                    want = (k * (layer + 1))[cu[at]:cu[at + 1], h].double()
+                    assert ((kk - want).abs() <= 2.0 ** -4 * want.abs() + 2.0 ** -10 * 2.0 ** -5).all()
+                    p = torch.softmax(q[i, h * 3:h * 3 + 3].double() @ kk.T / math.sqrt(128), 1)
+                    assert ((out[i, h * 3:h * 3 + 3].double() - p @ vv).abs() <= 2.0 ** -8 * (p @ vv).abs() + 2.0 ** -8 * (p @ vv.abs())).all()
+
+    check([0, 1, 2, 3])
+    c.free(i32([0]))
+    c.page_refs[:n_pages - 20] = 0
+    c.compact()
+    assert int(c.page_refs.sum()) == int((c.page_refs[:6] > 0).sum()) == 6
+    check([3, 1, 2])
+    assert status() == 0
+
+
+def test_layers_on_streams_of_their_own():
+    """Appends and attention of different layers at once, over pages whose last owner's scales were large."""
+    import magi_b200 as mb
+    layers, hkv, n = 4, 2, [700, 33, 1500]
+    cu, total = [0, 700, 733, 2233], 2233
+
+    def fresh():
+        c = mb.TokenPagedKVCache(layers, 200, 16, hkv, 4, 120)
+        big = torch.full((1900, hkv, 128), 2.0 ** 30, device="cuda").to(torch.bfloat16)
+        c.reserve(i32([3]), i32([1900]))
+        for layer in range(layers):
+            c.append(layer, i32([3]), i32([0]), big, big, i32([0, 1900]), max_new=1900)
+        c.free(i32([3]))
+        return c
+
+    g = torch.Generator(device="cuda").manual_seed(0)
+    k, v = [[torch.randn(total, hkv, 128, generator=g, device="cuda").to(torch.bfloat16) for _ in range(layers)] for _ in range(2)]
+    q = [torch.randn(total, 6, 128, generator=g, device="cuda").to(torch.bfloat16) for _ in range(layers)]
+    seqs, cus = i32([0, 1, 2]), i32(cu)
+    halves = []   # every entry in two parts
+    for j in range(2):
+        rows = [torch.arange(cu[i] + (0 if j == 0 else n[i] // 3), cu[i] + (n[i] // 3 if j == 0 else n[i])) for i in range(3)]
+        halves.append((torch.cat(rows).cuda(), i32(np.concatenate([[0], np.cumsum([len(r) for r in rows])]).tolist()), i32([0 if j == 0 else x // 3 for x in n]), max(len(r) for r in rows)))
+
+    def step(c, layer, stream):
+        for (_, cu_part, first, most), kk, vv in zip(halves, ks[layer], vs[layer]):
+            c.append(layer, seqs, first, kk, vv, cu_part, max_new=most, stream=stream)
+        return mb.paged_attn(q[layer], c, layer, seqs, cus, max_q=1500, stream=stream)
+
+    ks = [[x[at].contiguous() for at, _, _, _ in halves] for x in k]
+    vs = [[x[at].contiguous() for at, _, _, _ in halves] for x in v]
+    one = fresh()
+    one.reserve(seqs, i32(n))
+    want = [step(one, layer, None) for layer in range(layers)]
+    books = R.Books(one)
+    assert float(one.k_scale[:, one.page_table[:3][one.page_table[:3] >= 0].long()].max()) <= 2.0 ** -5
+    for _ in range(5):
+        c = fresh()
+        c.reserve(seqs, i32(n))
+        streams = [torch.cuda.Stream() for _ in range(layers)]
+        torch.cuda.synchronize()
+        got = [step(c, layer, streams[layer]) for layer in range(layers)]
+        torch.cuda.synchronize()
+        assert books.same(c) is None, books.same(c)
+        for (a, la), (b, lb) in zip(want, got):
+            assert torch.equal(a, b) and torch.equal(la, lb)
+    assert status() == 0
+
+
+def test_proposed_tokens_are_taken_back():
+    """The books put back: what was proposed is gone, pages that it took are empty again, a page that goes on keeps its scale."""
+    import magi_b200 as mb
+    page, hkv = 16, 1
+    c = mb.TokenPagedKVCache(1, 12, page, hkv, 2, 5)
+    books = R.Books(c)
+    rng = np.random.RandomState(1)
+
+    def tokens(m, size):
+        return [torch.from_numpy(rng.randn(m, hkv, 128) * size).to(torch.bfloat16).cuda() for _ in range(2)]
+
+    def add(m, size):
+        k, v = tokens(m, size)
+        start = books.reserve([0], [m])
+        assert c.reserve(i32([0]), i32([m])).tolist() == start
+        c.append(0, i32([0]), i32(start), k, v, i32([0, m]), max_new=m)
+        books.append(0, 0, start[0], k.double().cpu().numpy(), v.double().cpu().numpy())
+
+    add(13, 1.0)
+    for turn in range(4):
+        saved = [t.clone() for t in (c.page_table, c.seq_lens, c.page_refs)]
+        kept = [list(x) for x in books.table], list(books.lens), list(books.refs)
+        add(7, 2.0 ** (10 * turn))   # over the page's end: the new page takes a large scale
+        assert books.same(c) is None
+        for t, x in zip((c.page_table, c.seq_lens, c.page_refs), saved):
+            t.copy_(x)
+        books.table, books.lens, books.refs = [list(x) for x in kept[0]], list(kept[1]), list(kept[2])
+        add(7, 1.0)
+        assert books.same(c) is None, books.same(c)
+        # A weight is off by 2^-17 where it is small, the reference is 2^12 for the largest product of a weight and its page's scale
+        # of V: 2^-29 of that product, times a key's codes.  It matters here, as the page that goes on keeps a scale 2^30 too large.
+        q = strided_bf16(3, 4, turn)
+        out, lse = mb.paged_attn(q, c, 0, i32([0]), i32([0, 3]), max_q=3)
+        ref, ref_l, tol, tol_l = R.attention(books, 0, q.double().cpu().numpy(), [0], [0, 3], 1)
+        key, _ = books.kv(0, 0, 0)
+        n = books.lens[0]
+        sv = np.repeat(books.vs[0, books.table[0], 0], page)[:n]
+        codes = np.concatenate([R.CODES[books.v8[0, p, 0]] for p in books.table[0]])[:n]
+        for t in range(3):
+            seen = slice(0, n - 2 + t)
+            w = np.exp(q[t].double().cpu().numpy() @ key[seen].T / math.sqrt(128) - ref_l[t][:, None])
+            tol[t] += 2.0 ** -29 * (w * sv[seen]).max(1, keepdims=True) * np.abs(codes[seen]).sum(0)
+        assert (np.abs(out.double().cpu().numpy() - ref) <= tol).all() and (np.abs(lse.double().cpu().numpy() - ref_l) <= tol_l).all()
+    assert status() == 0
