@@ -89,7 +89,7 @@ __device__ int find_free(const int32_t* refs, int n_pages, int need, int32_t* id
 }
 
 constexpr int kWritten = 1, kContinued = 2;  // page_uses: use * 4 and these
-__device__ __forceinline__ int next_use(int uses) { return (uses & ~3) + 4; }
+__device__ __forceinline__ int next_use(int uses) { return (int)(((uint32_t)uses & ~3u) + 4u); }  // may wrap: it is only compared
 
 // ------------------------------------------------------------------------------------------------ reserve
 __global__ void __launch_bounds__(kPlanThreads) reserve_kernel(const PagedView c, const int32_t* __restrict__ seqs,
